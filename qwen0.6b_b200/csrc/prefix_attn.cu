@@ -1,0 +1,1104 @@
+// prefix_attn.cu - attention for a batch whose sequences share their first
+// pages (B200 / sm_100a).  C ABI in include/qwen_b200_paged.h.
+//
+// A row r of group g sees the group's prefix (positions 0 .. P_g - 1, the
+// same for all rows) and its own positions P_g .. len_r - 1.  With the
+// softmax statistics of the two parts,
+//   m = max_t s_t, l = sum_t 2^(s_t - m), a = sum_t 2^(s_t - m) v_t,
+//   s_t = scale log2(e) q . k_t,
+// the parts join exactly: o = sum_i a_i 2^(m_i - m) / sum_i l_i 2^(m_i - m).
+//   prefix_kernel   the shared part: the group's queries (rows x heads of a
+//                   kv head) are the rows of a matrix product, so K and V are
+//                   read once per group: tcgen05, 128 or 256 queries per CTA;
+//   own_kernel      each row's own part, a few hundred tokens read by that
+//                   row alone: bound by their bytes, mma.sync on fragments
+//                   loaded straight from global memory;
+//   join_kernel     the partial (m, l, a) of both, summed in a fixed order.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdarg.h>
+#include <stdio.h>
+#include <stdlib.h>
+
+#include <mutex>
+#include <type_traits>
+
+#include "gemm_tc.cuh"
+#include "host_err.h"
+#include "launch.h"
+#include "ptx.cuh"
+#include "qwen_b200_paged.h"
+
+namespace qb200x {
+
+using qb200::mbar_arrive;
+using qb200::mbar_arrive_expect_tx;
+using qb200::mbar_init;
+using qb200::mbar_try_wait;
+using qb200::smem_u32;
+using qb200tc::ex2_approx;
+using qb200tc::gemm_record;
+using qb200tc::gemm_wait;
+using qb200tc::sw128_desc;
+using qb200tc::sw128_mn_desc;
+using qb200tc::tc_fence_after;
+using qb200tc::tc_fence_before;
+using qb200tc::tmem_alloc;
+using qb200tc::tmem_dealloc;
+using qb200tc::tmem_ld64;
+
+// ------------------------------------------------------------ plan (int32)
+// Header words, then the arrays they point at (offsets in words).
+enum PlanWord : int {
+  PW_MAGIC = 0, PW_ROWS, PW_GROUPS, PW_CTAS, PW_SEGS, PW_TILES, PW_HEADS, PW_KV_HEADS,
+  PW_CTA_SEG, PW_SEG, PW_TILE_SLOT, PW_ROW, PW_ERR, PW_WORDS, PW_MIN_PREFIX, PW_MAX_PREFIX
+};
+constexpr int PLAN_MAGIC = 0x51503031;
+// A segment is a CTA's run of token tiles of one query tile (up to 256
+// queries of a group for one kv head); it leaves one partial slot.
+struct Seg {
+  int row0;     // first row of the group
+  int nq;       // queries of the group: rows x (heads / kv_heads)
+  int q0;       // first query of the tile
+  int kvh;      // kv head
+  int t0, t1;   // token tiles [t0, t1) of TN tokens
+  int prefix;   // prefix tokens of the group
+  int dual;     // more than 128 queries in the tile
+};
+// Per row: the group's prefix (0: none), the group's first query tile, the
+// row's first query in the group.
+struct RowPlan {
+  int prefix, tile0, query, pad;
+};
+
+constexpr int TN = 128;      // tokens of a tile
+constexpr int QT = 128;      // queries of a stream's tile
+constexpr int THREADS = 320; // 10 warps: TMA, MMA, two streams of four softmax warps
+constexpr int OWN_THREADS = 128;
+
+struct Args {
+  const void *q;
+  void *out;
+  float *lse;
+  const int *page_table, *seq_ids, *lengths;
+  const int *plan;
+  float *slots;        // prefix partials
+  float *own;          // own partials
+  long long q_row, q_head, o_row, o_head;
+  long long table_pitch;
+  long long page_stride, head_stride, token_stride;
+  const void *k_pool, *v_pool;
+  unsigned long long *err;
+  int rows, heads, kv_heads, ratio;
+  int num_pages, page_tokens, box, num_seqs, max_pages;
+  int length_bias, own_splits;
+  float scale_log2;
+};
+
+template <typename T>
+struct Type;
+template <>
+struct Type<__half> {
+  static constexpr int kBf16 = 0;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  }
+};
+template <>
+struct Type<__nv_bfloat16> {
+  static constexpr int kBf16 = 1;
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  }
+};
+
+// Length of row r (bias added), or -1 when its sequence or length lies
+// outside the tables.
+__device__ __forceinline__ int row_length(const Args &a, int r, int *seq) {
+  const int s = a.seq_ids[r];
+  const long long n = static_cast<long long>(a.lengths[r]) + a.length_bias;
+  *seq = s;
+  if (s < 0 || s >= a.num_seqs || n < 0 || n > static_cast<long long>(a.max_pages) * a.page_tokens) return -1;
+  return static_cast<int>(n);
+}
+
+// ------------------------------------------------------------ prefix kernel
+// Floats of one slot: two streams of acc[dim / 4][128 queries][4], m[128], l[128].
+template <int D>
+constexpr int kStreamFloats = QT * D + 2 * QT;
+template <int D>
+constexpr int kStages = D == 128 ? 5 : 8;       // K / V tiles in the ring
+template <int D>
+constexpr int kTileBytes = TN * D * 2;
+template <int D>
+constexpr size_t kPrefixSmem = 2 * static_cast<size_t>(QT * D * 2) + kStages<D> * static_cast<size_t>(kTileBytes<D>) + 256 + 1024;
+
+__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, int c0, int c1, int c2, int c3,
+                                            uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// One tcgen05.mma (M = 128, K = 16) of a converged warp, by an elected lane:
+// A from shared memory / from tensor memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "setp.ne.b32 q, %4, 0;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, q;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "setp.ne.b32 q, %4, 0;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, q;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void commit_elect(uint64_t *bar) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "@p tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
+      : "memory");
+}
+
+// 32 columns of this thread's lane, to and from registers.
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Instruction descriptor of kind::f16: fp32 accumulator, M = 128, N = n, both
+// operands fp16 or both bf16, A K-major, B K-major or MN-major.
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t idesc16(int n, bool b_mn) {
+  return (1u << 4) | (static_cast<uint32_t>(Type<T>::kBf16) << 7) | (static_cast<uint32_t>(Type<T>::kBf16) << 10) |
+         (b_mn ? (1u << 16) : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(QT >> 4) << 24);
+}
+
+// Place in the ring of token tile t's K and V, in the order in which the MMA
+// warp first needs them.  Dual: K0 V0 K1 V1 ...; single (the streams take
+// alternate tiles): K0 K1 V0 K2 V1 ... V(n-1).
+__device__ __forceinline__ int k_place(bool dual, int t) { return dual ? 2 * t : (t == 0 ? 0 : 2 * t - 1); }
+__device__ __forceinline__ int v_place(bool dual, int t, int n) {
+  return dual ? 2 * t + 1 : (t == n - 1 ? 2 * n - 1 : 2 * t + 2);
+}
+
+// One CTA works through its segments.  Two streams, each with its own score
+// and output accumulators in tensor memory and its own four softmax warps
+// (one query per thread): in a dual segment they hold two query tiles and use
+// each K / V tile together, in a single one they hold the same queries and
+// take alternate token tiles.  While one stream's softmax runs, the tensor
+// cores work for the other.
+//   S_s = Q_s K^T       tcgen05, both operands in shared memory
+//   P_s = 2^(S_s - m)   rounded to the input type over S_s in tensor memory
+//   O_s += P_s V        tcgen05, P from tensor memory, V as it lies (MN-major)
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS, 1)
+    prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Args a) {
+  constexpr int ST = kStages<D>, TILE = kTileBytes<D>, QB = QT * D * 2, HALVES = D / 64;
+  constexpr uint32_t S_COL = 0, O_COL = 256;  // tensor memory columns: S0 S1 | O0 O1, 128 each
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t *base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t *sq = base, *ring = base + 2 * QB;
+  uint64_t *kv_full = reinterpret_cast<uint64_t *>(ring + ST * TILE);
+  uint64_t *kv_empty = kv_full + ST;
+  uint64_t *s_full = kv_empty + ST, *p_full = s_full + 2, *q_full = p_full + 2, *o_full = q_full + 1;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(o_full + 1);
+  volatile uint32_t *abort = tmem_slot + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 4);
+    }
+    mbar_init(q_full, 8);
+    mbar_init(o_full, 1);
+    *abort = 0;
+    qb200::fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  qb200::griddep_wait();
+  if (threadIdx.x == 0) qb200::griddep_launch_dependents();
+
+  const int seg0 = a.plan[a.plan[PW_CTA_SEG] + blockIdx.x], seg1 = a.plan[a.plan[PW_CTA_SEG] + blockIdx.x + 1];
+  const Seg *segs = reinterpret_cast<const Seg *>(a.plan + a.plan[PW_SEG]);
+  const int boxes = TN / a.box;
+
+  // Page holding box b of token tile t of the segment's prefix, or num_pages
+  // (which the copy fills with zeros) when it is past the prefix or unmapped.
+  auto page_of = [&](const int *row, const Seg &s, int t, int b, bool *bad) {
+    const int pos = t * TN + b * a.box;
+    *bad = false;
+    if (pos >= s.prefix) return a.num_pages;
+    const int i = pos / a.page_tokens;
+    const int p = row != nullptr && i < a.max_pages ? row[i] : -1;
+    if (p >= 0 && p < a.num_pages) return p;
+    *bad = true;
+    return a.num_pages;
+  };
+  auto table_row = [&](const Seg &s) -> const int * {
+    const int seq = a.seq_ids[s.row0];
+    return seq >= 0 && seq < a.num_seqs ? a.page_table + seq * a.table_pitch : nullptr;
+  };
+
+  if (warp == 0) {
+    // ---- K / V tiles into the ring
+    int place = 0;  // tiles issued so far
+    bool ok = true;
+    for (int si = seg0; si < seg1 && ok; ++si) {
+      const Seg s = segs[si];
+      const int *row = table_row(s);
+      const int n = s.t1 - s.t0;
+      const int total = 2 * n;
+      for (int i = 0; i < total && ok; ++i) {
+        // Tile of place i (the inverse of k_place / v_place).
+        bool is_v;
+        int t;
+        if (s.dual) {
+          is_v = i & 1;
+          t = i >> 1;
+        } else if (i == 0) {
+          is_v = false;
+          t = 0;
+        } else if (i == total - 1) {
+          is_v = true;
+          t = n - 1;
+        } else {
+          is_v = !(i & 1);
+          t = is_v ? (i - 2) / 2 : (i + 1) / 2;
+        }
+        bool bad = false;
+        const int page = lane < boxes ? page_of(row, s, s.t0 + t, lane, &bad) : 0;
+        if (bad && !is_v) gemm_record(a.err, 3);
+        const int stage = place % ST;
+        if (place >= ST) ok = gemm_wait(&kv_empty[stage], ((place / ST) - 1) & 1, abort, a.err, 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&kv_full[stage], TILE);
+        __syncwarp();
+        if (lane < boxes) {
+          uint8_t *dst = ring + stage * TILE + lane * a.box * 128;
+          const int tok = (s.t0 + t) * TN + lane * a.box;
+          const int off = page == a.num_pages ? 0 : tok % a.page_tokens;
+#pragma unroll
+          for (int h = 0; h < HALVES; ++h)
+            tma_load_4d(dst + h * TN * 128, is_v ? &tm_v : &tm_k, 64 * h, off, s.kvh, page, &kv_full[stage]);
+        }
+        __syncwarp();
+        ++place;
+      }
+    }
+    // Every issued copy lands before the CTA may exit (matters after an abort).
+    for (int p = place > ST ? place - ST : 0; p < place; ++p) {
+      const uint64_t t0 = qb200::globaltimer_ns();
+      while (!mbar_try_wait(&kv_full[p % ST], (p / ST) & 1))
+        if (static_cast<long long>(qb200::globaltimer_ns() - t0) > qb200tc::WAIT_NS) {
+          if (lane == 0) gemm_record(a.err, 1);
+          break;
+        }
+    }
+  } else if (warp == 1) {
+    // ---- MMAs
+    constexpr uint32_t id_s = idesc16<T>(TN, false), id_o = idesc16<T>(D, true);
+    int ring0 = 0;            // ring place of the segment's first tile
+    int steps[2] = {0, 0};    // steps of each stream so far (phases of p_full)
+    bool ok = true;
+    for (int si = seg0; si < seg1 && ok; ++si) {
+      const Seg s = segs[si];
+      const bool dual = s.dual != 0;
+      const int nt = s.t1 - s.t0, n = dual ? 2 * nt : nt;
+      ok = gemm_wait(q_full, (si - seg0) & 1, abort, a.err, 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      auto score = [&](int i) {  // S of step i
+        const int st = i & 1, t = dual ? i >> 1 : i;
+        const int place = ring0 + k_place(dual, t), stage = place % ST;
+        ok = gemm_wait(&kv_full[stage], (place / ST) & 1, abort, a.err, 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t qa = smem_u32(sq + (dual ? st * QB : 0)), kb = smem_u32(ring + stage * TILE);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (k >> 2) * (TN * 128) + (k & 3) * 32;
+          mma_ss(tmem + S_COL + st * 128, sw128_desc(qa + off), sw128_desc(kb + off), id_s, k != 0);
+        }
+        commit_elect(&s_full[st]);
+        if (!dual || st == 1) commit_elect(&kv_empty[stage]);
+      };
+      score(0);
+      if (ok && n > 1) score(1);
+      for (int i = 0; i < n && ok; ++i) {
+        const int st = i & 1, t = dual ? i >> 1 : i;
+        ok = gemm_wait(&p_full[st], steps[st] & 1, abort, a.err, 1);
+        const int place = ring0 + v_place(dual, t, nt), stage = place % ST;
+        ok = ok && gemm_wait(&kv_full[stage], (place / ST) & 1, abort, a.err, 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ++steps[st];
+        tc_fence_after();
+        const uint32_t vb = smem_u32(ring + stage * TILE), pa = tmem + S_COL + st * 128;
+        // Only the 16-token steps inside the prefix: what lies behind it in a
+        // page may be anything (0 x NaN).
+        const int ks = min(TN, s.prefix - (s.t0 + t) * TN) / 16;
+        for (int k = 0; k < ks; ++k)
+          mma_ts(tmem + O_COL + st * 128, pa + 8 * k, sw128_mn_desc(vb + 2048 * k, TN * 128), id_o, k != 0 || i > 1);
+        if (!dual || st == 1) commit_elect(&kv_empty[stage]);
+        if (i + 2 < n) score(i + 2);
+      }
+      if (!ok) break;
+      commit_elect(o_full);
+      ring0 += 2 * nt;
+    }
+    if (!ok) {  // tensor memory is freed only after every issued MMA has completed
+      commit_elect(o_full);
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax: thread = query
+    const int st = warp >= 6 ? 1 : 0;
+    const int quad = warp & 3, ql = 32 * quad + lane;
+    const int tid = threadIdx.x - 64;  // 0..255
+    const uint32_t ts = tmem + S_COL + st * 128 + (static_cast<uint32_t>(32 * quad) << 16);
+    const uint32_t to = tmem + O_COL + st * 128 + (static_cast<uint32_t>(32 * quad) << 16);
+    int steps = 0;
+    bool ok = true;
+    for (int si = seg0; si < seg1 && ok; ++si) {
+      const Seg s = segs[si];
+      const bool dual = s.dual != 0;
+      const int nt = s.t1 - s.t0;
+      // Queries of this segment into shared memory (128-byte swizzled rows);
+      // rows past the group are zero.
+      {
+        constexpr int CPR = D / 8;  // 16-byte chunks of a query
+        const int nload = min(dual ? 256 : 128, (s.nq - s.q0 + 31) / 32 * 32);
+        const T *qg = static_cast<const T *>(a.q);
+        for (int i = tid; i < nload * CPR; i += 256) {
+          const int qi = i / CPR, c = i % CPR;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (s.q0 + qi < s.nq) {
+            const int r = (s.q0 + qi) / a.ratio, h = (s.q0 + qi) % a.ratio;
+            v = *reinterpret_cast<const uint4 *>(qg + (s.row0 + r) * a.q_row + (s.kvh * a.ratio + h) * a.q_head + 8 * c);
+          }
+          const int rr = qi & 127;
+          uint8_t *dst = sq + (qi >> 7) * QB + (c >> 3) * (QT * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
+          *reinterpret_cast<uint4 *>(dst) = v;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
+      }
+      const int my_steps = dual ? nt : (st == 0 ? (nt + 1) / 2 : nt / 2);
+      // Queries of this warp past the group: nothing to compute.
+      const bool live = s.q0 + (dual ? st * QT : 0) + 32 * quad < s.nq;
+      const int *row = table_row(s);
+      float m = -INFINITY, l = 0.f;
+      for (int i = 0; i < my_steps && ok; ++i) {
+        const int t = s.t0 + (dual ? i : 2 * i + st);
+        // Valid tokens of the tile: one bit per box of the copy.
+        bool bad = false;
+        const int page = lane < boxes ? page_of(row, s, t, lane, &bad) : 0;
+        const uint32_t valid = __ballot_sync(0xffffffffu, lane < boxes && page != a.num_pages);
+        const int ntok = min(TN, s.prefix - t * TN);
+        ok = gemm_wait(&s_full[st], steps & 1, abort, a.err, 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ++steps;
+        tc_fence_after();
+        if (live) {
+          float v[2][64];
+          tmem_ld64(ts, ts + 32, v[0]);
+          tmem_ld64(ts + 64, ts + 96, v[1]);
+          if (ntok < TN || valid != (1u << boxes) - 1u) {
+#pragma unroll
+            for (int c = 0; c < TN; ++c)
+              if (c >= ntok || ((valid >> (c / a.box)) & 1u) == 0) v[c >> 6][c & 63] = -INFINITY;
+          }
+          float mx[4] = {v[0][0], v[0][1], v[0][2], v[0][3]};
+#pragma unroll
+          for (int c = 4; c < TN; ++c) mx[c & 3] = fmaxf(mx[c & 3], v[c >> 6][c & 63]);
+          const float rowmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+          if (i == 0) {
+            m = rowmax;
+          } else if (__any_sync(0xffffffffu, rowmax > m + 8.f)) {
+            // The maximum moves only when a row has outgrown it by 2^8: the
+            // weights stay below 2^8, exact in relative terms, and the output
+            // is rescaled a few times at most.
+            const float mn = fmaxf(m, rowmax);
+            const float f = mn == -INFINITY ? 1.f : ex2_approx(m - mn);
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int c = 0; c < D; c += 64) {
+              float o[64];
+              tmem_ld64(to + c, to + c + 32, o);
+              uint32_t w[2][32];
+#pragma unroll
+              for (int j = 0; j < 64; ++j) w[j >> 5][j & 31] = __float_as_uint(o[j] * f);
+              tmem_st32(to + c, w[0]);
+              tmem_st32(to + c + 32, w[1]);
+            }
+          }
+          const float mu = m == -INFINITY ? 0.f : m;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          uint32_t p[2][32];
+#pragma unroll
+          for (int c = 0; c < TN; c += 2) {
+            const float x = ex2_approx(fmaf(v[c >> 6][c & 63], a.scale_log2, -mu));
+            const float y = ex2_approx(fmaf(v[c >> 6][(c & 63) + 1], a.scale_log2, -mu));
+            sum[c & 2] += x;
+            sum[(c & 2) + 1] += y;
+            // The weights enter the second product rounded to the input type
+            // (half a step each, as the values they weigh); their sum is not.
+            p[c >> 6][(c >> 1) & 31] = Type<T>::pack(x, y);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_st32(ts, p[0]);
+          tmem_st32(ts + 32, p[1]);
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[st]);
+      }
+      if (!ok) break;
+      ok = gemm_wait(o_full, (si - seg0) & 1, abort, a.err, 1);
+      ok = __all_sync(0xffffffffu, ok && !*abort);
+      if (!ok) break;
+      tc_fence_after();
+      if (live) {
+        float *slot = a.slots + (static_cast<size_t>(si) * 2 + st) * kStreamFloats<D>;
+        if (my_steps > 0) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 64) {
+            float o[64];
+            tmem_ld64(to + c, to + c + 32, o);
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              reinterpret_cast<float4 *>(slot)[(c / 4 + j) * QT + ql] =
+                  make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          }
+        }
+        slot[QT * D + ql] = m;
+        // A visible part whose scores are all -inf: the sum tells it from an
+        // empty one (the softmax of nothing but -inf is NaN).
+        slot[QT * D + QT + ql] = my_steps > 0 && m == -INFINITY ? 1.f : l;
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    if (*abort) {  // wait (bounded) for the MMAs still in flight
+      const uint64_t t0 = qb200::globaltimer_ns();
+      const int done = seg1 - seg0;
+      (void)done;
+      while (!mbar_try_wait(o_full, 0) && !mbar_try_wait(o_full, 1))
+        if (static_cast<long long>(qb200::globaltimer_ns() - t0) > qb200tc::WAIT_NS) break;
+    }
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// --------------------------------------------------------------- own kernel
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  if constexpr (Type<T>::kBf16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint4 ld_kv(const void *p, bool on) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (on)
+    asm volatile("ld.global.L1::no_allocate.L2::128B.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// grid (splits, kv heads x head tiles of 8, rows), 4 warps.  The CTA takes
+// positions [start + split * per, ...) of its row, its warps blocks of 16
+// tokens in turn, each with its own online softmax; the four join through
+// shared memory.  Per block, with tokens on the M side of the products:
+//   S^T[16 tokens, 8 heads] = K Q^T, O^T[D dims, 8 heads] += V^T P^T.
+// K fragments come straight from global memory: lane (g, c) = (lane / 4,
+// lane % 4) reads 16 bytes at dims 32 i + 8 c of tokens g and g + 8, and the
+// contraction runs over the dims in that order on both sides.  V likewise:
+// the lane reads tokens 2c, 2c+1, 2c+8, 2c+9 at dims 64 i + 8 g and pairs
+// tokens with byte permutes, which is the transposed operand.
+template <typename T, int D>
+__global__ void __launch_bounds__(OWN_THREADS) own_kernel(const Args a) {
+  qb200::griddep_wait();
+  qb200::griddep_launch_dependents();
+  constexpr int KI = D / 32;  // 16-byte chunks of a token per lane (scores)
+  constexpr int VI = D / 64;  // 16-byte chunks of a token per lane (values)
+  __shared__ float s_m[4][8], s_l[4][8];
+  __shared__ __align__(16) float s_o[4][8][D + 4];
+  const int split = blockIdx.x, row = blockIdx.z;
+  const int htiles = (a.ratio + 7) >> 3;
+  const int kvh = blockIdx.y / htiles, h0 = (blockIdx.y % htiles) * 8;
+  const int nh = min(8, a.ratio - h0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  int seq;
+  const int len = row_length(a, row, &seq);
+  const RowPlan rp = reinterpret_cast<const RowPlan *>(a.plan + a.plan[PW_ROW])[row];
+  if (len < 0) {
+    if (threadIdx.x == 0) gemm_record(a.err, 3);
+  }
+  const int start = len >= rp.prefix ? rp.prefix : 0;
+  const int count = max(0, len - start);
+  // Tokens of one split: a multiple of 64 that covers the row.
+  const int per = ((count + a.own_splits - 1) / a.own_splits + 63) / 64 * 64;
+  const int lo = start + split * per, hi = min(len, lo + per);
+  float *part = a.own + ((static_cast<size_t>(row) * a.heads + kvh * a.ratio + h0) * a.own_splits + split) * (D + 2);
+  const size_t part_head = static_cast<size_t>(a.own_splits) * (D + 2);
+  if (lo >= hi) {
+    if (static_cast<int>(threadIdx.x) < nh) {
+      part[threadIdx.x * part_head + D] = -INFINITY;
+      part[threadIdx.x * part_head + D + 1] = 0.f;
+    }
+    return;
+  }
+  const int *trow = a.page_table + seq * a.table_pitch;
+  const T *kp = static_cast<const T *>(a.k_pool) + kvh * a.head_stride;
+  const T *vp = static_cast<const T *>(a.v_pool) + kvh * a.head_stride;
+
+  // Q^T as the B operand: n = head g, k = dims in the order of the K loads.
+  uint32_t qb[KI][4];
+  {
+    const T *qr = static_cast<const T *>(a.q) + row * a.q_row + (kvh * a.ratio + h0 + g) * a.q_head;
+#pragma unroll
+    for (int i = 0; i < KI; ++i) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (g < nh) v = *reinterpret_cast<const uint4 *>(qr + 32 * i + 8 * c);
+      qb[i][0] = v.x; qb[i][1] = v.y; qb[i][2] = v.z; qb[i][3] = v.w;
+    }
+  }
+  float o[VI][4][2][2][2];  // [dims 64 i][m tile][rows g | g + 8][...]: see below
+  // O^T tile (i, e): rows = dims 64 i + 8 g + e (rows g) and 64 i + 8 g + e + 4
+  // (rows g + 8), columns = heads 2c, 2c + 1.
+#pragma unroll
+  for (int i = 0; i < VI; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) o[i][e][x][0][0] = o[i][e][x][0][1] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // heads 2c, 2c + 1
+  bool seen = false;
+
+  for (int b = lo + 16 * warp; b < hi; b += 64) {
+    const int pi = b / a.page_tokens;
+    const int page = trow[pi];
+    if (page < 0 || page >= a.num_pages) {
+      if (lane == 0) gemm_record(a.err, 3);
+      continue;
+    }
+    const long long at = page * a.page_stride + static_cast<long long>(b - pi * a.page_tokens) * a.token_stride;
+    const int n = min(16, hi - b);
+    uint4 kv[2][KI], vv[4][VI];
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int i = 0; i < KI; ++i)
+        kv[x][i] = ld_kv(kp + at + (g + 8 * x) * a.token_stride + 32 * i + 8 * c, g + 8 * x < n);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int tok = 2 * c + (x & 1) + 8 * (x >> 1);
+#pragma unroll
+      for (int i = 0; i < VI; ++i) vv[x][i] = ld_kv(vp + at + tok * a.token_stride + 64 * i + 8 * g, tok < n);
+    }
+    float s[4] = {0.f, 0.f, 0.f, 0.f};  // (token g, heads 2c, 2c+1), (token g + 8, ...)
+#pragma unroll
+    for (int i = 0; i < KI; ++i) {
+      mma16816<T>(s, kv[0][i].x, kv[1][i].x, kv[0][i].y, kv[1][i].y, qb[i][0], qb[i][1]);
+      mma16816<T>(s, kv[0][i].z, kv[1][i].z, kv[0][i].w, kv[1][i].w, qb[i][2], qb[i][3]);
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) s[2 * x + h] = g + 8 * x < n ? s[2 * x + h] * a.scale_log2 : -INFINITY;
+    float p[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float mx = fmaxf(s[h], s[2 + h]);
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+      const float mn = fmaxf(m[h], mx);
+      const float mu = mn == -INFINITY ? 0.f : mn;
+      const float f = ex2_approx(m[h] - mu);
+      p[h] = ex2_approx(s[h] - mu);
+      p[2 + h] = ex2_approx(s[2 + h] - mu);
+      l[h] = l[h] * f + (p[h] + p[2 + h]);
+      m[h] = mn;
+#pragma unroll
+      for (int i = 0; i < VI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          o[i][e][0][0][h] *= f;
+          o[i][e][1][0][h] *= f;
+        }
+    }
+    seen = true;
+    // P^T as the B operand (n = head g, k = tokens 2c, 2c+1 / 2c+8, 2c+9).
+    const uint32_t b0 = transpose8x8(Type<T>::pack(p[0], p[1]));
+    const uint32_t b1 = transpose8x8(Type<T>::pack(p[2], p[3]));
+#pragma unroll
+    for (int i = 0; i < VI; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        // A rows g: dim 8 g + e; rows g + 8: dim 8 g + e + 4.
+        const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
+        const int w0 = e >> 1, w1 = 2 + (e >> 1);
+        const uint32_t a0 = __byte_perm(word(vv[0][i], w0), word(vv[1][i], w0), sel);
+        const uint32_t a1 = __byte_perm(word(vv[0][i], w1), word(vv[1][i], w1), sel);
+        const uint32_t a2 = __byte_perm(word(vv[2][i], w0), word(vv[3][i], w0), sel);
+        const uint32_t a3 = __byte_perm(word(vv[2][i], w1), word(vv[3][i], w1), sel);
+        float d[4] = {o[i][e][0][0][0], o[i][e][0][0][1], o[i][e][1][0][0], o[i][e][1][0][1]};
+        mma16816<T>(d, a0, a1, a2, a3, b0, b1);
+        o[i][e][0][0][0] = d[0];
+        o[i][e][0][0][1] = d[1];
+        o[i][e][1][0][0] = d[2];
+        o[i][e][1][0][1] = d[3];
+      }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 4);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 8);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 16);
+    // Seen tokens whose scores are all -inf: as in the prefix kernel.
+    if (seen && m[h] == -INFINITY) l[h] = 1.f;
+    if (g == 0) {
+      s_m[warp][2 * c + h] = m[h];
+      s_l[warp][2 * c + h] = l[h];
+    }
+#pragma unroll
+    for (int i = 0; i < VI; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s_o[warp][2 * c + h][64 * i + 8 * g + e] = o[i][e][0][0][h];
+        s_o[warp][2 * c + h][64 * i + 8 * g + e + 4] = o[i][e][1][0][h];
+      }
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < nh * D; x += OWN_THREADS) {
+    const int h = x / D, d = x % D;
+    float mm = fmaxf(fmaxf(s_m[0][h], s_m[1][h]), fmaxf(s_m[2][h], s_m[3][h]));
+    float acc = 0.f, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = mm == -INFINITY ? 1.f : ex2_approx(s_m[w][h] - mm);
+      acc += s_m[w][h] == -INFINITY ? 0.f : s_o[w][h][d] * f;
+      sum += s_m[w][h] == -INFINITY && mm != -INFINITY ? 0.f : s_l[w][h] * f;
+    }
+    part[h * part_head + d] = acc;
+    if (d == 0) {
+      part[h * part_head + D] = mm;
+      part[h * part_head + D + 1] = sum;
+    }
+  }
+}
+
+// -------------------------------------------------------------- join kernel
+// grid (heads, rows), 32 lanes of D / 32 dims: every partial of the row's
+// prefix tile, then of its own splits, in that order.
+template <typename T, int D>
+__global__ void __launch_bounds__(D / 4) join_kernel(const Args a) {
+  qb200::griddep_wait();
+  qb200::griddep_launch_dependents();
+  const int head = blockIdx.x, row = blockIdx.y, lane = threadIdx.x;  // lane: 4 dims
+  int seq;
+  const int len = row_length(a, row, &seq);
+  const RowPlan rp = reinterpret_cast<const RowPlan *>(a.plan + a.plan[PW_ROW])[row];
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float none = 0.f;  // visible parts whose scores are all -inf
+  auto add = [&](float mi, float li, const float4 &v) {
+    if (mi == -INFINITY) {
+      none += li;
+      return;
+    }
+    const float mn = fmaxf(m, mi);
+    const float f = ex2_approx(m - mn), h = ex2_approx(mi - mn);
+    l = l * f + li * h;
+    acc.x = acc.x * f + v.x * h;
+    acc.y = acc.y * f + v.y * h;
+    acc.z = acc.z * f + v.z * h;
+    acc.w = acc.w * f + v.w * h;
+    m = mn;
+  };
+  if (rp.prefix > 0 && len >= rp.prefix) {
+    const int kvh = head / a.ratio, qi = rp.query + head % a.ratio;
+    const int tile = rp.tile0 + (qi / (2 * QT)) * a.kv_heads + kvh;
+    const int *ts = a.plan + a.plan[PW_TILE_SLOT];
+    const Seg *segs = reinterpret_cast<const Seg *>(a.plan + a.plan[PW_SEG]);
+    const int s0 = ts[tile], s1 = ts[tile + 1];
+    const bool dual = segs[s0].dual != 0;
+    const int ql = qi % QT, st0 = dual ? (qi / QT) & 1 : 0, st1 = dual ? st0 + 1 : 2;
+    for (int s = s0; s < s1; ++s)
+      for (int st = st0; st < st1; ++st) {
+        if (!dual && st == 1 && segs[s].t1 - segs[s].t0 < 2) continue;  // the stream had no tile
+        const float *slot = a.slots + (static_cast<size_t>(s) * 2 + st) * kStreamFloats<D>;
+        add(slot[QT * D + ql], slot[QT * D + QT + ql], reinterpret_cast<const float4 *>(slot)[lane * QT + ql]);
+      }
+  }
+  const float *own = a.own + (static_cast<size_t>(row) * a.heads + head) * a.own_splits * (D + 2);
+  if (len > 0) {
+    const int start = len >= rp.prefix ? rp.prefix : 0;
+    const int count = len - start;
+    const int per = ((count + a.own_splits - 1) / a.own_splits + 63) / 64 * 64;
+    const int ns = count > 0 ? (count + per - 1) / per : 0;
+    for (int s = 0; s < ns; ++s) {
+      const float *p = own + static_cast<size_t>(s) * (D + 2);
+      add(p[D], p[D + 1], make_float4(p[4 * lane], p[4 * lane + 1], p[4 * lane + 2], p[4 * lane + 3]));
+    }
+  }
+  float lse;
+  if (m == -INFINITY) {  // nothing seen: 0; nothing but -inf: NaN
+    const float x = none > 0.f ? __int_as_float(0x7fffffff) : 0.f;
+    acc = make_float4(x, x, x, x);
+    lse = -INFINITY;
+  } else {
+    const float inv = 1.f / l;
+    acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    lse = (m + log2f(l)) * 0.6931471805599453f;
+  }
+  uint2 w;
+  w.x = Type<T>::pack(acc.x, acc.y);
+  w.y = Type<T>::pack(acc.z, acc.w);
+  *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + row * a.o_row + head * a.o_head + 4 * lane) = w;
+  if (lane == 0 && a.lse != nullptr) a.lse[static_cast<size_t>(row) * a.heads + head] = lse;
+}
+
+}  // namespace qb200x
+
+// ====================================================================== host
+using namespace qb200x;
+
+namespace {
+
+int fail(int code, const char *fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return qb200_set_error(code, buf);
+}
+
+bool al16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+constexpr int MAX_SPLITS = 64;
+
+// Splits of a row's own part: enough CTAs for a few per SM when the batch is
+// small, at least 128 tokens each.
+int own_splits(int rows, int kv_heads, int ratio, int own_tokens) {
+  const long long ctas = static_cast<long long>(rows) * kv_heads * ((ratio + 7) / 8);
+  long long s = (592 + ctas - 1) / ctas;
+  const long long most = (own_tokens + 127) / 128;
+  if (s > most) s = most;
+  if (s > MAX_SPLITS) s = MAX_SPLITS;
+  return s < 1 ? 1 : static_cast<int>(s);
+}
+
+int plan_splits(const int *h, int max_length) {
+  const int own = max_length - h[PW_MIN_PREFIX];
+  return own_splits(h[PW_ROWS], h[PW_KV_HEADS], h[PW_HEADS] / h[PW_KV_HEADS], own < 1 ? 1 : own);
+}
+
+long long up256(long long b) { return (b + 255) / 256 * 256; }
+long long slot_bytes(const int *h, int dim) {
+  return up256(static_cast<long long>(h[PW_SEGS]) * 2 * (QT * dim + 2 * QT) * 4);
+}
+
+bool plan_ok(const int *h) { return h != nullptr && h[PW_MAGIC] == PLAN_MAGIC; }
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                   const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encoder() {
+  static EncodeTiledFn fn = [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult st{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &st) != cudaSuccess) p = nullptr;
+    return reinterpret_cast<EncodeTiledFn>(p);
+  }();
+  return fn;
+}
+
+// Pool [num_pages][kv_heads][page_tokens][dim] as a 4-D tensor map with boxes
+// of `box` tokens x 64 elements, 128-byte swizzle.
+int encode_pool(CUtensorMap *m, const QwenPrefixAttention &a, const void *pool, int box) {
+  EncodeTiledFn enc = encoder();
+  if (enc == nullptr) return fail(30, "cuTensorMapEncodeTiled is unavailable from the driver");
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(a.page_tokens),
+                              static_cast<cuuint64_t>(a.kv_heads), static_cast<cuuint64_t>(a.num_pages)};
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(a.token_stride) * 2, static_cast<cuuint64_t>(a.head_stride) * 2,
+                                 static_cast<cuuint64_t>(a.page_stride) * 2};
+  const cuuint32_t bx[4] = {64, static_cast<cuuint32_t>(box), 1, 1};
+  const cuuint32_t es[4] = {1, 1, 1, 1};
+  const CUresult r = enc(m, a.dtype ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                         const_cast<void *>(pool), dims, strides, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(31, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+  return 0;
+}
+
+template <typename T, int D>
+int launch(const QwenPrefixAttention &u, const Args &a, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t st) {
+  const int *h = u.plan_header;
+  if (h[PW_SEGS] > 0) {
+    static std::mutex mu;
+    static bool set[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return fail(2, "cudaGetDevice failed");
+    {
+      std::lock_guard<std::mutex> lk(mu);
+      if (!set[dev]) {
+        const cudaError_t e = cudaFuncSetAttribute(prefix_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   static_cast<int>(kPrefixSmem<D>));
+        if (e != cudaSuccess) return fail(4, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+        set[dev] = true;
+      }
+    }
+    const cudaError_t e = qb200_launch(prefix_kernel<T, D>, dim3(h[PW_CTAS]), dim3(THREADS), kPrefixSmem<D>, st, true,
+                                       mk, mv, a);
+    if (e != cudaSuccess) return fail(20, "prefix attention launch: %s", cudaGetErrorString(e));
+  }
+  cudaError_t e = qb200_launch(own_kernel<T, D>, dim3(a.own_splits, a.kv_heads * ((a.ratio + 7) / 8), a.rows),
+                               dim3(OWN_THREADS), 0, st, true, a);
+  if (e != cudaSuccess) return fail(20, "own attention launch: %s", cudaGetErrorString(e));
+  e = qb200_launch(join_kernel<T, D>, dim3(a.heads, a.rows), dim3(D / 4), 0, st, true, a);
+  if (e != cudaSuccess) return fail(20, "attention join launch: %s", cudaGetErrorString(e));
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_lens, int heads, int kv_heads, int ctas,
+                          int *words, int capacity) {
+  qb200_clear_error();
+  const auto bad = [](int code, const char *msg) {
+    qb200_set_error(code, msg);
+    return 0;
+  };
+  if (groups < 1 || group_rows == nullptr || prefix_lens == nullptr) return bad(13, "plan: no groups");
+  if (kv_heads < 1 || heads < kv_heads || heads % kv_heads != 0 || heads / kv_heads > 128 || kv_heads > 4096)
+    return bad(10, "plan: heads must be a multiple of kv_heads, at most 128 per kv head");
+  if (ctas < 1 || ctas > 4096) return bad(10, "plan: ctas outside [1, 4096]");
+  const int ratio = heads / kv_heads;
+  long long rows = 0, tiles = 0, weight = 0;
+  int min_prefix = 0x7fffffff, max_prefix = 0;
+  // A group of one row shares nothing: its row runs on its own pages.  The
+  // prefix is cut to whole steps of 16 tokens of the products; the tokens
+  // behind the cut count as each row's own.
+  const auto prefix_of = [&](int g) { return group_rows[g] > 1 ? prefix_lens[g] / 16 * 16 : 0; };
+  for (int g = 0; g < groups; ++g) {
+    if (group_rows[g] < 0 || prefix_lens[g] < 0) return bad(10, "plan: negative group size or prefix");
+    rows += group_rows[g];
+    const int p = prefix_of(g);
+    if (group_rows[g] > 0 && p < min_prefix) min_prefix = p;
+    if (p > max_prefix) max_prefix = p;
+    if (p == 0) continue;
+    const long long nq = static_cast<long long>(group_rows[g]) * ratio, nt = (p + TN - 1) / TN;
+    if (nq > (1ll << 24)) return bad(10, "plan: a group of over 2^24 queries");
+    const long long qt = (nq + 2 * QT - 1) / (2 * QT);
+    tiles += qt * kv_heads;
+    for (long long t = 0; t < qt; ++t) weight += (nq - t * 2 * QT > QT ? 2 : 1) * nt * kv_heads;
+  }
+  if (rows < 1 || rows > 65535) return bad(10, "plan: rows outside [1, 65535]");
+  if (tiles > (1 << 20)) return bad(10, "plan: over 2^20 query tiles");
+  if (min_prefix == 0x7fffffff) min_prefix = 0;
+  // Contiguous shares of the weighted token tiles for every CTA.
+  if (ctas > weight) ctas = weight > 0 ? static_cast<int>(weight) : 1;
+  const long long max_segs = tiles + ctas;
+  const long long o_cta = QWEN_PREFIX_HEADER, o_seg = (o_cta + ctas + 1 + 7) / 8 * 8, o_tile = o_seg + max_segs * 8,
+                  o_row = (o_tile + tiles + 1 + 7) / 8 * 8, o_err = o_row + rows * 4, total = o_err + 4;
+  if (total > 0x7fffffffll) return bad(10, "plan: too large");
+  if (words == nullptr) return static_cast<int>(total);
+  if (capacity < total) return bad(15, "plan: the buffer is too small");
+  for (long long i = 0; i < total; ++i) words[i] = 0;
+  int nseg = 0, ntile = 0, cta = 0;
+  long long done = 0;  // weight handed out
+  Seg *segs = reinterpret_cast<Seg *>(words + o_seg);
+  RowPlan *rp = reinterpret_cast<RowPlan *>(words + o_row);
+  int row0 = 0;
+  const auto limit = [&](int c) { return weight * (c + 1) / ctas; };  // end of CTA c's share
+  for (int g = 0; g < groups; ++g) {
+    const int p = prefix_of(g);
+    for (int r = 0; r < group_rows[g]; ++r) rp[row0 + r] = RowPlan{p, ntile, r * ratio, 0};
+    if (p > 0) {
+      const int nq = group_rows[g] * ratio, nt = (p + TN - 1) / TN;
+      for (int q0 = 0; q0 < nq; q0 += 2 * QT) {
+        const int dual = nq - q0 > QT ? 1 : 0, w = dual ? 2 : 1;
+        for (int h = 0; h < kv_heads; ++h) {
+          words[o_tile + ntile++] = nseg;
+          for (int t = 0; t < nt;) {
+            while (cta + 1 < ctas && done >= limit(cta)) words[o_cta + ++cta] = nseg;
+            long long take = (limit(cta) - done + w - 1) / w;
+            if (take < 1 || cta + 1 == ctas) take = cta + 1 == ctas ? nt - t : 1;
+            if (take > nt - t) take = nt - t;
+            segs[nseg++] = Seg{row0, nq, q0, h, t, t + static_cast<int>(take), p, dual};
+            t += static_cast<int>(take);
+            done += take * w;
+          }
+        }
+      }
+    }
+    row0 += group_rows[g];
+  }
+  words[o_tile + ntile] = nseg;
+  while (cta + 1 <= ctas) words[o_cta + ++cta] = nseg;
+  const int head[QWEN_PREFIX_HEADER] = {PLAN_MAGIC, static_cast<int>(rows), groups, ctas, nseg, ntile, heads, kv_heads,
+                                        static_cast<int>(o_cta), static_cast<int>(o_seg), static_cast<int>(o_tile),
+                                        static_cast<int>(o_row), static_cast<int>(o_err), static_cast<int>(total),
+                                        min_prefix, max_prefix};
+  for (int i = 0; i < QWEN_PREFIX_HEADER; ++i) words[i] = head[i];
+  return static_cast<int>(total);
+}
+
+long long qwen_b200_prefix_workspace(const int *h, int dim, int max_length) {
+  if (!plan_ok(h) || (dim != 64 && dim != 128)) return 0;
+  return slot_bytes(h, dim) +
+         up256(static_cast<long long>(h[PW_ROWS]) * h[PW_HEADS] * plan_splits(h, max_length) * (dim + 2) * 4);
+}
+
+int qwen_b200_prefix_attention(const QwenPrefixAttention *u, void *stream) {
+  qb200_clear_error();
+  if (u == nullptr) return fail(13, "null argument");
+  const int *h = u->plan_header;
+  if (!plan_ok(h)) return fail(13, "plan: not the words of qwen_b200_prefix_plan");
+  if (u->rows != h[PW_ROWS] || u->heads != h[PW_HEADS] || u->kv_heads != h[PW_KV_HEADS])
+    return fail(10, "the plan is for %d rows, %d / %d heads; called with %d rows, %d / %d heads", h[PW_ROWS],
+                h[PW_HEADS], h[PW_KV_HEADS], u->rows, u->heads, u->kv_heads);
+  if (u->dim != 64 && u->dim != 128) return fail(10, "dim=%d: 64 or 128", u->dim);
+  if (u->dtype != 0 && u->dtype != 1) return fail(10, "dtype=%d: 0 (fp16) or 1 (bf16)", u->dtype);
+  if (u->num_pages < 1 || u->page_tokens < 16 || u->page_tokens % 16 != 0)
+    return fail(10, "num_pages=%d page_tokens=%d: pages of a multiple of 16 tokens", u->num_pages, u->page_tokens);
+  if (u->num_seqs < 1 || u->max_pages < 1 || u->table_pitch < u->max_pages)
+    return fail(10, "page table: num_seqs=%d max_pages=%d pitch=%lld", u->num_seqs, u->max_pages, u->table_pitch);
+  if (static_cast<long long>(u->max_pages) * u->page_tokens > 0x7fff0000ll)
+    return fail(10, "page table rows of over 2^31 tokens");
+  if (!(u->scale > 0.f) || u->scale > 1e30f) return fail(10, "scale=%g must be positive", static_cast<double>(u->scale));
+  if (u->max_length < 0) return fail(10, "max_length=%d", u->max_length);
+  const void *need[] = {u->q, u->out, u->k_pool, u->v_pool, u->page_table, u->seq_ids, u->lengths, u->plan, u->workspace};
+  for (const void *p : need)
+    if (p == nullptr) return fail(13, "null pointer argument");
+  for (const void *p : {u->q, static_cast<const void *>(u->out), u->k_pool, u->v_pool, static_cast<const void *>(u->plan),
+                        static_cast<const void *>(u->workspace)})
+    if (!al16(p)) return fail(14, "q, out, pools, plan and workspace must be 16-byte aligned");
+  for (long long s : {u->q_row_stride, u->q_head_stride, u->out_row_stride, u->out_head_stride, u->page_stride,
+                      u->head_stride, u->token_stride})
+    if (s < 0 || s % 8 != 0 || s > (1ll << 38)) return fail(14, "stride of %lld elements: must be a multiple of 8", s);
+  if (u->token_stride < u->dim || (u->kv_heads > 1 && u->head_stride < u->dim) || (u->num_pages > 1 && u->page_stride < u->dim))
+    return fail(14, "pool strides overlap");
+  const long long ws = qwen_b200_prefix_workspace(h, u->dim, u->max_length);
+  if (u->workspace_bytes < ws) return fail(15, "workspace of %lld bytes, need %lld", u->workspace_bytes, ws);
+  Args a{};
+  a.q = u->q;
+  a.out = u->out;
+  a.lse = u->lse;
+  a.page_table = u->page_table;
+  a.seq_ids = u->seq_ids;
+  a.lengths = u->lengths;
+  a.plan = static_cast<const int *>(u->plan);
+  a.slots = static_cast<float *>(u->workspace);
+  a.own = reinterpret_cast<float *>(static_cast<char *>(u->workspace) + slot_bytes(h, u->dim));
+  a.q_row = u->q_row_stride;
+  a.q_head = u->q_head_stride;
+  a.o_row = u->out_row_stride;
+  a.o_head = u->out_head_stride;
+  a.table_pitch = u->table_pitch;
+  a.page_stride = u->page_stride;
+  a.head_stride = u->head_stride;
+  a.token_stride = u->token_stride;
+  a.k_pool = u->k_pool;
+  a.v_pool = u->v_pool;
+  a.err = reinterpret_cast<unsigned long long *>(static_cast<int *>(u->plan) + h[PW_ERR]);
+  a.rows = u->rows;
+  a.heads = u->heads;
+  a.kv_heads = u->kv_heads;
+  a.ratio = u->heads / u->kv_heads;
+  a.num_pages = u->num_pages;
+  a.page_tokens = u->page_tokens;
+  a.num_seqs = u->num_seqs;
+  a.max_pages = u->max_pages;
+  a.length_bias = u->length_bias;
+  a.own_splits = plan_splits(h, u->max_length);
+  a.scale_log2 = u->scale * 1.4426950408889634f;
+  a.box = u->page_tokens % 128 == 0 ? 128 : u->page_tokens % 64 == 0 ? 64 : u->page_tokens % 32 == 0 ? 32 : 16;
+  CUtensorMap mk, mv;
+  if (h[PW_SEGS] > 0) {
+    if (int rc = encode_pool(&mk, *u, u->k_pool, a.box)) return rc;
+    if (int rc = encode_pool(&mv, *u, u->v_pool, a.box)) return rc;
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (u->dtype == 0)
+    return u->dim == 128 ? launch<__half, 128>(*u, a, mk, mv, st) : launch<__half, 64>(*u, a, mk, mv, st);
+  return u->dim == 128 ? launch<__nv_bfloat16, 128>(*u, a, mk, mv, st) : launch<__nv_bfloat16, 64>(*u, a, mk, mv, st);
+}
+
+int qwen_b200_prefix_status(const int *h, void *plan, uint64_t *detail) {
+  if (!plan_ok(h) || plan == nullptr) return -1;
+  unsigned long long v = 0;
+  void *err = static_cast<int *>(plan) + h[PW_ERR];
+  if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpy(&v, err, sizeof(v), cudaMemcpyDeviceToHost) != cudaSuccess)
+    return -2;
+  if (detail) *detail = v;
+  if (v != 0) cudaMemset(err, 0, sizeof(v));
+  return static_cast<int>(v >> 32);
+}
+
+}  // extern "C"
