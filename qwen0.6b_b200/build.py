@@ -3,8 +3,8 @@
 * ``libqwen_b200.so``: every CUDA kernel plus the C ABI of ``include/*.h``,
   compiled by nvcc for sm_100a only (``-gencode arch=compute_100a,code=sm_100a``).
 * ``qwen_megakernel_C``, ``rmsnorm``, ``swiglu_fused``: thin PyTorch extension
-  modules with the upstream Python-facing operator APIs, linked against
-  ``libqwen_b200.so`` (rpath ``$ORIGIN``).
+  modules with the upstream Python-facing operator APIs, and ``paged_C`` behind
+  ``paged.py``, linked against ``libqwen_b200.so`` (rpath ``$ORIGIN``).
 
 Everything is written next to this file, so the built ``.so`` files travel
 with a snapshot of the repository.  Rebuilds are mtime-based.
@@ -31,6 +31,7 @@ EXTENSIONS = {
     "qwen_megakernel_C": ["qwen_ops.cpp"],
     "rmsnorm": ["rmsnorm_ops.cpp"],
     "swiglu_fused": ["swiglu_ops.cpp"],
+    "paged_C": ["paged_ops.cpp"],
 }
 
 

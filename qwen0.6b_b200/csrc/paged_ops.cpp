@@ -1,0 +1,206 @@
+// paged_C: PyTorch extension module behind paged.py, the operators on paged KV
+// pools.  The kernels and their C ABI live in libqwen_b200.so
+// (include/qwen_b200_paged.h); this file checks tensors and allocates the
+// outputs.  Bad arguments raise ValueError, failed launches RuntimeError.
+// (Through ctypes the same checks in Python took 41 us per attention call,
+// three times its time on the device.)
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/extension.h>
+
+#include <optional>
+#include <tuple>
+
+#include "qwen_b200.h"
+#include "qwen_b200_paged.h"
+
+namespace {
+
+using torch::Tensor;
+
+void check_rc(int rc, const char *what) {
+  if (rc == 0) return;
+  char msg[512];
+  qwen_b200_last_error(msg, sizeof(msg));
+  // Codes of the C ABI that name a bad argument; the others are launch failures.
+  const bool argument = rc == 10 || rc == 11 || rc == 13 || rc == 14 || rc == 15;
+  TORCH_CHECK_VALUE(!argument, what, " failed (code ", rc, "): ", msg);
+  TORCH_CHECK(false, what, " failed (code ", rc, "): ", msg);
+}
+
+void *stream_of(const Tensor &t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+
+QwenPagePools pools_of(const Tensor &k, const Tensor &v) {
+  for (const Tensor *t : {&k, &v})
+    TORCH_CHECK_VALUE(t->is_cuda() && t->dim() >= 3 && t->is_contiguous() && t->numel() > 0,
+                      t == &k ? "k_pool" : "v_pool",
+                      " must be a contiguous, non-empty CUDA tensor [num_pages, ..., page_tokens, dim]");
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type() && k.device() == v.device(),
+                    "k_pool and v_pool must have the same shape, type and device");
+  const int64_t n = k.size(0), tokens = k.size(-2), bytes = k.size(-1) * k.element_size();
+  const int64_t inner = k.numel() / (n * tokens * k.size(-1));
+  TORCH_CHECK_VALUE(n < (1ll << 31) && tokens < (1ll << 31) && bytes < (1ll << 31) && inner < (1ll << 31),
+                    "pool dimensions over 2^31");
+  return QwenPagePools{k.data_ptr(), v.data_ptr(), static_cast<int>(n), static_cast<int>(inner),
+                       static_cast<int>(tokens), static_cast<int>(bytes)};
+}
+
+QwenPageTable table_of(const Tensor &t) {
+  TORCH_CHECK_VALUE(t.is_cuda() && t.dim() == 2 && t.scalar_type() == torch::kInt && t.numel() > 0 &&
+                        (t.stride(1) == 1 || t.size(1) == 1),
+                    "page_table must be a CUDA int32 tensor [num_seqs, max_pages] with contiguous rows");
+  TORCH_CHECK_VALUE(t.size(0) < (1ll << 31) && t.size(1) < (1ll << 31), "page_table dimensions over 2^31");
+  return QwenPageTable{t.data_ptr<int>(), static_cast<int>(t.size(0)), static_cast<int>(t.size(1)),
+                       t.size(0) > 1 ? t.stride(0) : t.size(1)};
+}
+
+// A host list: contiguous int32 on the CPU (paged.py makes it one).
+const int *list_of(const Tensor &t, const Tensor &first, const char *name) {
+  TORCH_CHECK_VALUE(t.device().is_cpu() && t.dim() == 1 && t.scalar_type() == torch::kInt && t.is_contiguous(), name,
+                    " must be a contiguous int32 list on the host");
+  TORCH_CHECK_VALUE(t.numel() == first.numel(), name, " has ", t.numel(), " entries, the other lists ", first.numel());
+  TORCH_CHECK_VALUE(t.numel() < (1ll << 31), name, " has over 2^31 entries");
+  return t.data_ptr<int>();
+}
+
+void same_device(const Tensor &t, const Tensor &k) {
+  TORCH_CHECK_VALUE(t.device() == k.device(), "page_table is on ", t.device(), ", the pools on ", k.device());
+}
+
+void copy_pages(const Tensor &k, const Tensor &v, const Tensor &src, const Tensor &dst,
+                const std::optional<Tensor> &tokens) {
+  const QwenPagePools p = pools_of(k, v);
+  const c10::cuda::CUDAGuard guard(k.device());
+  check_rc(qwen_b200_pages_copy(&p, list_of(src, src, "src"), list_of(dst, src, "dst"),
+                                tokens ? list_of(*tokens, src, "tokens") : nullptr, static_cast<int>(src.numel()),
+                                stream_of(k)),
+           "copy_pages");
+}
+
+void fork_pages(const Tensor &table, const Tensor &k, const Tensor &v, const Tensor &parents, const Tensor &children,
+                const Tensor &lengths, const Tensor &new_pages) {
+  const QwenPagePools p = pools_of(k, v);
+  const QwenPageTable t = table_of(table);
+  same_device(table, k);
+  const c10::cuda::CUDAGuard guard(k.device());
+  check_rc(qwen_b200_pages_fork(&p, &t, list_of(parents, parents, "parents"), list_of(children, parents, "children"),
+                                list_of(lengths, parents, "lengths"), list_of(new_pages, parents, "new_pages"),
+                                static_cast<int>(parents.numel()), stream_of(k)),
+           "fork_pages");
+}
+
+void compact_pages(const Tensor &table, const Tensor &k, const Tensor &v, const Tensor &src, const Tensor &dst) {
+  const QwenPagePools p = pools_of(k, v);
+  const QwenPageTable t = table_of(table);
+  same_device(table, k);
+  const c10::cuda::CUDAGuard guard(k.device());
+  check_rc(qwen_b200_pages_compact(&p, &t, list_of(src, src, "src"), list_of(dst, src, "dst"),
+                                   static_cast<int>(src.numel()), stream_of(k)),
+           "compact_pages");
+}
+
+void free_pages(const Tensor &table, const Tensor &seqs) {
+  const QwenPageTable t = table_of(table);
+  const c10::cuda::CUDAGuard guard(table.device());
+  check_rc(qwen_b200_pages_free(&t, list_of(seqs, seqs, "seqs"), static_cast<int>(seqs.numel()), stream_of(table)),
+           "free_pages");
+}
+
+// Stride of a dimension; that of a one-element dimension, which torch leaves
+// arbitrary, as in a contiguous tensor.
+int64_t stride_of(const Tensor &t, int64_t d) {
+  if (t.size(d) > 1) return t.stride(d);
+  int64_t s = 1;
+  for (int64_t i = d + 1; i < t.dim(); ++i) s *= t.size(i);
+  return s;
+}
+
+std::tuple<Tensor, std::optional<Tensor>> prefix_attention(
+    const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &table, const Tensor &seq_ids,
+    const Tensor &lengths, const Tensor &header, const Tensor &words, int64_t max_length, int64_t workspace_bytes,
+    std::optional<double> scale, const std::optional<Tensor> &out_, bool return_lse) {
+  TORCH_CHECK_VALUE(q.dim() == 3 && k.dim() == 4 && v.dim() == 4, "q must have 3 dimensions, the pools 4");
+  const auto type = q.scalar_type();
+  TORCH_CHECK_VALUE(type == torch::kHalf || type == torch::kBFloat16, "q must be an fp16 or bf16 tensor, got ", type);
+  TORCH_CHECK_VALUE(q.is_cuda() && q.device() == words.device(), "q is on ", q.device(), ", the plan on ",
+                    words.device());
+  for (const Tensor *t : {&k, &v})
+    TORCH_CHECK_VALUE(t->scalar_type() == type && t->device() == q.device(), "pools of ", t->scalar_type(), " on ",
+                      t->device(), ", q is ", type, " on ", q.device());
+  const int *h = header.data_ptr<int>();
+  const int64_t rows = q.size(0), heads = q.size(1), dim = q.size(2);
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes(), "k_pool and v_pool must have the same shape");
+  for (int d = 0; d < 3; ++d)
+    TORCH_CHECK_VALUE(stride_of(k, d) == stride_of(v, d), "k_pool and v_pool must have the same strides");
+  TORCH_CHECK_VALUE(k.size(3) == dim, "pools of dim ", k.size(3), ", q of dim ", dim);
+  TORCH_CHECK_VALUE(k.size(0) < (1ll << 31) && k.size(2) < (1ll << 31) && k.numel() > 0, "pool dimensions");
+  const QwenPageTable t = table_of(table);
+  TORCH_CHECK_VALUE(table.device() == q.device(), "page_table is on ", table.device(), ", q on ", q.device());
+  for (const Tensor *x : {&seq_ids, &lengths})
+    TORCH_CHECK_VALUE(x->scalar_type() == torch::kInt && x->dim() == 1 && x->size(0) == rows && x->is_contiguous() &&
+                          x->device() == q.device(),
+                      x == &lengths ? "lengths" : "seq_ids", " must be a contiguous int32 tensor [", rows, "] on ",
+                      q.device());
+  const c10::cuda::CUDAGuard guard(q.device());
+  Tensor out;
+  if (out_) {
+    out = *out_;
+    TORCH_CHECK_VALUE(out.sizes() == q.sizes() && out.scalar_type() == type && out.device() == q.device(),
+                      "out must have q's shape, type and device");
+    for (int d = 0; d < 2; ++d)
+      TORCH_CHECK_VALUE(out.size(d) == 1 || out.stride(d) >= dim, "out's rows or heads overlap");
+  } else {
+    out = torch::empty({rows, heads, dim}, q.options());
+  }
+  for (const Tensor *x : {&q, &k, &v, const_cast<const Tensor *>(&out)})
+    TORCH_CHECK_VALUE(x->size(-1) == 1 || x->stride(-1) == 1, "the last dimension must be contiguous");
+  std::optional<Tensor> lse;
+  if (return_lse) lse = torch::empty({rows, heads}, q.options().dtype(torch::kFloat));
+  // The workspace comes from the caching allocator with each call: calls on
+  // several streams, or captured into several graphs, have one each.
+  const Tensor ws = torch::empty({workspace_bytes}, q.options().dtype(torch::kByte));
+  QwenPrefixAttention a{};
+  a.q = q.data_ptr();
+  a.out = out.data_ptr();
+  a.lse = lse ? lse->data_ptr<float>() : nullptr;
+  a.k_pool = k.data_ptr();
+  a.v_pool = v.data_ptr();
+  a.page_table = t.entries;
+  a.seq_ids = seq_ids.data_ptr<int>();
+  a.lengths = lengths.data_ptr<int>();
+  a.plan_header = h;
+  a.plan = words.data_ptr<int>();
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = workspace_bytes;
+  a.q_row_stride = stride_of(q, 0);
+  a.q_head_stride = stride_of(q, 1);
+  a.out_row_stride = stride_of(out, 0);
+  a.out_head_stride = stride_of(out, 1);
+  a.page_stride = stride_of(k, 0);
+  a.head_stride = stride_of(k, 1);
+  a.token_stride = stride_of(k, 2);
+  a.table_pitch = t.pitch;
+  a.rows = static_cast<int>(rows);
+  a.heads = static_cast<int>(heads);
+  a.kv_heads = static_cast<int>(k.size(1));
+  a.dim = static_cast<int>(dim);
+  a.dtype = type == torch::kBFloat16;
+  a.num_pages = static_cast<int>(k.size(0));
+  a.page_tokens = static_cast<int>(k.size(2));
+  a.num_seqs = t.num_seqs;
+  a.max_pages = t.max_pages;
+  a.max_length = static_cast<int>(max_length);
+  a.scale = scale ? static_cast<float>(*scale) : static_cast<float>(1.0 / std::sqrt(static_cast<double>(dim)));
+  check_rc(qwen_b200_prefix_attention(&a, stream_of(q)), "shared_prefix_attention");
+  return {out, lse};
+}
+
+}  // namespace
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("copy_pages", &copy_pages);
+  m.def("fork_pages", &fork_pages);
+  m.def("compact_pages", &compact_pages);
+  m.def("free_pages", &free_pages);
+  m.def("prefix_attention", &prefix_attention);
+}

@@ -20,23 +20,36 @@
 namespace qb200p {
 
 constexpr int THREADS = 256;
-constexpr int UNROLL = 8;                  // 16-byte units in flight per thread
-constexpr int CTA_UNITS = THREADS * UNROLL * 2;  // 16-byte units of one copying CTA (64 KB)
+constexpr int UNROLL = 8;       // 16-byte units in flight per thread
+constexpr int MAX_DST = 8;      // destinations that one CTA writes from one read
 constexpr int TABLE_PER_CTA = THREADS * 4;
 
 __device__ unsigned long long g_paged_err;
 
-struct PageMove {
-  int src;     // source page (copy, compact) or parent sequence (fork)
-  int dst;     // destination page
-  int tokens;  // tokens to move
-  int cta0;    // first copying CTA of this entry
+// A run: consecutive list entries with one source and one token count, at
+// most MAX_DST of them; its destinations are dst[first ..] of the list.
+struct PageRun {
+  int src;     // source page (copy) or parent sequence (fork)
+  int tokens;  // tokens to move (fork: the length)
+  int cta0;    // first copying CTA of this run
+  int first;
 };
-
 template <int N>
-struct PageList {
+struct RunList {
+  int runs, n;
+  PageRun r[N];
+  int dst[N];
+};
+// fork: children beside the destinations (parents and lengths of all entries).
+template <int N>
+struct ForkList {
+  RunList<N> l;
+  int child[N], parent[N], length[N];
+};
+template <int N>
+struct MoveList {   // compact: sorted by source
   int n;
-  PageMove e[N];
+  int2 e[N];
 };
 template <int N>
 struct IntList {
@@ -61,32 +74,49 @@ struct MoveArgs {
   long long page_units;    // 16-byte units of a page (inner x page_tokens x token_units)
   int row_units;           // of one (layer, head) of a page: page_tokens x token_units
   int token_units, inner, num_pages;
+  int cta_units;           // units that one CTA moves
+  int late;                // not the call's first launch
   int *table;              // fork, compact
   long long pitch;
   int num_seqs, max_pages, page_tokens;
   int table_ctas;
 };
 
-// The last list entry whose first CTA is at or before `cta`.
+// A call's later launches touch other pages than its earlier ones, so their
+// CTAs start while the previous launch drains; they wait for it before they
+// end, so that whoever waits for the last launch has waited for all.  (They
+// can only start once every CTA of the first has passed its own wait.)
+__device__ __forceinline__ void enter(const MoveArgs &a) {
+  if (!a.late) qb200::griddep_wait();
+  qb200::griddep_launch_dependents();
+}
+__device__ __forceinline__ void leave(const MoveArgs &a) {
+  if (a.late) qb200::griddep_wait();
+}
+
+// The last run whose first CTA is at or before `cta`.
 template <int N>
-__device__ __forceinline__ int find_entry(const PageList<N> &l, int cta) {
-  int lo = 0, hi = l.n - 1;
+__device__ __forceinline__ int find_run(const RunList<N> &l, int cta) {
+  int lo = 0, hi = l.runs - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (l.e[mid].cta0 <= cta) lo = mid; else hi = mid - 1;
+    if (l.r[mid].cta0 <= cta) lo = mid; else hi = mid - 1;
   }
   return lo;
 }
 
-// One CTA's CTA_UNITS units of entry `m` in one pool: unit u of the entry is
-// 16 bytes of row u / (tokens x token_units), so a whole page is one
-// contiguous run.
-__device__ __forceinline__ void move_units(const MoveArgs &a, int pool, int src, const PageMove &m, int chunk) {
+// Units [chunk x cta_units, ..) of the first `tokens` tokens of page src to nd
+// pages of one pool.  Unit u of the tokens is 16 bytes of row u / (tokens x
+// token_units); a whole page is one contiguous run.  The units are read once
+// and written to every destination: 255 children of one parent read their
+// tail 32 times, not 255 times.
+template <typename Dst>
+__device__ __forceinline__ void move_units(const MoveArgs &a, int pool, int src, int tokens, int chunk, int nd,
+                                           Dst dst) {
   const uint4 *s = a.pool[pool] + static_cast<long long>(src) * a.page_units;
-  uint4 *d = a.pool[pool] + static_cast<long long>(m.dst) * a.page_units;
-  const unsigned row = static_cast<unsigned>(m.tokens) * a.token_units;  // units copied of one row
-  const unsigned total = row * static_cast<unsigned>(a.inner);           // host: fits 31 bits
-  const unsigned u0 = static_cast<unsigned>(chunk) * CTA_UNITS, u1 = min(total, u0 + CTA_UNITS);
+  const unsigned row = static_cast<unsigned>(tokens) * a.token_units;  // units copied of one row
+  const unsigned total = row * static_cast<unsigned>(a.inner);          // host: fits 31 bits
+  const unsigned u0 = static_cast<unsigned>(chunk) * a.cta_units, u1 = min(total, u0 + a.cta_units);
   const unsigned gap = static_cast<unsigned>(a.row_units) - row;  // units left out between rows
   for (unsigned u = u0 + threadIdx.x; u < u1; u += THREADS * UNROLL) {
     uint4 v[UNROLL];
@@ -97,101 +127,96 @@ __device__ __forceinline__ void move_units(const MoveArgs &a, int pool, int src,
       at[i] = gap == 0 ? x : x + (x / row) * gap;
       if (x < u1) v[i] = ld_stream(s + at[i]);
     }
+    for (int k = 0; k < nd; ++k) {
+      uint4 *d = a.pool[pool] + static_cast<long long>(dst(k)) * a.page_units;
 #pragma unroll
-    for (int i = 0; i < UNROLL; ++i)
-      if (u + i * THREADS < u1) d[at[i]] = v[i];
+      for (int i = 0; i < UNROLL; ++i)
+        if (u + i * THREADS < u1) d[at[i]] = v[i];
+    }
   }
 }
 
 // copy: grid (copying CTAs, 2 pools).
 template <int N>
 __global__ void __launch_bounds__(THREADS) pages_copy_kernel(const MoveArgs a,
-                                                             const __grid_constant__ PageList<N> list) {
-  qb200::griddep_wait();
-  qb200::griddep_launch_dependents();
-  const PageMove m = list.e[find_entry(list, blockIdx.x)];
-  move_units(a, blockIdx.y, m.src, m, blockIdx.x - m.cta0);
+                                                             const __grid_constant__ RunList<N> l) {
+  enter(a);
+  const int x = find_run(l, blockIdx.x);
+  const PageRun r = l.r[x];
+  const int end = x + 1 < l.runs ? l.r[x + 1].first : l.n;
+  move_units(a, blockIdx.y, r.src, r.tokens, blockIdx.x - r.cta0, end - r.first,
+             [&](int k) { return l.dst[r.first + k]; });
+  leave(a);
 }
-
-template <int N>
-struct ForkList {
-  int n;
-  PageMove e[N];   // src = parent, dst = new page, tokens = length
-  int child[N];
-};
 
 // fork: CTA (x < n, 0) writes child x's table row, the other CTAs copy tails.
 // Only children's rows are written and only parents' rows are read, and no
 // child is a parent.
 template <int N>
 __global__ void __launch_bounds__(THREADS) pages_fork_kernel(const MoveArgs a,
-                                                             const __grid_constant__ ForkList<N> list) {
-  qb200::griddep_wait();
-  qb200::griddep_launch_dependents();
+                                                             const __grid_constant__ ForkList<N> f) {
+  enter(a);
   if (static_cast<int>(blockIdx.x) < a.table_ctas) {
-    if (blockIdx.y != 0) return;
-    const PageMove m = list.e[blockIdx.x];
-    const int *from = a.table + m.src * a.pitch;
-    int *to = a.table + list.child[blockIdx.x] * a.pitch;
-    const int full = m.tokens / a.page_tokens, tail = m.tokens % a.page_tokens;
-    for (int i = threadIdx.x; i < a.max_pages; i += THREADS) to[i] = i < full ? from[i] : (i == full && tail ? m.dst : -1);
-    return;
+    if (blockIdx.y == 0) {
+      const int x = blockIdx.x;
+      const int *from = a.table + f.parent[x] * a.pitch;
+      int *to = a.table + f.child[x] * a.pitch;
+      const int full = f.length[x] / a.page_tokens, tail = f.length[x] % a.page_tokens;
+      for (int i = threadIdx.x; i < a.max_pages; i += THREADS)
+        to[i] = i < full ? from[i] : (i == full && tail ? f.l.dst[x] : -1);
+    }
+  } else {
+    const int cta = blockIdx.x - a.table_ctas;
+    const int x = find_run(f.l, cta);
+    const PageRun r = f.l.r[x];
+    const int end = x + 1 < f.l.runs ? f.l.r[x + 1].first : f.l.n;
+    const int src = a.table[r.src * a.pitch + r.tokens / a.page_tokens];
+    bool ok = src >= 0 && src < a.num_pages;
+    for (int k = r.first; k < end; ++k) ok = ok && src != f.l.dst[k];
+    if (ok)
+      move_units(a, blockIdx.y, src, r.tokens % a.page_tokens, cta - r.cta0, end - r.first,
+                 [&](int k) { return f.l.dst[r.first + k]; });
+    else if (threadIdx.x == 0)
+      record_err(3, static_cast<uint32_t>(r.src));
   }
-  const int cta = blockIdx.x - a.table_ctas;
-  int lo = 0, hi = list.n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (list.e[mid].cta0 <= cta) lo = mid; else hi = mid - 1;
-  }
-  PageMove m = list.e[lo];
-  const int src = a.table[m.src * a.pitch + m.tokens / a.page_tokens];
-  if (src < 0 || src >= a.num_pages || src == m.dst) {
-    if (threadIdx.x == 0) record_err(3, static_cast<uint32_t>(m.src));
-    return;
-  }
-  const int chunk = cta - m.cta0;
-  m.tokens %= a.page_tokens;
-  move_units(a, blockIdx.y, src, m, chunk);
+  leave(a);
 }
 
 // compact: the first table_ctas CTAs renumber the table (binary search in the
-// list, which the host sorted by source), the others move the pages.
+// sorted list), the others move the pages, per_page CTAs each.
 template <int N>
-__global__ void __launch_bounds__(THREADS) pages_compact_kernel(const MoveArgs a,
-                                                                const __grid_constant__ PageList<N> list,
-                                                                const __grid_constant__ PageList<N> by_src) {
-  qb200::griddep_wait();
-  qb200::griddep_launch_dependents();
+__global__ void __launch_bounds__(THREADS) pages_compact_kernel(const MoveArgs a, int per_page,
+                                                                const __grid_constant__ MoveList<N> l) {
+  enter(a);
   if (static_cast<int>(blockIdx.x) < a.table_ctas) {
-    if (blockIdx.y != 0) return;
     const long long total = static_cast<long long>(a.num_seqs) * a.max_pages;
-    for (int k = 0; k < TABLE_PER_CTA / THREADS; ++k) {
+    for (int k = 0; k < TABLE_PER_CTA / THREADS && blockIdx.y == 0; ++k) {
       const long long i = static_cast<long long>(blockIdx.x) * TABLE_PER_CTA + k * THREADS + threadIdx.x;
-      if (i >= total) return;
+      if (i >= total) break;
       int *p = a.table + (i / a.max_pages) * a.pitch + i % a.max_pages;
       const int page = *p;
       if (page < 0) continue;
-      int lo = 0, hi = by_src.n - 1;
+      int lo = 0, hi = l.n - 1;
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (by_src.e[mid].src <= page) lo = mid; else hi = mid - 1;
+        if (l.e[mid].x <= page) lo = mid; else hi = mid - 1;
       }
-      if (by_src.e[lo].src == page) *p = by_src.e[lo].dst;
+      if (l.e[lo].x == page) *p = l.e[lo].y;
     }
-    return;
+  } else {
+    const int cta = blockIdx.x - a.table_ctas, x = cta / per_page;
+    const int to = l.e[x].y;
+    move_units(a, blockIdx.y, l.e[x].x, a.page_tokens, cta - x * per_page, 1, [&](int) { return to; });
   }
-  const int cta = blockIdx.x - a.table_ctas;
-  const PageMove m = list.e[find_entry(list, cta)];
-  move_units(a, blockIdx.y, m.src, m, cta - m.cta0);
+  leave(a);
 }
 
 template <int N>
-__global__ void __launch_bounds__(THREADS) pages_free_kernel(int *table, long long pitch, int max_pages,
-                                                             const __grid_constant__ IntList<N> list) {
-  qb200::griddep_wait();
-  qb200::griddep_launch_dependents();
-  int *row = table + list.v[blockIdx.x] * pitch;
-  for (int i = threadIdx.x; i < max_pages; i += THREADS) row[i] = -1;
+__global__ void __launch_bounds__(THREADS) pages_free_kernel(const MoveArgs a, const __grid_constant__ IntList<N> l) {
+  enter(a);
+  int *row = a.table + l.v[blockIdx.x] * a.pitch;
+  for (int i = threadIdx.x; i < a.max_pages; i += THREADS) row[i] = -1;
+  leave(a);
 }
 
 }  // namespace qb200p
@@ -201,7 +226,11 @@ using namespace qb200p;
 
 namespace {
 
-constexpr int SMALL = 64, LARGE = 1024;  // list entries of a launch: 1 KB or 16 to 20 KB of parameters
+// Entries of one launch's list: they are kernel parameters, of which a launch
+// takes 32,764 bytes; a short list is its own kernel so that it does not carry
+// the long one's bytes.
+constexpr int SMALL = 64;
+constexpr int COPY_LARGE = 1024, FORK_LARGE = 768, MOVE_LARGE = 3840, FREE_LARGE = 4096;
 
 int fail(int code, const char *fmt, ...) {
   char buf[512];
@@ -265,14 +294,16 @@ int check_moves(int num_pages, const int *src, const int *dst, int n, bool disti
 
 MoveArgs move_args(const QwenPagePools *p, const QwenPageTable *t) {
   MoveArgs a{};
-  a.pool[0] = static_cast<uint4 *>(p->k_pool);
-  a.pool[1] = static_cast<uint4 *>(p->v_pool);
-  a.token_units = p->token_bytes / 16;
-  a.row_units = p->page_tokens * a.token_units;
-  a.inner = p->inner;
-  a.page_units = static_cast<long long>(a.row_units) * p->inner;
-  a.num_pages = p->num_pages;
-  a.page_tokens = p->page_tokens;
+  if (p != nullptr) {
+    a.pool[0] = static_cast<uint4 *>(p->k_pool);
+    a.pool[1] = static_cast<uint4 *>(p->v_pool);
+    a.token_units = p->token_bytes / 16;
+    a.row_units = p->page_tokens * a.token_units;
+    a.inner = p->inner;
+    a.page_units = static_cast<long long>(a.row_units) * p->inner;
+    a.num_pages = p->num_pages;
+    a.page_tokens = p->page_tokens;
+  }
   if (t != nullptr) {
     a.table = t->entries;
     a.pitch = t->pitch;
@@ -282,10 +313,16 @@ MoveArgs move_args(const QwenPagePools *p, const QwenPageTable *t) {
   return a;
 }
 
-// Copying CTAs for `tokens` tokens of a page.
-long long ctas_of(const MoveArgs &a, int tokens) {
-  return (static_cast<long long>(tokens) * a.token_units * a.inner + CTA_UNITS - 1) / CTA_UNITS;
+// Units of one CTA for `units` units in all (one pool): 64 KB, less while
+// that would leave the device with fewer than two CTAs per SM.
+int cta_units_for(long long units) {
+  int c = THREADS * UNROLL * 2;
+  while (c > THREADS * 2 && units / c < 148) c /= 2;
+  return c;
 }
+
+long long units_of(const MoveArgs &a, int tokens) { return static_cast<long long>(tokens) * a.token_units * a.inner; }
+long long ctas_of(const MoveArgs &a, int tokens) { return (units_of(a, tokens) + a.cta_units - 1) / a.cta_units; }
 
 #define LAUNCH(kernel, grid, ...)                                                                      \
   do {                                                                                                 \
@@ -293,72 +330,86 @@ long long ctas_of(const MoveArgs &a, int tokens) {
     if (le != cudaSuccess) return fail(20, "page operator launch: %s", cudaGetErrorString(le));         \
   } while (0)
 
-// Fills `list` with entries [i, n) until it is full; returns the next i and
-// the copying CTAs.
+// Appends entry (src, tokens) -> dst to a list's runs.  `moved`: tokens that
+// are copied.  False when the grid is full.
 template <int N>
-int launch_copy(const MoveArgs &a, const int *src, const int *dst, const int *tokens, int &i, int n,
-                cudaStream_t st) {
-  PageList<N> l;
-  l.n = 0;
-  long long ctas = 0;
-  for (; i < n && l.n < N; ++i) {
-    const int t = tokens != nullptr ? tokens[i] : a.page_tokens;
-    const long long c = ctas_of(a, t);
-    if (c == 0) continue;
-    if (ctas + c > 0x7fffffffll) break;
-    l.e[l.n++] = PageMove{src[i], dst[i], t, static_cast<int>(ctas)};
+bool append(RunList<N> &l, const MoveArgs &a, int src, int tokens, int moved, int dst, long long &ctas) {
+  const long long c = ctas_of(a, moved);
+  if (l.runs == 0 || l.r[l.runs - 1].src != src || l.r[l.runs - 1].tokens != tokens ||
+      l.n - l.r[l.runs - 1].first >= MAX_DST) {
+    if (ctas + c > 0x70000000ll) return false;
+    l.r[l.runs++] = PageRun{src, tokens, static_cast<int>(ctas), l.n};
     ctas += c;
   }
-  if (ctas > 0) LAUNCH(pages_copy_kernel<N>, dim3(static_cast<unsigned>(ctas), 2), a, l);
+  l.dst[l.n++] = dst;
+  return true;
+}
+
+// Each launch_* takes entries from [i, n) until its list is full.
+template <int N>
+int launch_copy(MoveArgs &a, const int *src, const int *dst, const int *tokens, int &i, int n, cudaStream_t st) {
+  RunList<N> l;
+  l.runs = l.n = 0;
+  long long ctas = 0, units = 0;
+  for (int k = i; k < n && k < i + N; ++k) units += units_of(a, tokens != nullptr ? tokens[k] : a.page_tokens);
+  a.cta_units = cta_units_for(units);
+  for (; i < n && l.n < N; ++i) {
+    const int t = tokens != nullptr ? tokens[i] : a.page_tokens;
+    if (t > 0 && !append(l, a, src[i], t, t, dst[i], ctas)) break;
+  }
+  if (ctas == 0) return 0;
+  LAUNCH(pages_copy_kernel<N>, dim3(static_cast<unsigned>(ctas), 2), a, l);
+  a.late = 1;
   return 0;
 }
 
 template <int N>
-int launch_fork(MoveArgs a, const int *parents, const int *children, const int *lengths, const int *new_pages, int &i,
+int launch_fork(MoveArgs &a, const int *parents, const int *children, const int *lengths, const int *new_pages, int &i,
                 int n, cudaStream_t st) {
-  ForkList<N> l;
-  l.n = 0;
-  long long ctas = 0;
-  for (; i < n && l.n < N; ++i) {
-    const long long c = ctas_of(a, lengths[i] % a.page_tokens);
-    if (ctas + c > 0x70000000ll) break;
-    l.child[l.n] = children[i];
-    l.e[l.n++] = PageMove{parents[i], new_pages[i], lengths[i], static_cast<int>(ctas)};
-    ctas += c;
+  ForkList<N> f;
+  f.l.runs = f.l.n = 0;
+  long long ctas = 0, units = 0;
+  for (int k = i; k < n && k < i + N; ++k) units += units_of(a, lengths[k] % a.page_tokens);
+  a.cta_units = cta_units_for(units);
+  for (; i < n && f.l.n < N; ++i) {
+    const int k = f.l.n;
+    if (!append(f.l, a, parents[i], lengths[i], lengths[i] % a.page_tokens, new_pages[i], ctas)) break;
+    f.child[k] = children[i];
+    f.parent[k] = parents[i];
+    f.length[k] = lengths[i];
   }
-  a.table_ctas = l.n;
-  LAUNCH(pages_fork_kernel<N>, dim3(static_cast<unsigned>(ctas + l.n), 2), a, l);
+  a.table_ctas = f.l.n;
+  LAUNCH(pages_fork_kernel<N>, dim3(static_cast<unsigned>(ctas + a.table_ctas), 2), a, f);
+  a.late = 1;
   return 0;
 }
 
 int by_source(const void *x, const void *y) {
-  const int a = static_cast<const PageMove *>(x)->src, b = static_cast<const PageMove *>(y)->src;
+  const int a = static_cast<const int2 *>(x)->x, b = static_cast<const int2 *>(y)->x;
   return (a > b) - (a < b);
 }
 
 template <int N>
-int launch_compact(MoveArgs a, const int *src, const int *dst, int &i, int n, cudaStream_t st) {
-  PageList<N> l, s;
+int launch_compact(MoveArgs &a, const int *src, const int *dst, int &i, int n, cudaStream_t st) {
+  MoveList<N> l;
   l.n = 0;
-  long long ctas = 0;
+  a.cta_units = cta_units_for(units_of(a, a.page_tokens) * (n - i < N ? n - i : N));
   const long long c = ctas_of(a, a.page_tokens);
-  for (; i < n && l.n < N && ctas + c <= 0x70000000ll; ++i) {
-    l.e[l.n++] = PageMove{src[i], dst[i], a.page_tokens, static_cast<int>(ctas)};
-    ctas += c;
-  }
-  s = l;
-  qsort(s.e, s.n, sizeof(PageMove), by_source);
+  for (; i < n && l.n < N && (l.n == 0 || (l.n + 1) * c <= 0x70000000ll); ++i) l.e[l.n++] = make_int2(src[i], dst[i]);
+  qsort(l.e, l.n, sizeof(int2), by_source);
   a.table_ctas = static_cast<int>((static_cast<long long>(a.num_seqs) * a.max_pages + TABLE_PER_CTA - 1) / TABLE_PER_CTA);
-  LAUNCH(pages_compact_kernel<N>, dim3(static_cast<unsigned>(ctas + a.table_ctas), 2), a, l, s);
+  LAUNCH(pages_compact_kernel<N>, dim3(static_cast<unsigned>(l.n * c + a.table_ctas), 2), a, static_cast<int>(c), l);
+  // The next launch renumbers the same table: it has to see this one's.
   return 0;
 }
 
 template <int N>
-int launch_free(const QwenPageTable *t, const int *seqs, int &i, int n, cudaStream_t st) {
+int launch_free(MoveArgs &a, const int *seqs, int &i, int n, cudaStream_t st) {
   IntList<N> l;
   l.n = 0;
   for (; i < n && l.n < N; ++i) l.v[l.n++] = seqs[i];
-  LAUNCH(pages_free_kernel<N>, dim3(static_cast<unsigned>(l.n)), t->entries, t->pitch, t->max_pages, l);
+  LAUNCH(pages_free_kernel<N>, dim3(static_cast<unsigned>(l.n)), a, l);
+  a.late = 1;
   return 0;
 }
 #undef LAUNCH
@@ -378,11 +429,11 @@ int qwen_b200_pages_copy(const QwenPagePools *pools, const int *src, const int *
   for (int i = 0; tokens != nullptr && i < n; ++i)
     if (tokens[i] < 0 || tokens[i] > pools->page_tokens)
       return fail(11, "entry %d: %d tokens of a page of %d", i, tokens[i], pools->page_tokens);
-  const MoveArgs a = move_args(pools, nullptr);
+  MoveArgs a = move_args(pools, nullptr);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   for (int i = 0; i < n;)
     if (int rc = n - i <= SMALL ? launch_copy<SMALL>(a, src, dst, tokens, i, n, st)
-                                : launch_copy<LARGE>(a, src, dst, tokens, i, n, st))
+                                : launch_copy<COPY_LARGE>(a, src, dst, tokens, i, n, st))
       return rc;
   return 0;
 }
@@ -420,11 +471,11 @@ int qwen_b200_pages_fork(const QwenPagePools *pools, const QwenPageTable *table,
       seqs.m[children[i]] |= 2;
     }
   }
-  const MoveArgs a = move_args(pools, table);
+  MoveArgs a = move_args(pools, table);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   for (int i = 0; i < n;)
     if (int rc = n - i <= SMALL ? launch_fork<SMALL>(a, parents, children, lengths, new_pages, i, n, st)
-                                : launch_fork<LARGE>(a, parents, children, lengths, new_pages, i, n, st))
+                                : launch_fork<FORK_LARGE>(a, parents, children, lengths, new_pages, i, n, st))
       return rc;
   return 0;
 }
@@ -438,11 +489,11 @@ int qwen_b200_pages_compact(const QwenPagePools *pools, const QwenPageTable *tab
   if (n == 0) return 0;
   if (src == nullptr || dst == nullptr) return fail(13, "null list");
   if (int rc = check_moves(pools->num_pages, src, dst, n, true)) return rc;
-  const MoveArgs a = move_args(pools, table);
+  MoveArgs a = move_args(pools, table);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   for (int i = 0; i < n;)
     if (int rc = n - i <= SMALL ? launch_compact<SMALL>(a, src, dst, i, n, st)
-                                : launch_compact<LARGE / 2>(a, src, dst, i, n, st))
+                                : launch_compact<MOVE_LARGE>(a, src, dst, i, n, st))
       return rc;
   return 0;
 }
@@ -457,8 +508,9 @@ int qwen_b200_pages_free(const QwenPageTable *table, const int *seqs, int n, voi
     if (seqs[i] < 0 || seqs[i] >= table->num_seqs)
       return fail(11, "entry %d: sequence %d outside the table of %d", i, seqs[i], table->num_seqs);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  MoveArgs a = move_args(nullptr, table);
   for (int i = 0; i < n;)
-    if (int rc = n - i <= SMALL ? launch_free<SMALL>(table, seqs, i, n, st) : launch_free<LARGE>(table, seqs, i, n, st))
+    if (int rc = n - i <= SMALL ? launch_free<SMALL>(a, seqs, i, n, st) : launch_free<FREE_LARGE>(a, seqs, i, n, st))
       return rc;
   return 0;
 }

@@ -68,9 +68,9 @@ struct Seg {
   int dual;     // more than 128 queries in the tile
 };
 // Per row: the group's prefix (0: none), the group's first query tile, the
-// row's first query in the group.
+// row's first query in the group, the queries of the group.
 struct RowPlan {
-  int prefix, tile0, query, pad;
+  int prefix, tile0, query, queries;
 };
 
 constexpr int TN = 128;      // tokens of a tile
@@ -83,7 +83,10 @@ struct Args {
   void *out;
   float *lse;
   const int *page_table, *seq_ids, *lengths;
-  const int *plan;
+  const int *cta_seg;      // parts of the plan
+  const Seg *segs;
+  const int *tile_slot;
+  const RowPlan *row_plan;
   float *slots;        // prefix partials
   float *own;          // own partials
   long long q_row, q_head, o_row, o_head;
@@ -94,6 +97,7 @@ struct Args {
   int rows, heads, kv_heads, ratio;
   int num_pages, page_tokens, box, num_seqs, max_pages;
   int length_bias, own_splits;
+  int after_prefix;    // the own kernel follows a prefix kernel of the same call
   float scale_log2;
 };
 
@@ -248,8 +252,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   qb200::griddep_wait();
   if (threadIdx.x == 0) qb200::griddep_launch_dependents();
 
-  const int seg0 = a.plan[a.plan[PW_CTA_SEG] + blockIdx.x], seg1 = a.plan[a.plan[PW_CTA_SEG] + blockIdx.x + 1];
-  const Seg *segs = reinterpret_cast<const Seg *>(a.plan + a.plan[PW_SEG]);
+  const int seg0 = a.cta_seg[blockIdx.x], seg1 = a.cta_seg[blockIdx.x + 1];
+  const Seg *segs = a.segs;
   const int boxes = TN / a.box;
 
   // Page holding box b of token tile t of the segment's prefix, or num_pages
@@ -563,205 +567,12 @@ __device__ __forceinline__ uint4 ld_kv(const void *p, bool on) {
 }
 __device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-// grid (splits, kv heads x head tiles of 8, rows), 4 warps.  The CTA takes
-// positions [start + split * per, ...) of its row, its warps blocks of 16
-// tokens in turn, each with its own online softmax; the four join through
-// shared memory.  Per block, with tokens on the M side of the products:
-//   S^T[16 tokens, 8 heads] = K Q^T, O^T[D dims, 8 heads] += V^T P^T.
-// K fragments come straight from global memory: lane (g, c) = (lane / 4,
-// lane % 4) reads 16 bytes at dims 32 i + 8 c of tokens g and g + 8, and the
-// contraction runs over the dims in that order on both sides.  V likewise:
-// the lane reads tokens 2c, 2c+1, 2c+8, 2c+9 at dims 64 i + 8 g and pairs
-// tokens with byte permutes, which is the transposed operand.
-template <typename T, int D>
-__global__ void __launch_bounds__(OWN_THREADS) own_kernel(const Args a) {
-  qb200::griddep_wait();
-  qb200::griddep_launch_dependents();
-  constexpr int KI = D / 32;  // 16-byte chunks of a token per lane (scores)
-  constexpr int VI = D / 64;  // 16-byte chunks of a token per lane (values)
-  __shared__ float s_m[4][8], s_l[4][8];
-  __shared__ __align__(16) float s_o[4][8][D + 4];
-  const int split = blockIdx.x, row = blockIdx.z;
-  const int htiles = (a.ratio + 7) >> 3;
-  const int kvh = blockIdx.y / htiles, h0 = (blockIdx.y % htiles) * 8;
-  const int nh = min(8, a.ratio - h0);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  int seq;
-  const int len = row_length(a, row, &seq);
-  const RowPlan rp = reinterpret_cast<const RowPlan *>(a.plan + a.plan[PW_ROW])[row];
-  if (len < 0) {
-    if (threadIdx.x == 0) gemm_record(a.err, 3);
-  }
-  const int start = len >= rp.prefix ? rp.prefix : 0;
-  const int count = max(0, len - start);
-  // Tokens of one split: a multiple of 64 that covers the row.
-  const int per = ((count + a.own_splits - 1) / a.own_splits + 63) / 64 * 64;
-  const int lo = start + split * per, hi = min(len, lo + per);
-  float *part = a.own + ((static_cast<size_t>(row) * a.heads + kvh * a.ratio + h0) * a.own_splits + split) * (D + 2);
-  const size_t part_head = static_cast<size_t>(a.own_splits) * (D + 2);
-  if (lo >= hi) {
-    if (static_cast<int>(threadIdx.x) < nh) {
-      part[threadIdx.x * part_head + D] = -INFINITY;
-      part[threadIdx.x * part_head + D + 1] = 0.f;
-    }
-    return;
-  }
-  const int *trow = a.page_table + seq * a.table_pitch;
-  const T *kp = static_cast<const T *>(a.k_pool) + kvh * a.head_stride;
-  const T *vp = static_cast<const T *>(a.v_pool) + kvh * a.head_stride;
-
-  // Q^T as the B operand: n = head g, k = dims in the order of the K loads.
-  uint32_t qb[KI][4];
-  {
-    const T *qr = static_cast<const T *>(a.q) + row * a.q_row + (kvh * a.ratio + h0 + g) * a.q_head;
-#pragma unroll
-    for (int i = 0; i < KI; ++i) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (g < nh) v = *reinterpret_cast<const uint4 *>(qr + 32 * i + 8 * c);
-      qb[i][0] = v.x; qb[i][1] = v.y; qb[i][2] = v.z; qb[i][3] = v.w;
-    }
-  }
-  float o[VI][4][2][2][2];  // [dims 64 i][m tile][rows g | g + 8][...]: see below
-  // O^T tile (i, e): rows = dims 64 i + 8 g + e (rows g) and 64 i + 8 g + e + 4
-  // (rows g + 8), columns = heads 2c, 2c + 1.
-#pragma unroll
-  for (int i = 0; i < VI; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-#pragma unroll
-      for (int x = 0; x < 2; ++x) o[i][e][x][0][0] = o[i][e][x][0][1] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // heads 2c, 2c + 1
-  bool seen = false;
-
-  for (int b = lo + 16 * warp; b < hi; b += 64) {
-    const int pi = b / a.page_tokens;
-    const int page = trow[pi];
-    if (page < 0 || page >= a.num_pages) {
-      if (lane == 0) gemm_record(a.err, 3);
-      continue;
-    }
-    const long long at = page * a.page_stride + static_cast<long long>(b - pi * a.page_tokens) * a.token_stride;
-    const int n = min(16, hi - b);
-    uint4 kv[2][KI], vv[4][VI];
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int i = 0; i < KI; ++i)
-        kv[x][i] = ld_kv(kp + at + (g + 8 * x) * a.token_stride + 32 * i + 8 * c, g + 8 * x < n);
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int tok = 2 * c + (x & 1) + 8 * (x >> 1);
-#pragma unroll
-      for (int i = 0; i < VI; ++i) vv[x][i] = ld_kv(vp + at + tok * a.token_stride + 64 * i + 8 * g, tok < n);
-    }
-    float s[4] = {0.f, 0.f, 0.f, 0.f};  // (token g, heads 2c, 2c+1), (token g + 8, ...)
-#pragma unroll
-    for (int i = 0; i < KI; ++i) {
-      mma16816<T>(s, kv[0][i].x, kv[1][i].x, kv[0][i].y, kv[1][i].y, qb[i][0], qb[i][1]);
-      mma16816<T>(s, kv[0][i].z, kv[1][i].z, kv[0][i].w, kv[1][i].w, qb[i][2], qb[i][3]);
-    }
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) s[2 * x + h] = g + 8 * x < n ? s[2 * x + h] * a.scale_log2 : -INFINITY;
-    float p[4];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float mx = fmaxf(s[h], s[2 + h]);
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-      const float mn = fmaxf(m[h], mx);
-      const float mu = mn == -INFINITY ? 0.f : mn;
-      const float f = ex2_approx(m[h] - mu);
-      p[h] = ex2_approx(s[h] - mu);
-      p[2 + h] = ex2_approx(s[2 + h] - mu);
-      l[h] = l[h] * f + (p[h] + p[2 + h]);
-      m[h] = mn;
-#pragma unroll
-      for (int i = 0; i < VI; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          o[i][e][0][0][h] *= f;
-          o[i][e][1][0][h] *= f;
-        }
-    }
-    seen = true;
-    // P^T as the B operand (n = head g, k = tokens 2c, 2c+1 / 2c+8, 2c+9).
-    const uint32_t b0 = transpose8x8(Type<T>::pack(p[0], p[1]));
-    const uint32_t b1 = transpose8x8(Type<T>::pack(p[2], p[3]));
-#pragma unroll
-    for (int i = 0; i < VI; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        // A rows g: dim 8 g + e; rows g + 8: dim 8 g + e + 4.
-        const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
-        const int w0 = e >> 1, w1 = 2 + (e >> 1);
-        const uint32_t a0 = __byte_perm(word(vv[0][i], w0), word(vv[1][i], w0), sel);
-        const uint32_t a1 = __byte_perm(word(vv[0][i], w1), word(vv[1][i], w1), sel);
-        const uint32_t a2 = __byte_perm(word(vv[2][i], w0), word(vv[3][i], w0), sel);
-        const uint32_t a3 = __byte_perm(word(vv[2][i], w1), word(vv[3][i], w1), sel);
-        float d[4] = {o[i][e][0][0][0], o[i][e][0][0][1], o[i][e][1][0][0], o[i][e][1][0][1]};
-        mma16816<T>(d, a0, a1, a2, a3, b0, b1);
-        o[i][e][0][0][0] = d[0];
-        o[i][e][0][0][1] = d[1];
-        o[i][e][1][0][0] = d[2];
-        o[i][e][1][0][1] = d[3];
-      }
-  }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 4);
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 8);
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 16);
-    // Seen tokens whose scores are all -inf: as in the prefix kernel.
-    if (seen && m[h] == -INFINITY) l[h] = 1.f;
-    if (g == 0) {
-      s_m[warp][2 * c + h] = m[h];
-      s_l[warp][2 * c + h] = l[h];
-    }
-#pragma unroll
-    for (int i = 0; i < VI; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s_o[warp][2 * c + h][64 * i + 8 * g + e] = o[i][e][0][0][h];
-        s_o[warp][2 * c + h][64 * i + 8 * g + e + 4] = o[i][e][1][0][h];
-      }
-  }
-  __syncthreads();
-  for (int x = threadIdx.x; x < nh * D; x += OWN_THREADS) {
-    const int h = x / D, d = x % D;
-    float mm = fmaxf(fmaxf(s_m[0][h], s_m[1][h]), fmaxf(s_m[2][h], s_m[3][h]));
-    float acc = 0.f, sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = mm == -INFINITY ? 1.f : ex2_approx(s_m[w][h] - mm);
-      acc += s_m[w][h] == -INFINITY ? 0.f : s_o[w][h][d] * f;
-      sum += s_m[w][h] == -INFINITY && mm != -INFINITY ? 0.f : s_l[w][h] * f;
-    }
-    part[h * part_head + d] = acc;
-    if (d == 0) {
-      part[h * part_head + D] = mm;
-      part[h * part_head + D + 1] = sum;
-    }
-  }
-}
-
-// -------------------------------------------------------------- join kernel
-// grid (heads, rows), 32 lanes of D / 32 dims: every partial of the row's
-// prefix tile, then of its own splits, in that order.
-template <typename T, int D>
-__global__ void __launch_bounds__(D / 4) join_kernel(const Args a) {
-  qb200::griddep_wait();
-  qb200::griddep_launch_dependents();
-  const int head = blockIdx.x, row = blockIdx.y, lane = threadIdx.x;  // lane: 4 dims
-  int seq;
-  const int len = row_length(a, row, &seq);
-  const RowPlan rp = reinterpret_cast<const RowPlan *>(a.plan + a.plan[PW_ROW])[row];
+// The running join of partial results (m, l, a) of four dims of a query.
+struct Joined {
   float m = -INFINITY, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float none = 0.f;  // visible parts whose scores are all -inf
-  auto add = [&](float mi, float li, const float4 &v) {
+  __device__ __forceinline__ void add(float mi, float li, const float4 &v) {
     if (mi == -INFINITY) {
       none += li;
       return;
@@ -774,48 +585,322 @@ __global__ void __launch_bounds__(D / 4) join_kernel(const Args a) {
     acc.z = acc.z * f + v.z * h;
     acc.w = acc.w * f + v.w * h;
     m = mn;
-  };
-  if (rp.prefix > 0 && len >= rp.prefix) {
-    const int kvh = head / a.ratio, qi = rp.query + head % a.ratio;
-    const int tile = rp.tile0 + (qi / (2 * QT)) * a.kv_heads + kvh;
-    const int *ts = a.plan + a.plan[PW_TILE_SLOT];
-    const Seg *segs = reinterpret_cast<const Seg *>(a.plan + a.plan[PW_SEG]);
-    const int s0 = ts[tile], s1 = ts[tile + 1];
-    const bool dual = segs[s0].dual != 0;
-    const int ql = qi % QT, st0 = dual ? (qi / QT) & 1 : 0, st1 = dual ? st0 + 1 : 2;
-    for (int s = s0; s < s1; ++s)
-      for (int st = st0; st < st1; ++st) {
-        if (!dual && st == 1 && segs[s].t1 - segs[s].t0 < 2) continue;  // the stream had no tile
-        const float *slot = a.slots + (static_cast<size_t>(s) * 2 + st) * kStreamFloats<D>;
-        add(slot[QT * D + ql], slot[QT * D + QT + ql], reinterpret_cast<const float4 *>(slot)[lane * QT + ql]);
+  }
+};
+
+// Partial results of the prefix for one query: count of them, and where the
+// k-th lies.
+struct PrefixParts {
+  int first, count, ql;  // first stream slot, slots, query within the stream
+  int step;              // stream slots between two of them
+};
+__device__ __forceinline__ PrefixParts prefix_parts(const Args &a, const RowPlan &rp, int head) {
+  const int kvh = head / a.ratio, qi = rp.query + head % a.ratio;
+  const int tile = rp.tile0 + (qi / (2 * QT)) * a.kv_heads + kvh;
+  const int s0 = a.tile_slot[tile], s1 = a.tile_slot[tile + 1];
+  PrefixParts p;
+  p.ql = qi % QT;
+  if (rp.queries - qi / (2 * QT) * (2 * QT) > QT) {  // dual: the query's own stream of every slot
+    p.first = 2 * s0 + ((qi / QT) & 1);
+    p.count = s1 - s0;
+    p.step = 2;
+  } else {                                           // single: both streams (an idle one left m = -inf, l = 0)
+    p.first = 2 * s0;
+    p.count = 2 * (s1 - s0);
+    p.step = 1;
+  }
+  return p;
+}
+
+// Joins partials k0, k0 + dk, ... of a query's prefix, dims 4 d4 .. 4 d4 + 3;
+// four are requested before the first is used.
+template <int D>
+__device__ __forceinline__ void join_prefix(const Args &a, const PrefixParts &p, int d4, int k0, int dk, Joined &j) {
+  for (int k = k0; k < p.count; k += 4 * dk) {
+    float m[4], l[4];
+    float4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      m[u] = -INFINITY;
+      l[u] = 0.f;
+      v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (k + u * dk < p.count) {
+        const float *slot = a.slots + static_cast<size_t>(p.first + (k + u * dk) * p.step) * kStreamFloats<D>;
+        m[u] = slot[QT * D + p.ql];
+        l[u] = slot[QT * D + QT + p.ql];
+        v[u] = reinterpret_cast<const float4 *>(slot)[d4 * QT + p.ql];
       }
-  }
-  const float *own = a.own + (static_cast<size_t>(row) * a.heads + head) * a.own_splits * (D + 2);
-  if (len > 0) {
-    const int start = len >= rp.prefix ? rp.prefix : 0;
-    const int count = len - start;
-    const int per = ((count + a.own_splits - 1) / a.own_splits + 63) / 64 * 64;
-    const int ns = count > 0 ? (count + per - 1) / per : 0;
-    for (int s = 0; s < ns; ++s) {
-      const float *p = own + static_cast<size_t>(s) * (D + 2);
-      add(p[D], p[D + 1], make_float4(p[4 * lane], p[4 * lane + 1], p[4 * lane + 2], p[4 * lane + 3]));
     }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) j.add(m[u], l[u], v[u]);
   }
-  float lse;
-  if (m == -INFINITY) {  // nothing seen: 0; nothing but -inf: NaN
-    const float x = none > 0.f ? __int_as_float(0x7fffffff) : 0.f;
-    acc = make_float4(x, x, x, x);
-    lse = -INFINITY;
+}
+
+// The row's output for dims 4 d4 .. of a head, and its lse (once).
+template <typename T>
+__device__ __forceinline__ void put_result(const Args &a, int row, int head, int d4, const Joined &j) {
+  float lse = -INFINITY;
+  float4 o;
+  if (j.m == -INFINITY) {  // nothing seen: 0; nothing but -inf: NaN
+    const float x = j.none > 0.f ? __int_as_float(0x7fffffff) : 0.f;
+    o = make_float4(x, x, x, x);
   } else {
-    const float inv = 1.f / l;
-    acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-    lse = (m + log2f(l)) * 0.6931471805599453f;
+    const float inv = 1.f / j.l;
+    o = make_float4(j.acc.x * inv, j.acc.y * inv, j.acc.z * inv, j.acc.w * inv);
+    lse = (j.m + log2f(j.l)) * 0.6931471805599453f;
   }
   uint2 w;
-  w.x = Type<T>::pack(acc.x, acc.y);
-  w.y = Type<T>::pack(acc.z, acc.w);
-  *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + row * a.o_row + head * a.o_head + 4 * lane) = w;
-  if (lane == 0 && a.lse != nullptr) a.lse[static_cast<size_t>(row) * a.heads + head] = lse;
+  w.x = Type<T>::pack(o.x, o.y);
+  w.y = Type<T>::pack(o.z, o.w);
+  *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + row * a.o_row + head * a.o_head + 4 * d4) = w;
+  if (d4 == 0 && a.lse != nullptr) a.lse[static_cast<size_t>(row) * a.heads + head] = lse;
+}
+
+// grid (splits, kv heads x head tiles of 8, rows), 4 warps.  The CTA takes
+// positions [start + split * per, ...) of its row, its warps blocks of 16
+// tokens in turn, each with its own online softmax; the four join through
+// shared memory.  Per block, with tokens on the M side of the products:
+//   S^T[16 tokens, 8 heads] = K Q^T, O^T[D dims, 8 heads] += V^T P^T.
+// K fragments come straight from global memory: lane (g, c) = (lane / 4,
+// lane % 4) reads 16 bytes at dims 32 i + 8 c of tokens g and g + 8, and the
+// contraction runs over the dims in that order on both sides.  V likewise:
+// the lane reads tokens 2c, 2c+1, 2c+8, 2c+9 at dims 64 i + 8 g and pairs
+// tokens with byte permutes, which is the transposed operand.  The next
+// block's K is requested as soon as this one's has been multiplied, its V
+// likewise.  With one split the CTA also joins the prefix's partial results
+// and writes the output; else it leaves partial results to the join kernel.
+template <typename T, int D>
+__global__ void __launch_bounds__(OWN_THREADS) own_kernel(const Args a) {
+  // Behind a prefix kernel of the same call nothing that this part reads is
+  // new: the prefix kernel's CTAs have all passed their own wait for whatever
+  // came before.  Its results are waited for where they are read, below.
+  if (!a.after_prefix) qb200::griddep_wait();
+  qb200::griddep_launch_dependents();
+  constexpr int KI = D / 32;  // 16-byte chunks of a token per lane (scores)
+  constexpr int VI = D / 64;  // 16-byte chunks of a token per lane (values)
+  __shared__ float s_m[4][8], s_l[4][8];
+  __shared__ __align__(16) float s_o[4][8][D + 4];
+  const int split = blockIdx.x, row = blockIdx.z;
+  const int htiles = (a.ratio + 7) >> 3;
+  const int kvh = blockIdx.y / htiles, h0 = (blockIdx.y % htiles) * 8;
+  const int nh = min(8, a.ratio - h0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  int seq;
+  const int len = row_length(a, row, &seq);
+  const RowPlan rp = a.row_plan[row];
+  if (len < 0 && threadIdx.x == 0) gemm_record(a.err, 3);
+  const int start = len >= rp.prefix ? rp.prefix : 0;
+  const int count = max(0, len - start);
+  // Tokens of one split: a multiple of 64 that covers the row.
+  const int per = ((count + a.own_splits - 1) / a.own_splits + 63) / 64 * 64;
+  const int lo = start + split * per, hi = min(len, lo + per);
+  const bool fused = a.own_splits == 1;
+
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // heads 2c, 2c + 1
+  // O^T tile (i, e): rows g = dims 64 i + 8 g + e, rows g + 8 = those + 4;
+  // columns = heads 2c, 2c + 1.
+  float o[VI][4][4];
+#pragma unroll
+  for (int i = 0; i < VI; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) o[i][e][x] = 0.f;
+  bool seen = false;
+  const int b0 = lo + 16 * warp;
+  if (b0 < hi) {
+    const int *trow = a.page_table + seq * a.table_pitch;
+    const T *kp = static_cast<const T *>(a.k_pool) + kvh * a.head_stride + g * a.token_stride + 8 * c;
+    const T *vp = static_cast<const T *>(a.v_pool) + kvh * a.head_stride + 2 * c * a.token_stride + 8 * g;
+    // Element offset of block j of this warp in the pools; -1: its page is not
+    // mapped.  The pages of 32 blocks are looked up at once.
+    long long where = 0;
+    const auto lookup = [&](int j) {
+      const int b = b0 + 64 * (j + lane);
+      where = -1;
+      if (b < hi) {
+        const int pi = b / a.page_tokens, page = trow[pi];
+        if (page >= 0 && page < a.num_pages)
+          where = page * a.page_stride + static_cast<long long>(b - pi * a.page_tokens) * a.token_stride;
+        else
+          gemm_record(a.err, 3);
+      }
+    };
+    lookup(0);
+    // Q^T as the B operand: n = head g, k = dims in the order of the K loads.
+    uint32_t qb[KI][4];
+    {
+      const T *qr = static_cast<const T *>(a.q) + row * a.q_row + (kvh * a.ratio + h0 + g) * a.q_head;
+#pragma unroll
+      for (int i = 0; i < KI; ++i) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (g < nh) v = *reinterpret_cast<const uint4 *>(qr + 32 * i + 8 * c);
+        qb[i][0] = v.x; qb[i][1] = v.y; qb[i][2] = v.z; qb[i][3] = v.w;
+      }
+    }
+    const int nb = (hi - b0 + 63) / 64;
+    uint4 kv[2][KI], vv[4][VI];
+    const auto load_k = [&](long long at, int n) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int i = 0; i < KI; ++i) kv[x][i] = ld_kv(kp + at + 8 * x * a.token_stride + 32 * i, g + 8 * x < n);
+    };
+    const auto load_v = [&](long long at, int n) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int t = (x & 1) + 8 * (x >> 1);
+#pragma unroll
+        for (int i = 0; i < VI; ++i) vv[x][i] = ld_kv(vp + at + t * a.token_stride + 64 * i, 2 * c + t < n);
+      }
+    };
+    // Tokens of block j that count: none behind the row or of an unmapped page.
+    const auto tokens = [&](int j, long long at) { return at < 0 ? 0 : min(16, hi - (b0 + 64 * j)); };
+    long long at = __shfl_sync(0xffffffffu, where, 0);
+    int n = tokens(0, at);
+    load_k(at, n);
+    load_v(at, n);
+    for (int j = 0; j < nb; ++j) {
+      if (j + 1 < nb && ((j + 1) & 31) == 0) lookup(j + 1);
+      const long long at1 = __shfl_sync(0xffffffffu, where, (j + 1) & 31);
+      const int n1 = j + 1 < nb ? tokens(j + 1, at1) : 0;
+      float s[4] = {0.f, 0.f, 0.f, 0.f};  // (token g, heads 2c, 2c+1), (token g + 8, ...)
+#pragma unroll
+      for (int i = 0; i < KI; ++i) {
+        mma16816<T>(s, kv[0][i].x, kv[1][i].x, kv[0][i].y, kv[1][i].y, qb[i][0], qb[i][1]);
+        mma16816<T>(s, kv[0][i].z, kv[1][i].z, kv[0][i].w, kv[1][i].w, qb[i][2], qb[i][3]);
+      }
+      load_k(at1, n1);
+      float p[4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float s0 = g < n ? s[h] * a.scale_log2 : -INFINITY, s1 = g + 8 < n ? s[2 + h] * a.scale_log2 : -INFINITY;
+        float mx = fmaxf(s0, s1);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float mn = fmaxf(m[h], mx);
+        const float mu = mn == -INFINITY ? 0.f : mn;
+        const float f = ex2_approx(m[h] - mu);
+        p[h] = ex2_approx(s0 - mu);
+        p[2 + h] = ex2_approx(s1 - mu);
+        l[h] = l[h] * f + (p[h] + p[2 + h]);
+        m[h] = mn;
+#pragma unroll
+        for (int i = 0; i < VI; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            o[i][e][h] *= f;
+            o[i][e][2 + h] *= f;
+          }
+      }
+      seen = seen || n > 0;
+      // P^T as the B operand (n = head g, k = tokens 2c, 2c+1 / 2c+8, 2c+9).
+      // The weights are rounded to the input type for the product (half a
+      // step each, as the values they weigh); their sum is not.
+      const uint32_t pb0 = transpose8x8(Type<T>::pack(p[0], p[1]));
+      const uint32_t pb1 = transpose8x8(Type<T>::pack(p[2], p[3]));
+#pragma unroll
+      for (int i = 0; i < VI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          // A rows g: dim 8 g + e; rows g + 8: dim 8 g + e + 4.
+          const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
+          const int w0 = e >> 1, w1 = 2 + (e >> 1);
+          const uint32_t a0 = __byte_perm(word(vv[0][i], w0), word(vv[1][i], w0), sel);
+          const uint32_t a1 = __byte_perm(word(vv[0][i], w1), word(vv[1][i], w1), sel);
+          const uint32_t a2 = __byte_perm(word(vv[2][i], w0), word(vv[3][i], w0), sel);
+          const uint32_t a3 = __byte_perm(word(vv[2][i], w1), word(vv[3][i], w1), sel);
+          mma16816<T>(o[i][e], a0, a1, a2, a3, pb0, pb1);
+        }
+      load_v(at1, n1);
+      at = at1;
+      n = n1;
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 4);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 8);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 16);
+    // Seen tokens whose scores are all -inf: as in the prefix kernel.
+    if (m[h] == -INFINITY) l[h] = seen ? 1.f : 0.f;
+    if (g == 0) {
+      s_m[warp][2 * c + h] = m[h];
+      s_l[warp][2 * c + h] = l[h];
+    }
+#pragma unroll
+    for (int i = 0; i < VI; ++i) {
+      float *d = &s_o[warp][2 * c + h][64 * i + 8 * g];
+      *reinterpret_cast<float4 *>(d) = make_float4(o[i][0][h], o[i][1][h], o[i][2][h], o[i][3][h]);
+      *reinterpret_cast<float4 *>(d + 4) = make_float4(o[i][0][2 + h], o[i][1][2 + h], o[i][2][2 + h], o[i][3][2 + h]);
+    }
+  }
+  __syncthreads();
+  if (a.after_prefix) qb200::griddep_wait();
+  constexpr int Q4 = D / 4;
+  for (int x = threadIdx.x; x < nh * Q4; x += OWN_THREADS) {
+    // Neighbouring threads take the heads of one row: their prefix partials are adjacent.
+    const int h = x % nh, d4 = x / nh, head = kvh * a.ratio + h0 + h;
+    Joined j;
+    if (fused && rp.prefix > 0 && len >= rp.prefix) join_prefix<D>(a, prefix_parts(a, rp, head), d4, 0, 1, j);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) j.add(s_m[w][h], s_l[w][h], *reinterpret_cast<const float4 *>(&s_o[w][h][4 * d4]));
+    if (fused) {
+      put_result<T>(a, row, head, d4, j);
+    } else {
+      float *part = a.own + ((static_cast<size_t>(row) * a.heads + head) * a.own_splits + split) * (D + 4);
+      *reinterpret_cast<float4 *>(part + 4 * d4) = j.acc;
+      if (d4 == 0) {
+        part[D] = j.m;
+        part[D + 1] = j.m == -INFINITY ? j.none : j.l;
+      }
+    }
+  }
+}
+
+// -------------------------------------------------------------- join kernel
+// grid (heads, rows), 128 threads: D / 4 threads per partial result, several
+// partials at a time; the groups meet in shared memory in a fixed order.
+constexpr int JOIN_THREADS = 128;
+template <typename T, int D>
+__global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args a) {
+  qb200::griddep_wait();
+  qb200::griddep_launch_dependents();
+  constexpr int Q4 = D / 4, NG = JOIN_THREADS / Q4;
+  __shared__ float s_m[NG], s_l[NG], s_none[NG];
+  __shared__ __align__(16) float4 s_acc[NG][Q4];
+  const int head = blockIdx.x, row = blockIdx.y, grp = threadIdx.x / Q4, d4 = threadIdx.x % Q4;
+  int seq;
+  const int len = row_length(a, row, &seq);
+  const RowPlan rp = a.row_plan[row];
+  Joined j;
+  if (rp.prefix > 0 && len >= rp.prefix) join_prefix<D>(a, prefix_parts(a, rp, head), d4, grp, NG, j);
+  if (len > 0) {
+    const int count = len - (len >= rp.prefix ? rp.prefix : 0);
+    const int per = ((count + a.own_splits - 1) / a.own_splits + 63) / 64 * 64;
+    const int ns = count > 0 ? (count + per - 1) / per : 0;
+    const float *own = a.own + (static_cast<size_t>(row) * a.heads + head) * a.own_splits * (D + 4);
+    for (int s = grp; s < ns; s += NG) {
+      const float *p = own + static_cast<size_t>(s) * (D + 4);
+      j.add(p[D], p[D + 1], *reinterpret_cast<const float4 *>(p + 4 * d4));
+    }
+  }
+  if (d4 == 0) {
+    s_m[grp] = j.m;
+    s_l[grp] = j.l;
+    s_none[grp] = j.none;
+  }
+  s_acc[grp][d4] = j.acc;
+  __syncthreads();
+  if (grp != 0) return;
+  Joined r;
+#pragma unroll
+  for (int k = 0; k < NG; ++k) {
+    r.add(s_m[k], s_l[k], s_acc[k][d4]);
+    r.none += s_none[k];
+  }
+  put_result<T>(a, row, head, d4, r);
 }
 
 }  // namespace qb200x
@@ -918,7 +1003,8 @@ int launch(const QwenPrefixAttention &u, const Args &a, const CUtensorMap &mk, c
   cudaError_t e = qb200_launch(own_kernel<T, D>, dim3(a.own_splits, a.kv_heads * ((a.ratio + 7) / 8), a.rows),
                                dim3(OWN_THREADS), 0, st, true, a);
   if (e != cudaSuccess) return fail(20, "own attention launch: %s", cudaGetErrorString(e));
-  e = qb200_launch(join_kernel<T, D>, dim3(a.heads, a.rows), dim3(D / 4), 0, st, true, a);
+  if (a.own_splits == 1) return 0;  // the own kernel has joined both parts
+  e = qb200_launch(join_kernel<T, D>, dim3(a.heads, a.rows), dim3(JOIN_THREADS), 0, st, true, a);
   if (e != cudaSuccess) return fail(20, "attention join launch: %s", cudaGetErrorString(e));
   return 0;
 }
@@ -978,7 +1064,7 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
   const auto limit = [&](int c) { return weight * (c + 1) / ctas; };  // end of CTA c's share
   for (int g = 0; g < groups; ++g) {
     const int p = prefix_of(g);
-    for (int r = 0; r < group_rows[g]; ++r) rp[row0 + r] = RowPlan{p, ntile, r * ratio, 0};
+    for (int r = 0; r < group_rows[g]; ++r) rp[row0 + r] = RowPlan{p, ntile, r * ratio, group_rows[g] * ratio};
     if (p > 0) {
       const int nq = group_rows[g] * ratio, nt = (p + TN - 1) / TN;
       for (int q0 = 0; q0 < nq; q0 += 2 * QT) {
@@ -1012,7 +1098,7 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
 long long qwen_b200_prefix_workspace(const int *h, int dim, int max_length) {
   if (!plan_ok(h) || (dim != 64 && dim != 128)) return 0;
   return slot_bytes(h, dim) +
-         up256(static_cast<long long>(h[PW_ROWS]) * h[PW_HEADS] * plan_splits(h, max_length) * (dim + 2) * 4);
+         up256(static_cast<long long>(h[PW_ROWS]) * h[PW_HEADS] * plan_splits(h, max_length) * (dim + 4) * 4);
 }
 
 int qwen_b200_prefix_attention(const QwenPrefixAttention *u, void *stream) {
@@ -1053,7 +1139,11 @@ int qwen_b200_prefix_attention(const QwenPrefixAttention *u, void *stream) {
   a.page_table = u->page_table;
   a.seq_ids = u->seq_ids;
   a.lengths = u->lengths;
-  a.plan = static_cast<const int *>(u->plan);
+  const int *plan = static_cast<const int *>(u->plan);
+  a.cta_seg = plan + h[PW_CTA_SEG];
+  a.segs = reinterpret_cast<const Seg *>(plan + h[PW_SEG]);
+  a.tile_slot = plan + h[PW_TILE_SLOT];
+  a.row_plan = reinterpret_cast<const RowPlan *>(plan + h[PW_ROW]);
   a.slots = static_cast<float *>(u->workspace);
   a.own = reinterpret_cast<float *>(static_cast<char *>(u->workspace) + slot_bytes(h, u->dim));
   a.q_row = u->q_row_stride;
@@ -1077,6 +1167,7 @@ int qwen_b200_prefix_attention(const QwenPrefixAttention *u, void *stream) {
   a.max_pages = u->max_pages;
   a.length_bias = u->length_bias;
   a.own_splits = plan_splits(h, u->max_length);
+  a.after_prefix = h[PW_SEGS] > 0;
   a.scale_log2 = u->scale * 1.4426950408889634f;
   a.box = u->page_tokens % 128 == 0 ? 128 : u->page_tokens % 64 == 0 ? 64 : u->page_tokens % 32 == 0 ? 32 : 16;
   CUtensorMap mk, mv;

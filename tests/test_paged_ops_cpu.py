@@ -10,6 +10,39 @@ import torch
 import paged
 
 
+class Pools(ctypes.Structure):
+    _fields_ = [("k_pool", ctypes.c_void_p), ("v_pool", ctypes.c_void_p), ("num_pages", ctypes.c_int),
+                ("inner", ctypes.c_int), ("page_tokens", ctypes.c_int), ("token_bytes", ctypes.c_int)]
+
+
+class Table(ctypes.Structure):
+    _fields_ = [("entries", ctypes.c_void_p), ("num_seqs", ctypes.c_int), ("max_pages", ctypes.c_int),
+                ("pitch", ctypes.c_longlong)]
+
+
+class Attention(ctypes.Structure):
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "out", "lse", "k_pool", "v_pool", "page_table", "seq_ids",
+                                                "lengths", "plan_header", "plan", "workspace")]
+                + [(n, ctypes.c_longlong) for n in ("workspace_bytes", "q_row_stride", "q_head_stride",
+                                                    "out_row_stride", "out_head_stride", "page_stride",
+                                                    "head_stride", "token_stride", "table_pitch")]
+                + [(n, ctypes.c_int) for n in ("rows", "heads", "kv_heads", "dim", "dtype", "num_pages",
+                                               "page_tokens", "num_seqs", "max_pages", "max_length", "length_bias")]
+                + [("scale", ctypes.c_float)])
+
+
+def _lib():
+    L = paged.lib()
+    vp, i = ctypes.c_void_p, ctypes.c_int
+    pools, table = ctypes.POINTER(Pools), ctypes.POINTER(Table)
+    for name, args in [("pages_copy", [pools, vp, vp, vp, i, vp]), ("pages_fork", [pools, table, vp, vp, vp, vp, i, vp]),
+                       ("pages_compact", [pools, table, vp, vp, i, vp]), ("pages_free", [table, vp, i, vp]),
+                       ("prefix_attention", [ctypes.POINTER(Attention), vp])]:
+        f = getattr(L, "qwen_b200_" + name)
+        f.restype, f.argtypes = i, args
+    return L
+
+
 def _err():
     return paged._last_error()
 
@@ -23,11 +56,11 @@ def _ints(v):
 
 
 def _call(name, pools=None, table=None, lists=(), n=None):
-    p = paged._Pools(**{**POOLS, **(pools or {})})
-    t = paged._Table(**{**TABLE, **(table or {})})
+    p = Pools(**{**POOLS, **(pools or {})})
+    t = Table(**{**TABLE, **(table or {})})
     arrays = [_ints(v) for v in lists]
     n = len(lists[0]) if n is None else n
-    f = getattr(paged.lib(), "qwen_b200_pages_" + name)
+    f = getattr(_lib(), "qwen_b200_pages_" + name)
     head = {"copy": [ctypes.byref(p)], "free": [ctypes.byref(t)]}.get(name, [ctypes.byref(p), ctypes.byref(t)])
     return f(*head, *arrays, n, None)
 
@@ -88,8 +121,8 @@ def _attention(**kw):
                 page_stride=2 * 64 * 128, head_stride=64 * 128, token_stride=128, table_pitch=8, rows=4, heads=4,
                 kv_heads=2, dim=128, dtype=0, num_pages=64, page_tokens=64, num_seqs=4, max_pages=8, max_length=512,
                 length_bias=0, scale=0.1)
-    a = paged._Attention(**{**base, **kw})
-    return paged.lib().qwen_b200_prefix_attention(ctypes.byref(a), None)
+    a = Attention(**{**base, **kw})
+    return _lib().qwen_b200_prefix_attention(ctypes.byref(a), None)
 
 
 @pytest.mark.parametrize("kw,what", [
@@ -137,15 +170,17 @@ def test_python_refusals_without_a_gpu():
         paged.free_pages(torch.zeros(2, 2, dtype=torch.int32), [0])
     with pytest.raises(ValueError, match="PrefixPlan"):
         paged.shared_prefix_attention(torch.zeros(2, 4, 64, dtype=torch.float16), z, z, z, z, z, None)
-    with pytest.raises(ValueError, match="fp16 or bf16"):
-        paged.shared_prefix_attention(torch.zeros(2, 4, 64), z, z, z, z, z, None)
+    with pytest.raises(ValueError, match="CUDA device"):
+        paged.PrefixPlan([2], [16], 4, 2, 64, max_length=32, device="cpu")
+    with pytest.raises(ValueError, match="head_dim"):
+        paged.PrefixPlan([2], [16], 4, 2, 96, max_length=32)
+    with pytest.raises(ValueError, match="entries"):
+        paged.PrefixPlan([2, 1], [16], 4, 2, 64, max_length=32)
     for bad in (torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2), torch.tensor([True])):
         with pytest.raises(ValueError, match="list of integers"):
             paged._host_list(bad, "x")
     with pytest.raises(ValueError, match="32 bits"):
         paged._host_list([1 << 40], "x")
-    with pytest.raises(ValueError, match="entries"):
-        paged._host_list([1, 2], "x", 3)
 
 
 def _plan(rows, lens, heads, kv, ctas):
