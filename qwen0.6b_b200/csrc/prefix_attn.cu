@@ -53,7 +53,7 @@ using qb200tc::tmem_ld64;
 // Header words, then the arrays they point at (offsets in words).
 enum PlanWord : int {
   PW_MAGIC = 0, PW_ROWS, PW_GROUPS, PW_CTAS, PW_SEGS, PW_TILES, PW_HEADS, PW_KV_HEADS,
-  PW_CTA_SEG, PW_SEG, PW_TILE_SLOT, PW_ROW, PW_ERR, PW_WORDS, PW_MIN_PREFIX, PW_MAX_PREFIX
+  PW_CTA, PW_SEG, PW_TILE_SLOT, PW_ROW, PW_ERR, PW_WORDS, PW_MIN_PREFIX, PW_MAX_PREFIX
 };
 constexpr int PLAN_MAGIC = 0x51503031;
 // A segment is a CTA's run of token tiles of one query tile (up to 256
@@ -66,6 +66,11 @@ struct Seg {
   int t0, t1;   // token tiles [t0, t1) of TN tokens
   int prefix;   // prefix tokens of the group
   int dual;     // more than 128 queries in the tile
+};
+// What a CTA reads first: its segments and a copy of the first one.
+struct CtaPlan {
+  int seg0, seg1, pad[6];
+  Seg first;
 };
 // Per row: the group's prefix (0: none), the group's first query tile, the
 // row's first query in the group, the queries of the group.
@@ -83,7 +88,7 @@ struct Args {
   void *out;
   float *lse;
   const int *page_table, *seq_ids, *lengths;
-  const int *cta_seg;      // parts of the plan
+  const CtaPlan *cta;      // parts of the plan
   const Seg *segs;
   const int *tile_slot;
   const RowPlan *row_plan;
@@ -95,7 +100,7 @@ struct Args {
   const void *k_pool, *v_pool;
   unsigned long long *err;
   int rows, heads, kv_heads, ratio;
-  int num_pages, page_tokens, box, num_seqs, max_pages;
+  int num_pages, page_tokens, box, box_shift, num_seqs, max_pages;
   int length_bias, own_splits;
   int after_prefix;    // the own kernel follows a prefix kernel of the same call
   float scale_log2;
@@ -190,6 +195,85 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Two fp32 lanes in one register pair, and the three-way maximum.
+__device__ __forceinline__ uint64_t pair2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpair2(uint64_t v, float &x, float &y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// NaN if any is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^x of two values on the FMA pipe: x = n + f with n the nearest integer
+// (added and taken off again at 1.5 x 2^23), 2^f by a polynomial of degree 4
+// fitted to it over [-1/2, 1/2] with equal relative errors (2.7e-6 in fp32, a
+// ninetieth of an fp16 half step), n added to the exponent.  Below -126 it
+// gives 2^-126.  The special function unit makes 16 results a clock and SM,
+// which alone would take as long as the tile's products; kPolyOf8 of eight
+// pairs go this way instead.
+constexpr int kPolyOf8 = 3;
+__device__ __forceinline__ void exp2_poly2(uint64_t x2, float &a, float &b) {
+  float x, y;
+  unpair2(x2, x, y);
+  x = fmaxf(x, -126.f);
+  y = fmaxf(y, -126.f);
+  x2 = pair2(x, y);
+  const uint64_t big = pair2(12582912.f, 12582912.f);
+  const uint64_t t2 = add2(x2, big);
+  const uint64_t n2 = add2(t2, pair2(-12582912.f, -12582912.f));
+  const uint64_t f2 = fma2(n2, pair2(-1.f, -1.f), x2);
+  uint64_t p = fma2(f2, pair2(0.009570102207362652f, 0.009570102207362652f), pair2(0.05591786280274391f, 0.05591786280274391f));
+  p = fma2(p, f2, pair2(0.240247443318367f, 0.240247443318367f));
+  p = fma2(p, f2, pair2(0.6931217908859253f, 0.6931217908859253f));
+  p = fma2(p, f2, pair2(0.9999992847442627f, 0.9999992847442627f));
+  float t, u;
+  unpair2(p, a, b);
+  unpair2(t2, t, u);
+  a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(t) << 23));
+  b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(u) << 23));
+}
+
 // Instruction descriptor of kind::f16: fp32 accumulator, M = 128, N = n, both
 // operands fp16 or both bf16, A K-major, B K-major or MN-major.
 template <typename T>
@@ -221,15 +305,20 @@ __global__ void __launch_bounds__(THREADS, 1)
   constexpr int ST = kStages<D>, TILE = kTileBytes<D>, QB = QT * D * 2, HALVES = D / 64;
   constexpr uint32_t S_COL = 0, O_COL = 256;  // tensor memory columns: S0 S1 | O0 O1, 128 each
   extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ float s_ml[2][QT];
   uint8_t *base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t *sq = base, *ring = base + 2 * QB;
   uint64_t *kv_full = reinterpret_cast<uint64_t *>(ring + ST * TILE);
   uint64_t *kv_empty = kv_full + ST;
-  uint64_t *s_full = kv_empty + ST, *p_full = s_full + 2, *q_full = p_full + 2, *o_full = q_full + 1;
+  uint64_t *s_full = kv_empty + ST, *p_full = s_full + 2, *q_full = p_full + 4, *o_full = q_full + 1;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(o_full + 1);
   volatile uint32_t *abort = tmem_slot + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  if (threadIdx.x == 32) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_k)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_v)) : "memory");
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
       mbar_init(&kv_full[s], 1);
@@ -237,7 +326,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 4);
+      mbar_init(&p_full[2 * s], 4);
+      mbar_init(&p_full[2 * s + 1], 4);
     }
     mbar_init(q_full, 8);
     mbar_init(o_full, 1);
@@ -249,20 +339,23 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  // The plan is read before the wait for the preceding kernel: nothing on the
+  // stream writes it.
+  const int seg0 = a.cta[blockIdx.x].seg0, seg1 = a.cta[blockIdx.x].seg1;
+  const Seg first = a.cta[blockIdx.x].first;
+  const auto segment = [&](int si) { return si == seg0 ? first : a.segs[si]; };
   qb200::griddep_wait();
   if (threadIdx.x == 0) qb200::griddep_launch_dependents();
 
-  const int seg0 = a.cta_seg[blockIdx.x], seg1 = a.cta_seg[blockIdx.x + 1];
-  const Seg *segs = a.segs;
   const int boxes = TN / a.box;
 
-  // Page holding box b of token tile t of the segment's prefix, or num_pages
-  // (which the copy fills with zeros) when it is past the prefix or unmapped.
-  auto page_of = [&](const int *row, const Seg &s, int t, int b, bool *bad) {
-    const int pos = t * TN + b * a.box;
+  const int per_page = a.page_tokens / a.box;  // boxes of a page
+  // Page holding box x (from position 0) of the segment's prefix, or num_pages
+  // (which a copy fills with zeros) when it is past the prefix or unmapped.
+  auto page_of = [&](const int *row, const Seg &s, int x, bool *bad) {
     *bad = false;
-    if (pos >= s.prefix) return a.num_pages;
-    const int i = pos / a.page_tokens;
+    if (x * a.box >= s.prefix) return a.num_pages;
+    const int i = x / per_page;
     const int p = row != nullptr && i < a.max_pages ? row[i] : -1;
     if (p >= 0 && p < a.num_pages) return p;
     *bad = true;
@@ -277,11 +370,23 @@ __global__ void __launch_bounds__(THREADS, 1)
     // ---- K / V tiles into the ring
     int place = 0;  // tiles issued so far
     bool ok = true;
+    const int wt = 32 / boxes;  // tiles whose pages one lookup of the warp covers
     for (int si = seg0; si < seg1 && ok; ++si) {
-      const Seg s = segs[si];
+      const Seg s = segment(si);
       const int *row = table_row(s);
       const int n = s.t1 - s.t0;
       const int total = 2 * n;
+      // Lane j holds the page of box j of the window's tiles, K and V each
+      // with a window of their own, and the next window's already requested.
+      int win[2] = {0, 0}, cur[2], nxt[2];
+      auto look = [&](int t, bool report) {
+        bool bad = false;
+        const int p = lane < wt * boxes ? page_of(row, s, (s.t0 + t) * boxes + lane, &bad) : a.num_pages;
+        if (bad && report && s.t0 + t + lane / boxes < s.t1) gemm_record(a.err, 3);
+        return p;
+      };
+      cur[0] = cur[1] = look(0, true);
+      nxt[0] = nxt[1] = look(wt, n > wt);
       for (int i = 0; i < total && ok; ++i) {
         // Tile of place i (the inverse of k_place / v_place).
         bool is_v;
@@ -299,9 +404,22 @@ __global__ void __launch_bounds__(THREADS, 1)
           is_v = !(i & 1);
           t = is_v ? (i - 2) / 2 : (i + 1) / 2;
         }
-        bool bad = false;
-        const int page = lane < boxes ? page_of(row, s, s.t0 + t, lane, &bad) : 0;
-        if (bad && !is_v) gemm_record(a.err, 3);
+        int page;
+        if (is_v) {
+          if (t >= win[1] + wt) {
+            win[1] += wt;
+            cur[1] = nxt[1];
+            nxt[1] = look(win[1] + wt, false);
+          }
+          page = __shfl_sync(0xffffffffu, cur[1], (t - win[1]) * boxes + (lane < boxes ? lane : 0));
+        } else {
+          if (t >= win[0] + wt) {
+            win[0] += wt;
+            cur[0] = nxt[0];
+            nxt[0] = look(win[0] + wt, true);
+          }
+          page = __shfl_sync(0xffffffffu, cur[0], (t - win[0]) * boxes + (lane < boxes ? lane : 0));
+        }
         const int stage = place % ST;
         if (place >= ST) ok = gemm_wait(&kv_empty[stage], ((place / ST) - 1) & 1, abort, a.err, 1);
         ok = __all_sync(0xffffffffu, ok);
@@ -310,8 +428,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
         if (lane < boxes) {
           uint8_t *dst = ring + stage * TILE + lane * a.box * 128;
-          const int tok = (s.t0 + t) * TN + lane * a.box;
-          const int off = page == a.num_pages ? 0 : tok % a.page_tokens;
+          const int off = (((s.t0 + t) * boxes + lane) % per_page) * a.box;
 #pragma unroll
           for (int h = 0; h < HALVES; ++h)
             tma_load_4d(dst + h * TN * 128, is_v ? &tm_v : &tm_k, 64 * h, off, s.kvh, page, &kv_full[stage]);
@@ -336,7 +453,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     int steps[2] = {0, 0};    // steps of each stream so far (phases of p_full)
     bool ok = true;
     for (int si = seg0; si < seg1 && ok; ++si) {
-      const Seg s = segs[si];
+      const Seg s = segment(si);
       const bool dual = s.dual != 0;
       const int nt = s.t1 - s.t0, n = dual ? 2 * nt : nt;
       ok = gemm_wait(q_full, (si - seg0) & 1, abort, a.err, 1);
@@ -363,19 +480,23 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (ok && n > 1) score(1);
       for (int i = 0; i < n && ok; ++i) {
         const int st = i & 1, t = dual ? i >> 1 : i;
-        ok = gemm_wait(&p_full[st], steps[st] & 1, abort, a.err, 1);
         const int place = ring0 + v_place(dual, t, nt), stage = place % ST;
-        ok = ok && gemm_wait(&kv_full[stage], (place / ST) & 1, abort, a.err, 1);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        ++steps[st];
-        tc_fence_after();
+        ok = gemm_wait(&kv_full[stage], (place / ST) & 1, abort, a.err, 1);
         const uint32_t vb = smem_u32(ring + stage * TILE), pa = tmem + S_COL + st * 128;
         // Only the 16-token steps inside the prefix: what lies behind it in a
-        // page may be anything (0 x NaN).
+        // page may be anything (0 x NaN).  The first half of the tile's
+        // weights is multiplied while the second is being computed.
         const int ks = min(TN, s.prefix - (s.t0 + t) * TN) / 16;
-        for (int k = 0; k < ks; ++k)
-          mma_ts(tmem + O_COL + st * 128, pa + 8 * k, sw128_mn_desc(vb + 2048 * k, TN * 128), id_o, k != 0 || i > 1);
+        for (int half = 0; half < 2; ++half) {
+          ok = ok && gemm_wait(&p_full[2 * st + half], steps[st] & 1, abort, a.err, 1);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          for (int k = 4 * half; k < min(ks, 4 * half + 4); ++k)
+            mma_ts(tmem + O_COL + st * 128, pa + 8 * k, sw128_mn_desc(vb + 2048 * k, TN * 128), id_o, k != 0 || i > 1);
+        }
+        if (!ok) break;
+        ++steps[st];
         if (!dual || st == 1) commit_elect(&kv_empty[stage]);
         if (i + 2 < n) score(i + 2);
       }
@@ -397,42 +518,60 @@ __global__ void __launch_bounds__(THREADS, 1)
     int steps = 0;
     bool ok = true;
     for (int si = seg0; si < seg1 && ok; ++si) {
-      const Seg s = segs[si];
+      const Seg s = segment(si);
       const bool dual = s.dual != 0;
       const int nt = s.t1 - s.t0;
       // Queries of this segment into shared memory (128-byte swizzled rows);
-      // rows past the group are zero.
+      // rows past the group are zero.  A warp takes 32 rows (16 in a single
+      // segment): each lane finds one row's address, then D / 8 lanes read a
+      // row, eight reads of a lane in flight (all of a single segment's).
+      const int *row = table_row(s);
       {
-        constexpr int CPR = D / 8;  // 16-byte chunks of a query
-        const int nload = min(dual ? 256 : 128, (s.nq - s.q0 + 31) / 32 * 32);
-        const T *qg = static_cast<const T *>(a.q);
-        for (int i = tid; i < nload * CPR; i += 256) {
-          const int qi = i / CPR, c = i % CPR;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (s.q0 + qi < s.nq) {
-            const int r = (s.q0 + qi) / a.ratio, h = (s.q0 + qi) % a.ratio;
-            v = *reinterpret_cast<const uint4 *>(qg + (s.row0 + r) * a.q_row + (s.kvh * a.ratio + h) * a.q_head + 8 * c);
+        constexpr int CPR = D / 8, RPI = 32 / CPR;  // 16-byte chunks of a query, rows per step
+        constexpr int U = 16 / RPI;                 // steps of a single segment
+        const int rpw = dual ? 32 : 16, r0 = (tid >> 5) * rpw;
+        const int mine = s.q0 + r0 + (lane & (rpw - 1));
+        long long off = -1;
+        if (mine < s.nq) {
+          const int r = mine / a.ratio, h = mine - r * a.ratio;
+          off = (s.row0 + r) * a.q_row + (s.kvh * a.ratio + h) * a.q_head;
+        }
+        const int c = lane % CPR;
+        const T *qg = static_cast<const T *>(a.q) + 8 * c;
+        for (int x = 0; x < rpw / RPI; x += U) {
+          uint4 v[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const long long at = __shfl_sync(0xffffffffu, off, (x + u) * RPI + lane / CPR);
+            v[u] = make_uint4(0, 0, 0, 0);
+            if (at >= 0) v[u] = *reinterpret_cast<const uint4 *>(qg + at);
           }
-          const int rr = qi & 127;
-          uint8_t *dst = sq + (qi >> 7) * QB + (c >> 3) * (QT * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
-          *reinterpret_cast<uint4 *>(dst) = v;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int qi = r0 + (x + u) * RPI + lane / CPR, rr = qi & 127;
+            uint8_t *dst = sq + (qi >> 7) * QB + (c >> 3) * (QT * 128) + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
+            *reinterpret_cast<uint4 *>(dst) = v[u];
+          }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
       }
+      // Whether every page of the segment is mapped (else each tile looks).
+      bool mapped = true;
+      for (int x = s.t0 * boxes + lane; x < s.t1 * boxes; x += 32) {
+        bool bad = false;
+        page_of(row, s, x, &bad);
+        mapped = mapped && !bad;
+      }
+      mapped = __all_sync(0xffffffffu, mapped);
       const int my_steps = dual ? nt : (st == 0 ? (nt + 1) / 2 : nt / 2);
       // Queries of this warp past the group: nothing to compute.
       const bool live = s.q0 + (dual ? st * QT : 0) + 32 * quad < s.nq;
-      const int *row = table_row(s);
       float m = -INFINITY, l = 0.f;
       for (int i = 0; i < my_steps && ok; ++i) {
         const int t = s.t0 + (dual ? i : 2 * i + st);
-        // Valid tokens of the tile: one bit per box of the copy.
-        bool bad = false;
-        const int page = lane < boxes ? page_of(row, s, t, lane, &bad) : 0;
-        const uint32_t valid = __ballot_sync(0xffffffffu, lane < boxes && page != a.num_pages);
         const int ntok = min(TN, s.prefix - t * TN);
         ok = gemm_wait(&s_full[st], steps & 1, abort, a.err, 1);
         ok = __all_sync(0xffffffffu, ok);
@@ -443,81 +582,152 @@ __global__ void __launch_bounds__(THREADS, 1)
           float v[2][64];
           tmem_ld64(ts, ts + 32, v[0]);
           tmem_ld64(ts + 64, ts + 96, v[1]);
-          if (ntok < TN || valid != (1u << boxes) - 1u) {
+          if (ntok < TN || !mapped) {
+            uint32_t valid = (1u << boxes) - 1u;  // one bit per box
+            if (!mapped) {
+              bool bad = true;
+              if (lane < boxes) page_of(row, s, t * boxes + lane, &bad);
+              valid = __ballot_sync(0xffffffffu, !bad);
+            }
 #pragma unroll
             for (int c = 0; c < TN; ++c)
-              if (c >= ntok || ((valid >> (c / a.box)) & 1u) == 0) v[c >> 6][c & 63] = -INFINITY;
+              if (c >= ntok || ((valid >> (c >> a.box_shift)) & 1u) == 0) v[c >> 6][c & 63] = -INFINITY;
           }
-          float mx[4] = {v[0][0], v[0][1], v[0][2], v[0][3]};
+          float mx[4];
 #pragma unroll
-          for (int c = 4; c < TN; ++c) mx[c & 3] = fmaxf(mx[c & 3], v[c >> 6][c & 63]);
-          const float rowmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+          for (int k = 0; k < 4; ++k) mx[k] = max3(v[0][k], v[0][k + 4], v[0][k + 4]);
+#pragma unroll
+          for (int c = 8; c < TN; c += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], v[c >> 6][(c & 63) + k], v[c >> 6][(c & 63) + k + 4]);
+          const float rowmax = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * a.scale_log2;
           if (i == 0) {
             m = rowmax;
-          } else if (__any_sync(0xffffffffu, rowmax > m + 8.f)) {
+          } else if (__any_sync(0xffffffffu, !(rowmax <= m + 8.f))) {
             // The maximum moves only when a row has outgrown it by 2^8: the
             // weights stay below 2^8, exact in relative terms, and the output
             // is rescaled a few times at most.
-            const float mn = fmaxf(m, rowmax);
+            const float mn = max3(m, rowmax, rowmax);
             const float f = mn == -INFINITY ? 1.f : ex2_approx(m - mn);
             m = mn;
             l *= f;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              float o[32];
+              tmem_ld32(to + c, o);
+              uint32_t w[32];
 #pragma unroll
-            for (int c = 0; c < D; c += 64) {
-              float o[64];
-              tmem_ld64(to + c, to + c + 32, o);
-              uint32_t w[2][32];
-#pragma unroll
-              for (int j = 0; j < 64; ++j) w[j >> 5][j & 31] = __float_as_uint(o[j] * f);
-              tmem_st32(to + c, w[0]);
-              tmem_st32(to + c + 32, w[1]);
+              for (int j = 0; j < 32; ++j) w[j] = __float_as_uint(o[j] * f);
+              tmem_st32(to + c, w);
             }
           }
-          const float mu = m == -INFINITY ? 0.f : m;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          uint32_t p[2][32];
+          // No finite maximum: -inf stands for nothing seen yet, +inf makes NaN.
+          const float mu = m == -INFINITY ? 0.f : (m == INFINITY ? __int_as_float(0x7fffffff) : m);
+          const uint64_t sc2 = pair2(a.scale_log2, a.scale_log2), mu2 = pair2(-mu, -mu);
+          uint64_t sum[2] = {0, 0};
 #pragma unroll
-          for (int c = 0; c < TN; c += 2) {
-            const float x = ex2_approx(fmaf(v[c >> 6][c & 63], a.scale_log2, -mu));
-            const float y = ex2_approx(fmaf(v[c >> 6][(c & 63) + 1], a.scale_log2, -mu));
-            sum[c & 2] += x;
-            sum[(c & 2) + 1] += y;
-            // The weights enter the second product rounded to the input type
-            // (half a step each, as the values they weigh); their sum is not.
-            p[c >> 6][(c >> 1) & 31] = Type<T>::pack(x, y);
+          for (int c0 = 0; c0 < TN; c0 += 32) {
+            uint32_t w[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              const int c = c0 + 2 * k;
+              const uint64_t x2 = fma2(pair2(v[c >> 6][c & 63], v[c >> 6][(c & 63) + 1]), sc2, mu2);
+              float x, y;
+              if (k % 8 < kPolyOf8) {
+                exp2_poly2(x2, x, y);
+              } else {
+                unpair2(x2, x, y);
+                x = ex2_approx(x);
+                y = ex2_approx(y);
+              }
+              sum[k & 1] = add2(sum[k & 1], pair2(x, y));
+              // The weights enter the second product rounded to the input type
+              // (half a step each, as the values they weigh); their sum is not.
+              w[k] = Type<T>::pack(x, y);
+            }
+            tmem_st16(ts + c0 / 2, w);
+            if (c0 == 32) {
+              tmem_wait_st();
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&p_full[2 * st]);
+            }
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-          tmem_st32(ts, p[0]);
-          tmem_st32(ts + 32, p[1]);
+          float s0, s1, s2, s3;
+          unpair2(sum[0], s0, s1);
+          unpair2(sum[1], s2, s3);
+          l += (s0 + s1) + (s2 + s3);
           tmem_wait_st();
+        } else if (lane == 0) {
+          mbar_arrive(&p_full[2 * st]);
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[st]);
+        if (lane == 0) mbar_arrive(&p_full[2 * st + 1]);
       }
-      if (!ok) break;
-      ok = gemm_wait(o_full, (si - seg0) & 1, abort, a.err, 1);
-      ok = __all_sync(0xffffffffu, ok && !*abort);
+      ok = ok && gemm_wait(o_full, (si - seg0) & 1, abort, a.err, 1);
+      ok = !qb200::named_bar_or(1, 256, !ok || *abort);  // all eight warps go on, or none
       if (!ok) break;
       tc_fence_after();
-      if (live) {
-        float *slot = a.slots + (static_cast<size_t>(si) * 2 + st) * kStreamFloats<D>;
-        if (my_steps > 0) {
+      // A visible part whose scores are all -inf: the sum tells it from an
+      // empty one (the softmax of nothing but -inf is NaN).
+      if (my_steps > 0 && m == -INFINITY) l = 1.f;
+      float f0 = 1.f, f1 = 0.f;
+      const bool both = !dual && nt > 1;
+      if (both) {
+        // The two streams of a single segment join in the queries' shared
+        // memory, which every product has been through by now.
+        float4 *so = reinterpret_cast<float4 *>(sq);
+        if (st == 1 && live) {
 #pragma unroll 1
-          for (int c = 0; c < D; c += 64) {
-            float o[64];
-            tmem_ld64(to + c, to + c + 32, o);
+          for (int c = 0; c < D; c += 32) {
+            float o[32];
+            tmem_ld32(to + c, o);
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              reinterpret_cast<float4 *>(slot)[(c / 4 + j) * QT + ql] =
-                  make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            for (int j = 0; j < 8; ++j)
+              so[(c / 4 + j) * QT + ql] = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          }
+          s_ml[0][ql] = m;
+          s_ml[1][ql] = l;
+        }
+        qb200::named_bar_sync(1, 256);
+        if (st == 0 && live) {
+          const float m1 = s_ml[0][ql], l1 = s_ml[1][ql];
+          const float mn = max3(m, m1, m1);
+          if (mn == -INFINITY) {
+            l += l1;
+          } else {
+            f0 = ex2_approx(m - mn);
+            f1 = ex2_approx(m1 - mn);
+            l = (m == -INFINITY ? 0.f : l * f0) + (m1 == -INFINITY ? 0.f : l1 * f1);
+          }
+          m = mn;
+        }
+      }
+      if (live && (dual || st == 0)) {
+        float *slot = a.slots + (static_cast<size_t>(si) * 2 + st) * kStreamFloats<D>;
+        const float4 *so = reinterpret_cast<const float4 *>(sq);
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          float o[32];
+          tmem_ld32(to + c, o);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            float4 x = make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            if (both) {
+              const float4 y = so[(c / 4 + j) * QT + ql];
+              x.x = x.x * f0 + y.x * f1;
+              x.y = x.y * f0 + y.y * f1;
+              x.z = x.z * f0 + y.z * f1;
+              x.w = x.w * f0 + y.w * f1;
+            }
+            reinterpret_cast<float4 *>(slot)[(c / 4 + j) * QT + ql] = x;
           }
         }
         slot[QT * D + ql] = m;
-        // A visible part whose scores are all -inf: the sum tells it from an
-        // empty one (the softmax of nothing but -inf is NaN).
-        slot[QT * D + QT + ql] = my_steps > 0 && m == -INFINITY ? 1.f : l;
+        slot[QT * D + QT + ql] = l;
       }
+      if (both) qb200::named_bar_sync(1, 256);
     }
   }
   __syncwarp();
@@ -591,8 +801,7 @@ struct Joined {
 // Partial results of the prefix for one query: count of them, and where the
 // k-th lies.
 struct PrefixParts {
-  int first, count, ql;  // first stream slot, slots, query within the stream
-  int step;              // stream slots between two of them
+  int first, count, ql;  // first stream slot (one slot holds two), slots, query within the stream
 };
 __device__ __forceinline__ PrefixParts prefix_parts(const Args &a, const RowPlan &rp, int head) {
   const int kvh = head / a.ratio, qi = rp.query + head % a.ratio;
@@ -600,15 +809,10 @@ __device__ __forceinline__ PrefixParts prefix_parts(const Args &a, const RowPlan
   const int s0 = a.tile_slot[tile], s1 = a.tile_slot[tile + 1];
   PrefixParts p;
   p.ql = qi % QT;
-  if (rp.queries - qi / (2 * QT) * (2 * QT) > QT) {  // dual: the query's own stream of every slot
-    p.first = 2 * s0 + ((qi / QT) & 1);
-    p.count = s1 - s0;
-    p.step = 2;
-  } else {                                           // single: both streams (an idle one left m = -inf, l = 0)
-    p.first = 2 * s0;
-    p.count = 2 * (s1 - s0);
-    p.step = 1;
-  }
+  // Dual: the query's own stream of every slot; single: the streams are joined in the first.
+  const bool dual = rp.queries - qi / (2 * QT) * (2 * QT) > QT;
+  p.first = 2 * s0 + (dual ? (qi / QT) & 1 : 0);
+  p.count = s1 - s0;
   return p;
 }
 
@@ -625,7 +829,7 @@ __device__ __forceinline__ void join_prefix(const Args &a, const PrefixParts &p,
       l[u] = 0.f;
       v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (k + u * dk < p.count) {
-        const float *slot = a.slots + static_cast<size_t>(p.first + (k + u * dk) * p.step) * kStreamFloats<D>;
+        const float *slot = a.slots + static_cast<size_t>(p.first + 2 * (k + u * dk)) * kStreamFloats<D>;
         m[u] = slot[QT * D + p.ql];
         l[u] = slot[QT * D + QT + p.ql];
         v[u] = reinterpret_cast<const float4 *>(slot)[d4 * QT + p.ql];
@@ -665,12 +869,10 @@ __device__ __forceinline__ void put_result(const Args &a, int row, int head, int
 // lane % 4) reads 16 bytes at dims 32 i + 8 c of tokens g and g + 8, and the
 // contraction runs over the dims in that order on both sides.  V likewise:
 // the lane reads tokens 2c, 2c+1, 2c+8, 2c+9 at dims 64 i + 8 g and pairs
-// tokens with byte permutes, which is the transposed operand.  The next
-// block's K is requested as soon as this one's has been multiplied, its V
-// likewise.  With one split the CTA also joins the prefix's partial results
+// tokens with byte permutes, which is the transposed operand.  With one split the CTA also joins the prefix's partial results
 // and writes the output; else it leaves partial results to the join kernel.
 template <typename T, int D>
-__global__ void __launch_bounds__(OWN_THREADS) own_kernel(const Args a) {
+__global__ void __launch_bounds__(OWN_THREADS, 5) own_kernel(const Args a) {
   // Behind a prefix kernel of the same call nothing that this part reads is
   // new: the prefix kernel's CTAs have all passed their own wait for whatever
   // came before.  Its results are waited for where they are read, below.
@@ -680,6 +882,8 @@ __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const Args a) {
   constexpr int VI = D / 64;  // 16-byte chunks of a token per lane (values)
   __shared__ float s_m[4][8], s_l[4][8];
   __shared__ __align__(16) float s_o[4][8][D + 4];
+  constexpr int QP = D + 32;  // pitch of a query row: the fragment reads of two rows take all banks
+  __shared__ __align__(16) T s_q[8 * QP];
   const int split = blockIdx.x, row = blockIdx.z;
   const int htiles = (a.ratio + 7) >> 3;
   const int kvh = blockIdx.y / htiles, h0 = (blockIdx.y % htiles) * 8;
@@ -708,36 +912,35 @@ __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const Args a) {
       for (int x = 0; x < 4; ++x) o[i][e][x] = 0.f;
   bool seen = false;
   const int b0 = lo + 16 * warp;
+  const int *trow = a.page_table + (len < 0 ? 0 : seq * a.table_pitch);
+  // Element offset of block j of this warp in the pools; -1: its page is not
+  // mapped.  The pages of 32 blocks are looked up at once.
+  long long where = -1;
+  const auto lookup = [&](int j) {
+    const int b = b0 + 64 * (j + lane);
+    where = -1;
+    if (b < hi) {
+      const int pi = b / a.page_tokens, page = trow[pi];
+      if (page >= 0 && page < a.num_pages)
+        where = page * a.page_stride + static_cast<long long>(b - pi * a.page_tokens) * a.token_stride;
+      else
+        gemm_record(a.err, 3);
+    }
+  };
+  lookup(0);
+  // Q^T, the B operand of the scores, waits in shared memory: n = head g, k =
+  // dims in the order of the K loads.
+  for (int x = threadIdx.x; x < D; x += OWN_THREADS) {
+    const int h = x / (D / 8), d = 8 * (x % (D / 8));
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (h < nh)
+      v = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + row * a.q_row + (kvh * a.ratio + h0 + h) * a.q_head + d);
+    *reinterpret_cast<uint4 *>(s_q + h * QP + d) = v;
+  }
+  __syncthreads();
   if (b0 < hi) {
-    const int *trow = a.page_table + seq * a.table_pitch;
     const T *kp = static_cast<const T *>(a.k_pool) + kvh * a.head_stride + g * a.token_stride + 8 * c;
     const T *vp = static_cast<const T *>(a.v_pool) + kvh * a.head_stride + 2 * c * a.token_stride + 8 * g;
-    // Element offset of block j of this warp in the pools; -1: its page is not
-    // mapped.  The pages of 32 blocks are looked up at once.
-    long long where = 0;
-    const auto lookup = [&](int j) {
-      const int b = b0 + 64 * (j + lane);
-      where = -1;
-      if (b < hi) {
-        const int pi = b / a.page_tokens, page = trow[pi];
-        if (page >= 0 && page < a.num_pages)
-          where = page * a.page_stride + static_cast<long long>(b - pi * a.page_tokens) * a.token_stride;
-        else
-          gemm_record(a.err, 3);
-      }
-    };
-    lookup(0);
-    // Q^T as the B operand: n = head g, k = dims in the order of the K loads.
-    uint32_t qb[KI][4];
-    {
-      const T *qr = static_cast<const T *>(a.q) + row * a.q_row + (kvh * a.ratio + h0 + g) * a.q_head;
-#pragma unroll
-      for (int i = 0; i < KI; ++i) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (g < nh) v = *reinterpret_cast<const uint4 *>(qr + 32 * i + 8 * c);
-        qb[i][0] = v.x; qb[i][1] = v.y; qb[i][2] = v.z; qb[i][3] = v.w;
-      }
-    }
     const int nb = (hi - b0 + 63) / 64;
     uint4 kv[2][KI], vv[4][VI];
     const auto load_k = [&](long long at, int n) {
@@ -756,21 +959,19 @@ __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const Args a) {
     };
     // Tokens of block j that count: none behind the row or of an unmapped page.
     const auto tokens = [&](int j, long long at) { return at < 0 ? 0 : min(16, hi - (b0 + 64 * j)); };
-    long long at = __shfl_sync(0xffffffffu, where, 0);
-    int n = tokens(0, at);
-    load_k(at, n);
-    load_v(at, n);
     for (int j = 0; j < nb; ++j) {
-      if (j + 1 < nb && ((j + 1) & 31) == 0) lookup(j + 1);
-      const long long at1 = __shfl_sync(0xffffffffu, where, (j + 1) & 31);
-      const int n1 = j + 1 < nb ? tokens(j + 1, at1) : 0;
+      if (j > 0 && (j & 31) == 0) lookup(j);
+      const long long at = __shfl_sync(0xffffffffu, where, j & 31);
+      const int n = tokens(j, at);
+      load_k(at, n);
+      load_v(at, n);
       float s[4] = {0.f, 0.f, 0.f, 0.f};  // (token g, heads 2c, 2c+1), (token g + 8, ...)
 #pragma unroll
       for (int i = 0; i < KI; ++i) {
-        mma16816<T>(s, kv[0][i].x, kv[1][i].x, kv[0][i].y, kv[1][i].y, qb[i][0], qb[i][1]);
-        mma16816<T>(s, kv[0][i].z, kv[1][i].z, kv[0][i].w, kv[1][i].w, qb[i][2], qb[i][3]);
+        const uint4 qv = *reinterpret_cast<const uint4 *>(s_q + g * QP + 32 * i + 8 * c);
+        mma16816<T>(s, kv[0][i].x, kv[1][i].x, kv[0][i].y, kv[1][i].y, qv.x, qv.y);
+        mma16816<T>(s, kv[0][i].z, kv[1][i].z, kv[0][i].w, kv[1][i].w, qv.z, qv.w);
       }
-      load_k(at1, n1);
       float p[4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -813,9 +1014,6 @@ __global__ void __launch_bounds__(OWN_THREADS) own_kernel(const Args a) {
           const uint32_t a3 = __byte_perm(word(vv[2][i], w1), word(vv[3][i], w1), sel);
           mma16816<T>(o[i][e], a0, a1, a2, a3, pb0, pb1);
         }
-      load_v(at1, n1);
-      at = at1;
-      n = n1;
     }
   }
 #pragma unroll
@@ -1047,10 +1245,40 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
   if (rows < 1 || rows > 65535) return bad(10, "plan: rows outside [1, 65535]");
   if (tiles > (1 << 20)) return bad(10, "plan: over 2^20 query tiles");
   if (min_prefix == 0x7fffffff) min_prefix = 0;
-  // Contiguous shares of the weighted token tiles for every CTA.
+  // Two ways to share the token tiles out, by weight (a dual tile's products
+  // count twice): every query tile cut into equal parts, one part per CTA; or
+  // contiguous shares of all of them, where a CTA's share may end in the next
+  // query tile and so become two segments.  A segment costs about kSegWeight
+  // more than its tiles (queries in, results out: 3 us; a weight: 0.55 us).
+  // A single tile alone would leave a stream idle, so parts are of two.
+  constexpr long long kSegWeight = 6;
+  const auto tile_weight = [](long long nq, long long t, long long nt) {
+    return nq - t * 2 * QT > QT ? 2 * nt : (nt + 1) / 2 * 2;
+  };
+  const auto parts_at = [&](long long q) {  // parts of at most weight q
+    long long n = 0;
+    for (int g = 0; g < groups; ++g) {
+      const int p = prefix_of(g);
+      if (p == 0) continue;
+      const long long nq = static_cast<long long>(group_rows[g]) * ratio, nt = (p + TN - 1) / TN;
+      for (long long t = 0; t * 2 * QT < nq; ++t) n += kv_heads * ((tile_weight(nq, t, nt) + q - 1) / q);
+    }
+    return n;
+  };
+  long long part = 0;  // weight of a part; 0: contiguous shares
+  if (tiles > 0 && tiles <= ctas) {
+    long long lo = 1, hi = 1;
+    while (parts_at(2 * hi) > ctas) hi *= 2;
+    while (lo < hi) {
+      const long long mid = (lo + hi) / 2;
+      if (parts_at(2 * mid) <= ctas) hi = mid; else lo = mid + 1;
+    }
+    if (2 * lo <= (weight + ctas - 1) / ctas + kSegWeight) part = 2 * lo;
+  }
+  if (part > 0) ctas = static_cast<int>(parts_at(part));
   if (ctas > weight) ctas = weight > 0 ? static_cast<int>(weight) : 1;
-  const long long max_segs = tiles + ctas;
-  const long long o_cta = QWEN_PREFIX_HEADER, o_seg = (o_cta + ctas + 1 + 7) / 8 * 8, o_tile = o_seg + max_segs * 8,
+  const long long max_segs = part > 0 ? ctas : tiles + ctas;
+  const long long o_cta = QWEN_PREFIX_HEADER, o_seg = o_cta + 16ll * ctas, o_tile = o_seg + max_segs * 8,
                   o_row = (o_tile + tiles + 1 + 7) / 8 * 8, o_err = o_row + rows * 4, total = o_err + 4;
   if (total > 0x7fffffffll) return bad(10, "plan: too large");
   if (words == nullptr) return static_cast<int>(total);
@@ -1058,6 +1286,7 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
   for (long long i = 0; i < total; ++i) words[i] = 0;
   int nseg = 0, ntile = 0, cta = 0;
   long long done = 0;  // weight handed out
+  CtaPlan *cp = reinterpret_cast<CtaPlan *>(words + o_cta);
   Seg *segs = reinterpret_cast<Seg *>(words + o_seg);
   RowPlan *rp = reinterpret_cast<RowPlan *>(words + o_row);
   int row0 = 0;
@@ -1069,10 +1298,25 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
       const int nq = group_rows[g] * ratio, nt = (p + TN - 1) / TN;
       for (int q0 = 0; q0 < nq; q0 += 2 * QT) {
         const int dual = nq - q0 > QT ? 1 : 0, w = dual ? 2 : 1;
+        const int parts = part > 0 ? static_cast<int>((tile_weight(nq, q0 / (2 * QT), nt) + part - 1) / part) : 0;
+        const int pairs = dual ? nt : (nt + 1) / 2;  // what the parts are made of: dual tiles, or two single ones
         for (int h = 0; h < kv_heads; ++h) {
           words[o_tile + ntile++] = nseg;
+          if (part > 0) {
+            for (int k = 0; k < parts; ++k) {
+              int t0 = static_cast<int>(static_cast<long long>(pairs) * k / parts);
+              int t1 = static_cast<int>(static_cast<long long>(pairs) * (k + 1) / parts);
+              if (!dual) {
+                t0 *= 2;
+                t1 = 2 * t1 < nt ? 2 * t1 : nt;
+              }
+              cp[cta++].seg0 = nseg;
+              segs[nseg++] = Seg{row0, nq, q0, h, t0, t1, p, dual};
+            }
+            continue;
+          }
           for (int t = 0; t < nt;) {
-            while (cta + 1 < ctas && done >= limit(cta)) words[o_cta + ++cta] = nseg;
+            while (cta + 1 < ctas && done >= limit(cta)) cp[++cta].seg0 = nseg;
             long long take = (limit(cta) - done + w - 1) / w;
             if (take < 1 || cta + 1 == ctas) take = cta + 1 == ctas ? nt - t : 1;
             if (take > nt - t) take = nt - t;
@@ -1086,7 +1330,11 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
     row0 += group_rows[g];
   }
   words[o_tile + ntile] = nseg;
-  while (cta + 1 <= ctas) words[o_cta + ++cta] = nseg;
+  for (++cta; part == 0 && cta < ctas; ++cta) cp[cta].seg0 = nseg;
+  for (int c = 0; c < ctas; ++c) {
+    cp[c].seg1 = c + 1 < ctas ? cp[c + 1].seg0 : nseg;
+    if (cp[c].seg0 < cp[c].seg1) cp[c].first = segs[cp[c].seg0];
+  }
   const int head[QWEN_PREFIX_HEADER] = {PLAN_MAGIC, static_cast<int>(rows), groups, ctas, nseg, ntile, heads, kv_heads,
                                         static_cast<int>(o_cta), static_cast<int>(o_seg), static_cast<int>(o_tile),
                                         static_cast<int>(o_row), static_cast<int>(o_err), static_cast<int>(total),
@@ -1140,7 +1388,7 @@ int qwen_b200_prefix_attention(const QwenPrefixAttention *u, void *stream) {
   a.seq_ids = u->seq_ids;
   a.lengths = u->lengths;
   const int *plan = static_cast<const int *>(u->plan);
-  a.cta_seg = plan + h[PW_CTA_SEG];
+  a.cta = reinterpret_cast<const CtaPlan *>(plan + h[PW_CTA]);
   a.segs = reinterpret_cast<const Seg *>(plan + h[PW_SEG]);
   a.tile_slot = plan + h[PW_TILE_SLOT];
   a.row_plan = reinterpret_cast<const RowPlan *>(plan + h[PW_ROW]);
@@ -1170,6 +1418,7 @@ int qwen_b200_prefix_attention(const QwenPrefixAttention *u, void *stream) {
   a.after_prefix = h[PW_SEGS] > 0;
   a.scale_log2 = u->scale * 1.4426950408889634f;
   a.box = u->page_tokens % 128 == 0 ? 128 : u->page_tokens % 64 == 0 ? 64 : u->page_tokens % 32 == 0 ? 32 : 16;
+  a.box_shift = a.box == 128 ? 7 : a.box == 64 ? 6 : a.box == 32 ? 5 : 4;
   CUtensorMap mk, mv;
   if (h[PW_SEGS] > 0) {
     if (int rc = encode_pool(&mk, *u, u->k_pool, a.box)) return rc;

@@ -187,7 +187,8 @@ def _plan(rows, lens, heads, kv, ctas):
     w = paged.plan_words(torch.tensor(rows, dtype=torch.int32), torch.tensor(lens, dtype=torch.int32), heads, kv,
                          ctas).tolist()
     h = w[:16]
-    return dict(rows=h[1], ctas=h[3], cta=w[h[8]:h[8] + h[3] + 1],
+    cta = [w[h[8] + 16 * i:h[8] + 16 * i + 16] for i in range(h[3])]  # what each CTA reads first
+    return dict(rows=h[1], cta=cta,
                 segs=[tuple(w[h[9] + 8 * i:h[9] + 8 * i + 8]) for i in range(h[4])],
                 tiles=w[h[10]:h[10] + h[5] + 1], row=[tuple(w[h[11] + 4 * i:h[11] + 4 * i + 4]) for i in range(h[1])])
 
@@ -195,8 +196,7 @@ def _plan(rows, lens, heads, kv, ctas):
 @pytest.mark.parametrize("seed", range(40))
 def test_plans_cover_every_tile_once(seed):
     """Every (query tile, kv head, token tile) of the shared parts belongs to
-    one CTA, each row finds the partial results of all its heads, and the CTAs'
-    shares differ by little."""
+    one CTA, and each row finds the partial results of all its heads."""
     r = random.Random(seed)
     n, kv = r.randint(1, 8), r.choice([1, 2, 4, 8])
     ratio = r.choice([1, 2, 3, 5, 8, 16])
@@ -204,8 +204,13 @@ def test_plans_cover_every_tile_once(seed):
     lens = [r.choice([0, 1, 15, 16, 127, 128, 129, 1000, 5000]) for _ in rows]
     ctas = r.choice([1, 3, 148])
     p = _plan(rows, lens, kv * ratio, kv, ctas)
-    assert p["rows"] == sum(rows) and p["cta"][0] == 0 and p["cta"][-1] == len(p["segs"])
-    assert p["cta"] == sorted(p["cta"]) and p["tiles"] == sorted(p["tiles"])
+    assert p["rows"] == sum(rows) and len(p["cta"]) <= ctas
+    assert [c[0] for c in p["cta"]] + [len(p["segs"])] == [0] + [c[1] for c in p["cta"]]
+    for first, last, *_, in p["cta"]:
+        assert first <= last
+    for c in p["cta"]:
+        assert c[0] == c[1] or tuple(c[8:]) == p["segs"][c[0]]
+    assert p["tiles"] == sorted(p["tiles"])
     seen = set()
     for row0, nq, q0, h, t0, t1, prefix, dual in p["segs"]:
         assert t0 < t1 and dual == (nq - q0 > 128)
@@ -217,8 +222,8 @@ def test_plans_cover_every_tile_once(seed):
         q = q // 16 * 16 if m > 1 else 0
         want += -(-q // 128) * kv * -(-m * ratio // 256) if q else 0
         for j in range(m):
-            prefix, tile0, query, _ = p["row"][row0 + j]
-            assert prefix == q and query == j * ratio
+            prefix, tile0, query, queries = p["row"][row0 + j]
+            assert prefix == q and query == j * ratio and queries == m * ratio
             for h in range(kv * ratio if q else 0):
                 qi = query + h % ratio
                 tile = tile0 + qi // 256 * kv + h // ratio
