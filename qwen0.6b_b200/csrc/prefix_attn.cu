@@ -155,16 +155,43 @@ __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, i
       : "memory");
 }
 
-// One tcgen05.mma (M = 128, K = 16) of a converged warp, by an elected lane:
-// A from shared memory / from tensor memory.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// Four steps (K = 16 each) of a product with M = 128, issued back to back by
+// an elected lane of a converged warp.  Each of them runs for 64 clocks at N =
+// 128; issued one by one, with an election and descriptor arithmetic between
+// them, they went out every 90 to 110 clocks and the tensor cores waited.
+// Scores: A and B from shared memory, a step is 32 bytes along their rows
+// (2 in a descriptor's address units).
+__device__ __forceinline__ void mma4_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
+      "{\n\t.reg .pred p, q, t;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+      "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
+      "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
       "elect.sync _|p, 0xffffffff;\n\t"
       "setp.ne.b32 q, %4, 0;\n\t"
-      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, q;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "setp.eq.b32 t, 0, 0;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, q;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, t;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
+// Values: A from tensor memory (a step is 8 columns), B MN-major in shared
+// memory (a step is 16 rows of 128 bytes: 128 address units).
+__device__ __forceinline__ void mma4_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q, t;\n\t.reg .b64 b1, b2, b3;\n\t.reg .b32 a1, a2, a3;\n\t"
+      "add.s32 a1, %1, 8;\n\tadd.s32 a2, %1, 16;\n\tadd.s32 a3, %1, 24;\n\t"
+      "add.s64 b1, %2, 128;\n\tadd.s64 b2, %2, 256;\n\tadd.s64 b3, %2, 384;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "setp.ne.b32 q, %4, 0;\n\t"
+      "setp.eq.b32 t, 0, 0;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, q;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, t;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, t;\n\t"
+      "@p tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, t;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// One step of it.
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
@@ -252,7 +279,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // gives 2^-126.  The special function unit makes 16 results a clock and SM,
 // which alone would take as long as the tile's products; kPolyOf8 of eight
 // pairs go this way instead.
-constexpr int kPolyOf8 = 3;
+constexpr int kPolyOf8 = 0;
 __device__ __forceinline__ void exp2_poly2(uint64_t x2, float &a, float &b) {
   float x, y;
   unpair2(x2, x, y);
@@ -468,11 +495,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (!ok) return;
         tc_fence_after();
         const uint32_t qa = smem_u32(sq + (dual ? st * QB : 0)), kb = smem_u32(ring + stage * TILE);
+        const uint64_t qd = sw128_desc(qa), kd = sw128_desc(kb);
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k >> 2) * (TN * 128) + (k & 3) * 32;
-          mma_ss(tmem + S_COL + st * 128, sw128_desc(qa + off), sw128_desc(kb + off), id_s, k != 0);
-        }
+        for (int h = 0; h < HALVES; ++h)  // 64 dims: TN rows of 128 bytes
+          mma4_ss(tmem + S_COL + st * 128, qd + h * (TN * 128 / 16), kd + h * (TN * 128 / 16), id_s, h);
         commit_elect(&s_full[st]);
         if (!dual || st == 1) commit_elect(&kv_empty[stage]);
       };
@@ -482,7 +508,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int st = i & 1, t = dual ? i >> 1 : i;
         const int place = ring0 + v_place(dual, t, nt), stage = place % ST;
         ok = gemm_wait(&kv_full[stage], (place / ST) & 1, abort, a.err, 1);
-        const uint32_t vb = smem_u32(ring + stage * TILE), pa = tmem + S_COL + st * 128;
+        const uint32_t pa = tmem + S_COL + st * 128;
+        const uint64_t vd = sw128_mn_desc(smem_u32(ring + stage * TILE), TN * 128);
         // Only the 16-token steps inside the prefix: what lies behind it in a
         // page may be anything (0 x NaN).  The first half of the tile's
         // weights is multiplied while the second is being computed.
@@ -492,8 +519,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
-          for (int k = 4 * half; k < min(ks, 4 * half + 4); ++k)
-            mma_ts(tmem + O_COL + st * 128, pa + 8 * k, sw128_mn_desc(vb + 2048 * k, TN * 128), id_o, k != 0 || i > 1);
+          if (ks >= 4 * half + 4)
+            mma4_ts(tmem + O_COL + st * 128, pa + 32 * half, vd + 512 * half, id_o, half != 0 || i > 1);
+          else
+            for (int k = 4 * half; k < ks; ++k)
+              mma_ts(tmem + O_COL + st * 128, pa + 8 * k, vd + 128 * k, id_o, k != 0 || i > 1);
         }
         if (!ok) break;
         ++steps[st];
