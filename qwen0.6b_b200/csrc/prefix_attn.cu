@@ -39,8 +39,6 @@ using qb200::mbar_init;
 using qb200::mbar_try_wait;
 using qb200::smem_u32;
 using qb200tc::ex2_approx;
-using qb200tc::gemm_record;
-using qb200tc::gemm_wait;
 using qb200tc::sw128_desc;
 using qb200tc::sw128_mn_desc;
 using qb200tc::tc_fence_after;
@@ -80,7 +78,12 @@ struct RowPlan {
 
 constexpr int TN = 128;      // tokens of a tile
 constexpr int QT = 128;      // queries of a stream's tile
-constexpr int THREADS = 320; // 10 warps: TMA, MMA, two streams of four softmax warps
+constexpr int THREADS = 384; // 3 warpgroups: TMA and MMA warps (two idle), two streams of four softmax warps
+// Registers after the split of the block's 384 x 168: the softmax warps hold a
+// query's 128 scores each, and with the shared memory taken by tiles there is
+// no L1 to spill to (a spilled value comes back from L2).
+constexpr int REGS_WORK = 88, REGS_SOFT = 208;
+static_assert(REGS_WORK + 2 * REGS_SOFT <= 3 * 168, "the split fits what the block was launched with");
 constexpr int OWN_THREADS = 128;
 
 struct Args {
@@ -105,6 +108,29 @@ struct Args {
   int after_prefix;    // the own kernel follows a prefix kernel of the same call
   float scale_log2;
 };
+
+// Status of a launch: the first code recorded stays.
+__device__ __forceinline__ void record(unsigned long long *err, uint32_t code) {
+  atomicCAS(err, 0ull, (static_cast<unsigned long long>(code) << 32) | (blockIdx.x & 0xffffffu));
+}
+
+// Bounded wait; false when it gave up (or another role already did).  Inline
+// like everything in the prefix kernel: a call would keep the compiler from
+// giving its warps different register counts.
+__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile uint32_t *abort,
+                                         unsigned long long *err) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = qb200::globaltimer_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*abort) return false;
+    if (static_cast<long long>(qb200::globaltimer_ns() - t0) > qb200tc::WAIT_NS) {
+      *abort = 1;
+      record(err, 1);
+      return false;
+    }
+  }
+  return true;
+}
 
 template <typename T>
 struct Type;
@@ -393,6 +419,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     return seq >= 0 && seq < a.num_seqs ? a.page_table + seq * a.table_pitch : nullptr;
   };
 
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_WORK));
   if (warp == 0) {
     // ---- K / V tiles into the ring
     int place = 0;  // tiles issued so far
@@ -409,7 +437,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       auto look = [&](int t, bool report) {
         bool bad = false;
         const int p = lane < wt * boxes ? page_of(row, s, (s.t0 + t) * boxes + lane, &bad) : a.num_pages;
-        if (bad && report && s.t0 + t + lane / boxes < s.t1) gemm_record(a.err, 3);
+        if (bad && report && s.t0 + t + lane / boxes < s.t1) record(a.err, 3);
         return p;
       };
       cur[0] = cur[1] = look(0, true);
@@ -448,7 +476,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           page = __shfl_sync(0xffffffffu, cur[0], (t - win[0]) * boxes + (lane < boxes ? lane : 0));
         }
         const int stage = place % ST;
-        if (place >= ST) ok = gemm_wait(&kv_empty[stage], ((place / ST) - 1) & 1, abort, a.err, 1);
+        if (place >= ST) ok = wait_bar(&kv_empty[stage], ((place / ST) - 1) & 1, abort, a.err);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&kv_full[stage], TILE);
@@ -469,7 +497,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint64_t t0 = qb200::globaltimer_ns();
       while (!mbar_try_wait(&kv_full[p % ST], (p / ST) & 1))
         if (static_cast<long long>(qb200::globaltimer_ns() - t0) > qb200tc::WAIT_NS) {
-          if (lane == 0) gemm_record(a.err, 1);
+          if (lane == 0) record(a.err, 1);
           break;
         }
     }
@@ -483,14 +511,14 @@ __global__ void __launch_bounds__(THREADS, 1)
       const Seg s = segment(si);
       const bool dual = s.dual != 0;
       const int nt = s.t1 - s.t0, n = dual ? 2 * nt : nt;
-      ok = gemm_wait(q_full, (si - seg0) & 1, abort, a.err, 1);
+      ok = wait_bar(q_full, (si - seg0) & 1, abort, a.err);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
       auto score = [&](int i) {  // S of step i
         const int st = i & 1, t = dual ? i >> 1 : i;
         const int place = ring0 + k_place(dual, t), stage = place % ST;
-        ok = gemm_wait(&kv_full[stage], (place / ST) & 1, abort, a.err, 1);
+        ok = wait_bar(&kv_full[stage], (place / ST) & 1, abort, a.err);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) return;
         tc_fence_after();
@@ -507,7 +535,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int i = 0; i < n && ok; ++i) {
         const int st = i & 1, t = dual ? i >> 1 : i;
         const int place = ring0 + v_place(dual, t, nt), stage = place % ST;
-        ok = gemm_wait(&kv_full[stage], (place / ST) & 1, abort, a.err, 1);
+        ok = wait_bar(&kv_full[stage], (place / ST) & 1, abort, a.err);
         const uint32_t pa = tmem + S_COL + st * 128;
         const uint64_t vd = sw128_mn_desc(smem_u32(ring + stage * TILE), TN * 128);
         // Only the 16-token steps inside the prefix: what lies behind it in a
@@ -515,7 +543,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         // weights is multiplied while the second is being computed.
         const int ks = min(TN, s.prefix - (s.t0 + t) * TN) / 16;
         for (int half = 0; half < 2; ++half) {
-          ok = ok && gemm_wait(&p_full[2 * st + half], steps[st] & 1, abort, a.err, 1);
+          ok = ok && wait_bar(&p_full[2 * st + half], steps[st] & 1, abort, a.err);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
@@ -538,11 +566,24 @@ __global__ void __launch_bounds__(THREADS, 1)
       commit_elect(o_full);
     }
     __syncwarp();
+  }
+  __syncwarp();
+  tc_fence_before();
+  qb200::named_bar_sync(0, THREADS);
+  if (warp == 1) {
+    if (*abort) {  // wait (bounded) for the MMAs still in flight
+      const uint64_t t0 = qb200::globaltimer_ns();
+      while (!mbar_try_wait(o_full, 0) && !mbar_try_wait(o_full, 1))
+        if (static_cast<long long>(qb200::globaltimer_ns() - t0) > qb200tc::WAIT_NS) break;
+    }
+    tmem_dealloc(tmem, 512);
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFT));
     // ---- softmax: thread = query
-    const int st = warp >= 6 ? 1 : 0;
+    const int st = (warp - 4) >> 2;
     const int quad = warp & 3, ql = 32 * quad + lane;
-    const int tid = threadIdx.x - 64;  // 0..255
+    const int tid = threadIdx.x - 128;  // 0..255
     const uint32_t ts = tmem + S_COL + st * 128 + (static_cast<uint32_t>(32 * quad) << 16);
     const uint32_t to = tmem + O_COL + st * 128 + (static_cast<uint32_t>(32 * quad) << 16);
     int steps = 0;
@@ -603,7 +644,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int i = 0; i < my_steps && ok; ++i) {
         const int t = s.t0 + (dual ? i : 2 * i + st);
         const int ntok = min(TN, s.prefix - t * TN);
-        ok = gemm_wait(&s_full[st], steps & 1, abort, a.err, 1);
+        ok = wait_bar(&s_full[st], steps & 1, abort, a.err);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         ++steps;
@@ -695,7 +736,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[2 * st + 1]);
       }
-      ok = ok && gemm_wait(o_full, (si - seg0) & 1, abort, a.err, 1);
+      ok = ok && wait_bar(o_full, (si - seg0) & 1, abort, a.err);
       ok = !qb200::named_bar_or(1, 256, !ok || *abort);  // all eight warps go on, or none
       if (!ok) break;
       tc_fence_after();
@@ -759,19 +800,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (both) qb200::named_bar_sync(1, 256);
     }
-  }
-  __syncwarp();
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    if (*abort) {  // wait (bounded) for the MMAs still in flight
-      const uint64_t t0 = qb200::globaltimer_ns();
-      const int done = seg1 - seg0;
-      (void)done;
-      while (!mbar_try_wait(o_full, 0) && !mbar_try_wait(o_full, 1))
-        if (static_cast<long long>(qb200::globaltimer_ns() - t0) > qb200tc::WAIT_NS) break;
-    }
-    tmem_dealloc(tmem, 512);
+    __syncwarp();
+    tc_fence_before();
+    qb200::named_bar_sync(0, THREADS);
   }
 }
 
@@ -922,7 +953,7 @@ __global__ void __launch_bounds__(OWN_THREADS, 5) own_kernel(const Args a) {
   int seq;
   const int len = row_length(a, row, &seq);
   const RowPlan rp = a.row_plan[row];
-  if (len < 0 && threadIdx.x == 0) gemm_record(a.err, 3);
+  if (len < 0 && threadIdx.x == 0) record(a.err, 3);
   const int start = len >= rp.prefix ? rp.prefix : 0;
   const int count = max(0, len - start);
   // Tokens of one split: a multiple of 64 that covers the row.
@@ -954,7 +985,7 @@ __global__ void __launch_bounds__(OWN_THREADS, 5) own_kernel(const Args a) {
       if (page >= 0 && page < a.num_pages)
         where = page * a.page_stride + static_cast<long long>(b - pi * a.page_tokens) * a.token_stride;
       else
-        gemm_record(a.err, 3);
+        record(a.err, 3);
     }
   };
   lookup(0);
