@@ -114,22 +114,27 @@ __device__ __forceinline__ void record(unsigned long long *err, uint32_t code) {
   atomicCAS(err, 0ull, (static_cast<unsigned long long>(code) << 32) | (blockIdx.x & 0xffffffu));
 }
 
-// Bounded wait; false when it gave up (or another role already did).  Inline
-// like everything in the prefix kernel: a call would keep the compiler from
-// giving its warps different register counts.
+// Bounded wait of a whole warp; false for all its lanes when it gave up (or
+// another role already did).  The lanes may leave the loop apart and meet
+// again in the vote: what follows a wait is warp-collective (tensor memory
+// accesses, elections, named barriers, which count a warp once per group of
+// lanes that arrives).  Inline like everything in the prefix kernel: a call
+// would keep the compiler from giving its warps different register counts.
 __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile uint32_t *abort,
                                          unsigned long long *err) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = qb200::globaltimer_ns();
-  while (!mbar_try_wait(bar, parity)) {
-    if (*abort) return false;
-    if (static_cast<long long>(qb200::globaltimer_ns() - t0) > qb200tc::WAIT_NS) {
-      *abort = 1;
-      record(err, 1);
-      return false;
+  bool ok = mbar_try_wait(bar, parity);
+  if (!ok) {
+    const uint64_t t0 = qb200::globaltimer_ns();
+    while (!(ok = mbar_try_wait(bar, parity))) {
+      if (*abort) break;
+      if (static_cast<long long>(qb200::globaltimer_ns() - t0) > qb200tc::WAIT_NS) {
+        *abort = 1;
+        record(err, 1);
+        break;
+      }
     }
   }
-  return true;
+  return __all_sync(0xffffffffu, ok);
 }
 
 template <typename T>
@@ -363,12 +368,13 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint8_t *sq = base, *ring = base + 2 * QB;
   uint64_t *kv_full = reinterpret_cast<uint64_t *>(ring + ST * TILE);
   uint64_t *kv_empty = kv_full + ST;
-  uint64_t *s_full = kv_empty + ST, *p_full = s_full + 2, *q_full = p_full + 4, *o_full = q_full + 1;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(o_full + 1);
+  uint64_t *s_full = kv_empty + ST, *p_full = s_full + 2, *q_full = p_full + 4, *o_full = q_full + 1,
+           *drained = o_full + 1;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drained + 1);
   volatile uint32_t *abort = tmem_slot + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  if (threadIdx.x == 32) {
+  if (threadIdx.x == 96) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_k)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_v)) : "memory");
   }
@@ -384,9 +390,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     mbar_init(q_full, 8);
     mbar_init(o_full, 1);
+    mbar_init(drained, 1);
     *abort = 0;
+    abort[1] = 0;  // never set: the wait for what is in flight is not cut short
     qb200::fence_mbar_init();
   }
+  __syncwarp();
   if (warp == 1) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
@@ -477,7 +486,6 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         const int stage = place % ST;
         if (place >= ST) ok = wait_bar(&kv_empty[stage], ((place / ST) - 1) & 1, abort, a.err);
-        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&kv_full[stage], TILE);
         __syncwarp();
@@ -512,39 +520,43 @@ __global__ void __launch_bounds__(THREADS, 1)
       const bool dual = s.dual != 0;
       const int nt = s.t1 - s.t0, n = dual ? 2 * nt : nt;
       ok = wait_bar(q_full, (si - seg0) & 1, abort, a.err);
-      ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
+      // The K tile of step i, if there is one (a copy has nothing to do with
+      // the tensor cores' own ordering: no fence).
+      auto k_ready = [&](int i) {
+        if (i >= n) return true;
+        const int place = ring0 + k_place(dual, dual ? i >> 1 : i);
+        return wait_bar(&kv_full[place % ST], (place / ST) & 1, abort, a.err);
+      };
       auto score = [&](int i) {  // S of step i
-        const int st = i & 1, t = dual ? i >> 1 : i;
-        const int place = ring0 + k_place(dual, t), stage = place % ST;
-        ok = wait_bar(&kv_full[stage], (place / ST) & 1, abort, a.err);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) return;
-        tc_fence_after();
-        const uint32_t qa = smem_u32(sq + (dual ? st * QB : 0)), kb = smem_u32(ring + stage * TILE);
-        const uint64_t qd = sw128_desc(qa), kd = sw128_desc(kb);
+        const int st = i & 1, stage = (ring0 + k_place(dual, dual ? i >> 1 : i)) % ST;
+        const uint64_t qd = sw128_desc(smem_u32(sq + (dual ? st * QB : 0))), kd = sw128_desc(smem_u32(ring + stage * TILE));
 #pragma unroll
         for (int h = 0; h < HALVES; ++h)  // 64 dims: TN rows of 128 bytes
           mma4_ss(tmem + S_COL + st * 128, qd + h * (TN * 128 / 16), kd + h * (TN * 128 / 16), id_s, h);
         commit_elect(&s_full[st]);
         if (!dual || st == 1) commit_elect(&kv_empty[stage]);
       };
+      ok = k_ready(0) && k_ready(1);
+      if (!ok) break;
       score(0);
-      if (ok && n > 1) score(1);
+      if (n > 1) score(1);
       for (int i = 0; i < n && ok; ++i) {
         const int st = i & 1, t = dual ? i >> 1 : i;
+        // Both tiles of the step are waited for while the tensor cores still
+        // work on the last one.
         const int place = ring0 + v_place(dual, t, nt), stage = place % ST;
-        ok = wait_bar(&kv_full[stage], (place / ST) & 1, abort, a.err);
+        ok = wait_bar(&kv_full[stage], (place / ST) & 1, abort, a.err) && k_ready(i + 2);
         const uint32_t pa = tmem + S_COL + st * 128;
         const uint64_t vd = sw128_mn_desc(smem_u32(ring + stage * TILE), TN * 128);
         // Only the 16-token steps inside the prefix: what lies behind it in a
         // page may be anything (0 x NaN).  The first half of the tile's
         // weights is multiplied while the second is being computed.
         const int ks = min(TN, s.prefix - (s.t0 + t) * TN) / 16;
+#pragma unroll
         for (int half = 0; half < 2; ++half) {
           ok = ok && wait_bar(&p_full[2 * st + half], steps[st] & 1, abort, a.err);
-          ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
           if (ks >= 4 * half + 4)
@@ -562,22 +574,16 @@ __global__ void __launch_bounds__(THREADS, 1)
       commit_elect(o_full);
       ring0 += 2 * nt;
     }
-    if (!ok) {  // tensor memory is freed only after every issued MMA has completed
-      commit_elect(o_full);
-    }
+    // Tensor memory is freed, and the CTA ends, only after every product and
+    // every arrival that was asked for (also after an abort).
+    commit_elect(drained);
+    wait_bar(drained, 0, abort + 1, a.err);
     __syncwarp();
   }
   __syncwarp();
   tc_fence_before();
   qb200::named_bar_sync(0, THREADS);
-  if (warp == 1) {
-    if (*abort) {  // wait (bounded) for the MMAs still in flight
-      const uint64_t t0 = qb200::globaltimer_ns();
-      while (!mbar_try_wait(o_full, 0) && !mbar_try_wait(o_full, 1))
-        if (static_cast<long long>(qb200::globaltimer_ns() - t0) > qb200tc::WAIT_NS) break;
-    }
-    tmem_dealloc(tmem, 512);
-  }
+  if (warp == 1) tmem_dealloc(tmem, 512);
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFT));
     // ---- softmax: thread = query
@@ -645,7 +651,6 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int t = s.t0 + (dual ? i : 2 * i + st);
         const int ntok = min(TN, s.prefix - t * TN);
         ok = wait_bar(&s_full[st], steps & 1, abort, a.err);
-        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         ++steps;
         tc_fence_after();
@@ -664,14 +669,17 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int c = 0; c < TN; ++c)
               if (c >= ntok || ((valid >> (c >> a.box_shift)) & 1u) == 0) v[c >> 6][c & 63] = -INFINITY;
           }
-          float mx[4];
+          float mx[8];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mx[k] = max3(v[0][k], v[0][k + 4], v[0][k + 4]);
+          for (int k = 0; k < 8; ++k) mx[k] = max3(v[0][k], v[0][k + 8], v[0][k + 16]);
 #pragma unroll
-          for (int c = 8; c < TN; c += 8)
+          for (int c = 24; c + 8 < TN; c += 16)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mx[k] = max3(mx[k], v[c >> 6][(c & 63) + k], v[c >> 6][(c & 63) + k + 4]);
-          const float rowmax = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * a.scale_log2;
+            for (int k = 0; k < 8; ++k) mx[k] = max3(mx[k], v[c >> 6][(c & 63) + k], v[(c + 8) >> 6][((c + 8) & 63) + k]);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) mx[k] = max3(mx[k], v[1][56 + k], v[1][56 + k]);
+          const float rowmax =
+              max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), max3(mx[6], mx[7], mx[7])) * a.scale_log2;
           if (i == 0) {
             m = rowmax;
           } else if (__any_sync(0xffffffffu, !(rowmax <= m + 8.f))) {
@@ -717,7 +725,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               w[k] = Type<T>::pack(x, y);
             }
             tmem_st16(ts + c0 / 2, w);
-            if (c0 == 32) {
+            if (c0 == 64) {  // announces the first half without a pause for its stores
               tmem_wait_st();
               tc_fence_before();
               __syncwarp();
@@ -761,6 +769,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           s_ml[0][ql] = m;
           s_ml[1][ql] = l;
         }
+        __syncwarp();
         qb200::named_bar_sync(1, 256);
         if (st == 0 && live) {
           const float m1 = s_ml[0][ql], l1 = s_ml[1][ql];
@@ -774,6 +783,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           m = mn;
         }
+        __syncwarp();
       }
       if (live && (dual || st == 0)) {
         float *slot = a.slots + (static_cast<size_t>(si) * 2 + st) * kStreamFloats<D>;
@@ -798,6 +808,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         slot[QT * D + ql] = m;
         slot[QT * D + QT + ql] = l;
       }
+      __syncwarp();
       if (both) qb200::named_bar_sync(1, 256);
     }
     __syncwarp();
