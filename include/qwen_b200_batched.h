@@ -160,6 +160,20 @@ int qwen_b200_batched_step_logits(void *handle, int rows, const int *seq_ids, co
                                   const int *tokens_in, float *logits, long long ld, float *norm_out,
                                   int max_position, float attn_scale, void *stream);
 
+/* A step whose rows share prefixes (paged pools only; no upstream
+ * counterpart): the attention of every layer is qwen_b200_prefix_attention
+ * (include/qwen_b200_paged.h) under the plan `plan_header` (host) / `plan`
+ * (device) of these rows, 16 / 8 heads, with a workspace of
+ * qwen_b200_prefix_workspace(plan_header, 128, max_length) bytes; max_length
+ * as there.  Consecutive rows of a group must hold the same tokens in their
+ * sequences' first prefix_lens[g] positions (e.g. after a fork).  Writes the
+ * greedy tokens (tokens_out, logits NULL) or the logits (tokens_out NULL). */
+int qwen_b200_batched_step_prefix(void *handle, int rows, const int *seq_ids, const int *positions,
+                                  const int *tokens_in, int *tokens_out, float *logits, long long ld,
+                                  float *norm_out, const int *plan_header, void *plan, void *workspace,
+                                  long long workspace_bytes, int max_length, float attn_scale,
+                                  void *stream);
+
 /* Synchronises the device; returns 0 if no batched kernel has recorded an
  * error since the last call, else its code (1: a bounded wait gave up, 2: a
  * token id outside the vocabulary, 3: a sequence id or position outside the

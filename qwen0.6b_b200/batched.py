@@ -23,6 +23,8 @@ import os
 
 import torch
 
+from paged import PrefixPlan, compact_pages, copy_pages, fork_pages, free_pages
+
 _PKG = os.path.dirname(os.path.abspath(__file__))
 _lib = None
 
@@ -55,6 +57,9 @@ def lib() -> ctypes.CDLL:
         L.qwen_b200_batched_step.argtypes = [vp, i, vp, vp, vp, vp, vp, i, ctypes.c_float, vp]
         L.qwen_b200_batched_step_logits.restype = i
         L.qwen_b200_batched_step_logits.argtypes = [vp, i, vp, vp, vp, vp, ll, vp, i, ctypes.c_float, vp]
+        L.qwen_b200_batched_step_prefix.restype = i
+        L.qwen_b200_batched_step_prefix.argtypes = [vp, i, vp, vp, vp, vp, vp, ll, vp, vp, vp, vp, ll, i,
+                                                    ctypes.c_float, vp]
         L.qwen_b200_batched_status.restype = i
         L.qwen_b200_batched_status.argtypes = [vp, ctypes.POINTER(ctypes.c_uint64)]
         L.qwen_b200_batched_destroy.restype = None
@@ -95,12 +100,29 @@ PAGE = 128  # tokens per KV page
 
 class PagePool:
     """Host bookkeeping of paged KV pools: which page holds positions
-    [128 i, 128 i + 128) of each sequence (-1: none), and the free pages."""
+    [128 i, 128 i + 128) of each sequence (-1: none), how many sequences hold
+    each page, and the free pages.  The methods that change shared pages return
+    what has to happen on the device."""
 
     def __init__(self, num_pages: int, num_seqs: int, max_pages: int):
         self.num_pages, self.num_seqs, self.max_pages = num_pages, num_seqs, max_pages
         self.table = [[-1] * max_pages for _ in range(num_seqs)]
+        self.refs = [0] * num_pages
         self.free = list(range(num_pages - 1, -1, -1))  # pop() hands out the lowest page first
+
+    def _take(self) -> int:
+        page = self.free.pop()
+        self.refs[page] = 1
+        return page
+
+    def _drop(self, page: int) -> None:
+        self.refs[page] -= 1
+        if self.refs[page] == 0:
+            self.free.append(page)
+
+    def _enough(self, pages: int) -> None:
+        if pages > len(self.free):
+            raise RuntimeError(f"KV page pool exhausted ({self.num_pages} pages of {PAGE} tokens)")
 
     def reserve(self, seq: int, upto_position: int) -> bool:
         """Maps pages for positions 0..upto_position; True if the row changed."""
@@ -109,18 +131,76 @@ class PagePool:
             raise ValueError(f"sequence {seq} / position {upto_position} outside the page table")
         row = self.table[seq]
         missing = [i for i in range(need) if row[i] < 0]
-        if len(missing) > len(self.free):
-            raise RuntimeError(f"KV page pool exhausted ({self.num_pages} pages of {PAGE} tokens)")
+        self._enough(len(missing))
         for i in missing:
-            row[i] = self.free.pop()
+            row[i] = self._take()
         return bool(missing)
+
+    def unshare(self, seq: int, write_from: int, upto_position: int) -> list[tuple[int, int, int]]:
+        """Gives sequence `seq` pages of its own for the positions
+        write_from..upto_position, which are about to be written, where it
+        shares them with another one: (source, destination, tokens to copy) of
+        each; the tokens before write_from stay, those behind it are dropped."""
+        row = self.table[seq]
+        shared = [i for i in range(write_from // PAGE, upto_position // PAGE + 1) if row[i] >= 0 and self.refs[row[i]] > 1]
+        self._enough(len(shared))
+        moves = []
+        for i in shared:
+            src, row[i] = row[i], self._take()
+            self._drop(src)
+            moves.append((src, row[i], max(0, write_from - i * PAGE)))
+        return moves
+
+    def fork(self, parent: int, children: list[int], length: int) -> list[int]:
+        """Makes the children (sequences without pages) copies of the parent's
+        first `length` positions: its full pages are shared, the last, partly
+        filled one is a new page of each child.  Returns those pages (-1:
+        none)."""
+        full, tail = divmod(length, PAGE)
+        if not 0 <= parent < self.num_seqs or not 0 <= length <= self.max_pages * PAGE:
+            raise ValueError(f"sequence {parent} / length {length} outside the page table")
+        pages = self.table[parent][:full + (tail > 0)]
+        if any(p < 0 for p in pages):
+            raise ValueError(f"sequence {parent} has no page for some of its first {length} positions")
+        if len(set(children)) != len(children) or parent in children:
+            raise ValueError("children must be distinct and differ from the parent")
+        for c in children:
+            if not 0 <= c < self.num_seqs or any(p >= 0 for p in self.table[c]):
+                raise ValueError(f"sequence {c} is outside the page table or still holds pages (release it first)")
+        if tail:
+            self._enough(len(children))
+        new = []
+        for c in children:
+            for i in range(full):
+                self.table[c][i] = pages[i]
+                self.refs[pages[i]] += 1
+            if tail:
+                self.table[c][full] = self._take()
+            new.append(self.table[c][full] if tail else -1)
+        return new
 
     def release(self, seq: int) -> None:
         row = self.table[seq]
         for i, pg in enumerate(row):
             if pg >= 0:
-                self.free.append(pg)
+                self._drop(pg)
                 row[i] = -1
+
+    def compact(self) -> tuple[list[int], list[int]]:
+        """Renames the pages in use so that they are 0..in_use - 1: the moves
+        (sources, destinations)."""
+        used = self.in_use
+        src = [p for p in range(used, self.num_pages) if self.refs[p]]
+        dst = [p for p in range(used) if not self.refs[p]]
+        name = dict(zip(src, dst))
+        for row in self.table:
+            for i, p in enumerate(row):
+                if p in name:
+                    row[i] = name[p]
+        for a, b in name.items():
+            self.refs[b], self.refs[a] = self.refs[a], 0
+        self.free = list(range(self.num_pages - 1, used - 1, -1))
+        return src, dst
 
     @property
     def in_use(self) -> int:
@@ -141,6 +221,10 @@ class BatchedDecoder:
     are used (``prefill``, ``prefill_parallel`` and ``generate`` do it), and
     ``release`` returns a finished sequence's pages.  max_seq may then exceed
     2048 (RoPE tables are rebuilt to max_seq rows when the weights' are shorter).
+    Sequences can share pages: ``fork`` makes copies of a sequence that share
+    its full pages, ``generate_shared`` continues many prompts that begin alike
+    (their common part is computed, kept and attended to once), ``compact``
+    moves the pages in use to the front of the pools.
     """
 
     def __init__(self, weights: dict, num_seqs: int, max_rows: int | None = None,
@@ -208,22 +292,57 @@ class BatchedDecoder:
         self._h = h
 
     # ----------------------------------------------------------- paged pools
-    def reserve(self, seq: int, upto_position: int) -> None:
+    def reserve(self, seq: int, upto_position: int, write_from: int | None = None) -> None:
         """Maps pages for positions 0..upto_position of sequence `seq` (paged
-        pools; a no-op otherwise).  Raises when the pool is exhausted."""
+        pools; a no-op otherwise).  Raises when the pool is exhausted.
+        Positions write_from (default: upto_position) .. upto_position are about
+        to be written: pages of them that the sequence shares with others
+        become its own, with the tokens before write_from copied."""
         if not self.paged:
             return
         if not 0 <= upto_position < self.max_seq:
             raise ValueError(f"position {upto_position} outside [0, {self.max_seq})")
-        if self.pages.reserve(seq, upto_position):
+        write_from = upto_position if write_from is None else write_from
+        if not 0 <= write_from <= upto_position:
+            raise ValueError(f"write_from {write_from} outside [0, {upto_position}]")
+        changed = self.pages.reserve(seq, upto_position)
+        moves = self.pages.unshare(seq, write_from, upto_position)
+        if any(t for _, _, t in moves):
+            copy_pages(self.k_pool, self.v_pool, *zip(*moves))
+        if changed or moves:
             self.page_table[seq].copy_(torch.tensor(self.pages.table[seq], dtype=torch.int32))
 
-    def release(self, seq: int) -> None:
-        """Returns every page of sequence `seq` to the pool (paged pools)."""
+    def release(self, seq: int | list[int]) -> None:
+        """Returns every page of sequence `seq` (or of each in a list) to the
+        pool, once no other sequence holds it (paged pools)."""
         if not self.paged:
             return
-        self.pages.release(seq)
-        self.page_table[seq].fill_(-1)
+        seqs = [seq] if isinstance(seq, int) else list(seq)
+        for s in seqs:
+            self.pages.release(s)
+        free_pages(self.page_table, seqs)
+
+    def fork(self, parent: int, children: list[int], length: int) -> None:
+        """Makes the sequences `children` (without pages: new or released)
+        copies of the first `length` positions of `parent` (paged pools).  The
+        parent's full pages are shared, the tokens of the last, partly filled
+        one are copied; reserve() before a raw step writes into shared pages
+        (``prefill*`` and ``generate*`` do)."""
+        if not self.paged:
+            raise ValueError("fork needs paged pools")
+        children = list(children)
+        new = self.pages.fork(parent, children, length)
+        n = len(children)
+        fork_pages(self.page_table, self.k_pool, self.v_pool, [parent] * n, children, [length] * n, new)
+
+    def compact(self) -> int:
+        """Moves the pages in use to the front of the pools (paged pools);
+        returns how many moved."""
+        if not self.paged:
+            raise ValueError("compact needs paged pools")
+        src, dst = self.pages.compact()
+        compact_pages(self.page_table, self.k_pool, self.v_pool, src, dst)
+        return len(src)
 
     @property
     def pages_in_use(self) -> int:
@@ -242,12 +361,16 @@ class BatchedDecoder:
 
     def step(self, seq_ids: torch.Tensor, positions: torch.Tensor, tokens: torch.Tensor,
              max_position: int, norm_out: torch.Tensor | None = None,
-             out: torch.Tensor | None = None, sampling=None) -> torch.Tensor:
+             out: torch.Tensor | None = None, sampling=None,
+             prefix: PrefixPlan | None = None) -> torch.Tensor:
         """One step of rows = len(seq_ids) sequences (device int32 tensors):
         greedy, or drawn with ``sampling`` (a ``sampling.SamplingParams``; each
         row's random stream is keyed by its sequence id and position, so a
         draw does not depend on the batch composition).  Returns the device
-        int32 tensor of produced tokens.  No host synchronisation."""
+        int32 tensor of produced tokens.  No host synchronisation.
+        prefix (paged pools): the rows' groups that share a prefix, a
+        ``paged.PrefixPlan`` for these rows (16 / 8 heads of 128); the shared
+        part of each group is then attended to once for all its rows."""
         rows = int(seq_ids.numel())
         for t in (seq_ids, positions, tokens):
             if t.dtype != torch.int32 or t.device != self.dev or not t.is_contiguous():
@@ -259,6 +382,28 @@ class BatchedDecoder:
             from sampling import sample
             if getattr(self, "_logits", None) is None:
                 self._logits = torch.empty(self.max_rows, VOCAB, dtype=torch.float32, device=self.dev)
+        if prefix is not None:
+            if not self.paged:
+                raise ValueError("a shared prefix needs paged pools")
+            if (prefix.rows, prefix.num_q_heads, prefix.num_kv_heads, prefix.head_dim) != (rows, NQ, NKV, HD):
+                raise ValueError(f"the plan is for {prefix.rows} rows of {prefix.num_q_heads} / "
+                                 f"{prefix.num_kv_heads} heads of {prefix.head_dim}, the step has {rows} rows")
+            if prefix.device != self.dev:
+                raise ValueError(f"the plan is on {prefix.device}, the decoder on {self.dev}")
+            # From the caching allocator with every step, so that captured steps have one each.
+            ws = torch.empty(prefix.workspace_bytes, dtype=torch.uint8, device=self.dev)
+            with torch.cuda.device(self.dev):
+                _check(lib().qwen_b200_batched_step_prefix(
+                    self._h, rows, seq_ids.data_ptr(), positions.data_ptr(), tokens.data_ptr(),
+                    None if sampling is not None else out.data_ptr(),
+                    self._logits.data_ptr() if sampling is not None else None, VOCAB,
+                    norm_out.data_ptr() if norm_out is not None else None, prefix.header.data_ptr(),
+                    prefix.words.data_ptr(), ws.data_ptr(), prefix.workspace_bytes, prefix.max_length, self.attn_scale,
+                    ctypes.c_void_p(stream)), "batched_step_prefix")
+            if sampling is None:
+                return out
+            return sample(self._logits[:rows], sampling, out=out, row_seq=seq_ids, row_pos=positions)
+        if sampling is not None:
             _check(lib().qwen_b200_batched_step_logits(
                 self._h, rows, seq_ids.data_ptr(), positions.data_ptr(), tokens.data_ptr(),
                 self._logits.data_ptr(), VOCAB, norm_out.data_ptr() if norm_out is not None else None,
@@ -329,11 +474,53 @@ class BatchedDecoder:
             raise ValueError("generation would run past max_seq")
         outs = []
         for i, p in enumerate(prompts):
-            self.reserve(i, len(p) - 1 + max_tokens - 1)
+            self.reserve(i, len(p) - 1 + max_tokens - 1, write_from=len(p) - 1)
         for s in range(max_tokens):
             nxt = self.step(ids, pos, tok, start_max + s,
                             out=torch.empty(n, dtype=torch.int32, device=self.dev), sampling=sampling)
             outs.append(nxt)
             tok = nxt
+            pos = pos + 1
+        return torch.stack(outs, 1).cpu().tolist()
+
+    def generate_shared(self, prefix: list[int], suffixes: list[list[int]], max_tokens: int,
+                        sampling=None) -> list[list[int]]:
+        """`max_tokens` tokens after each prompt ``prefix + suffixes[i]``
+        (suffixes may be empty: several completions of one prompt), greedy or
+        drawn with ``sampling``.  Paged pools.  Sequence i holds prompt i; the
+        prefix is prefilled once, its full pages are shared by all sequences
+        and every step attends to it once for the whole batch.  The sequences
+        must hold no pages; they keep theirs afterwards (``release``)."""
+        if not self.paged:
+            raise ValueError("generate_shared needs paged pools")
+        n = len(suffixes)
+        prompts = [list(prefix) + list(s) for s in suffixes]
+        if not 1 <= n <= min(self.max_rows, self.num_seqs) or any(len(p) < 1 for p in prompts):
+            raise ValueError(f"{n} prompts: 1 to {min(self.max_rows, self.num_seqs)}, none of them empty")
+        longest = max(len(p) for p in prompts) - 1 + max_tokens
+        if max_tokens < 1 or longest > self.max_seq:
+            raise ValueError("generation would run past max_seq")
+        # Shared positions: the prefix, but for a last token that some prompt still has to feed.
+        shared = min(len(prefix), min(len(p) for p in prompts) - 1)
+        self.prefill_parallel([prompts[0][:shared + 1]], seqs=[0])
+        self.fork(0, list(range(1, n)), shared)
+        dev = dict(dtype=torch.int32, device=self.dev)
+
+        def plan(rows: int) -> PrefixPlan:
+            return PrefixPlan([rows], [shared], NQ, NKV, HD, max_length=longest, device=self.dev)
+
+        for i, p in enumerate(prompts):
+            self.reserve(i, len(p) - 1 + max_tokens - 1, write_from=shared)
+        rows = [(i, t, p[t]) for i, p in enumerate(prompts) for t in range(shared, len(p) - 1)]
+        for c0 in range(0, len(rows), self.max_rows):
+            ids, pos, tok = (torch.tensor(v, **dev) for v in zip(*rows[c0:c0 + self.max_rows]))
+            self.step(ids, pos, tok, int(pos.max()), out=torch.empty(len(ids), **dev), prefix=plan(len(ids)))
+        ids = torch.arange(n, **dev)
+        pos = torch.tensor([len(p) - 1 for p in prompts], **dev)
+        tok = torch.tensor([p[-1] for p in prompts], **dev)
+        steps, outs = plan(n), []
+        for s in range(max_tokens):
+            tok = self.step(ids, pos, tok, longest - 1, out=torch.empty(n, **dev), sampling=sampling, prefix=steps)
+            outs.append(tok)
             pos = pos + 1
         return torch.stack(outs, 1).cpu().tolist()

@@ -41,6 +41,7 @@
 #include "host_err.h"
 #include "ptx.cuh"
 #include "qwen_b200_batched.h"
+#include "qwen_b200_paged.h"
 
 namespace qb200b {
 
@@ -950,8 +951,11 @@ bool run_proj_slices(Plan *p, int i, const GemmPlan &gp, const GemmArgs &g, floa
 }
 
 // Every layer of a step plus the final RMSNorm (w.norm16 feeds the lm_head).
+// With `shared` (everything but the layer's pools filled in) the attention of
+// each layer is the shared-prefix one.
 int step_layers(Plan *p, int rows, const int *seq_ids, const int *positions, const int *tokens_in,
-                float *norm_out, int max_position, float attn_scale, cudaStream_t st) {
+                float *norm_out, int max_position, float attn_scale, cudaStream_t st,
+                QwenPrefixAttention *shared = nullptr) {
   const Workspace &w = p->ws;
   // The norm kernels take one warp per row; one-warp CTAs spread the rows
   // over all SMs (eight rows per CTA put the 256 rows of a step on 32 SMs).
@@ -986,12 +990,19 @@ int step_layers(Plan *p, int rows, const int *seq_ids, const int *positions, con
            static_cast<const __half *>(L.q_norm), static_cast<const __half *>(L.k_norm), p->cos_t,
            p->sin_t, seq_ids, positions, p->k_pool, p->v_pool, w.qrot, l, p->kg, p->max_seq,
            p->num_seqs, w.err);
-    LAUNCH(attn_split_kernel, dim3(nsplit, NKV, rows), dim3(ATT_THREADS), smem, p->tm_k,
-           static_cast<const __half *>(w.qrot), static_cast<const __half *>(p->k_pool),
-           static_cast<const __half *>(p->v_pool), seq_ids, positions, w.part, l, p->kg,
-           p->max_seq, p->max_splits, p->num_seqs, attn_scale, w.err);
-    LAUNCH(attn_combine_kernel, dim3(NQ, rows), dim3(HD), 0, static_cast<const float *>(w.part),
-           positions, w.attn, p->max_splits);
+    if (shared != nullptr) {
+      const size_t layer = static_cast<size_t>(l) * NKV * PAGE * HD;
+      shared->k_pool = p->k_pool + layer;
+      shared->v_pool = p->v_pool + layer;
+      if (int rc = qwen_b200_prefix_attention(shared, st)) return rc;
+    } else {
+      LAUNCH(attn_split_kernel, dim3(nsplit, NKV, rows), dim3(ATT_THREADS), smem, p->tm_k,
+             static_cast<const __half *>(w.qrot), static_cast<const __half *>(p->k_pool),
+             static_cast<const __half *>(p->v_pool), seq_ids, positions, w.part, l, p->kg,
+             p->max_seq, p->max_splits, p->num_seqs, attn_scale, w.err);
+      LAUNCH(attn_combine_kernel, dim3(NQ, rows), dim3(HD), 0, static_cast<const float *>(w.part),
+             positions, w.attn, p->max_splits);
+    }
     g.out = w.act;
     g.ldo = H;
     g.res = w.hidden;
@@ -1080,6 +1091,74 @@ int qwen_b200_batched_step_logits(void *handle, int rows, const int *seq_ids, co
   g.out = logits;
   g.ldo = static_cast<int>(ld);
   if (int rc = qb200_gemm_run(p->g_lm, qb200tc::EPI_F32, g, st)) return rc;
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(20, "batched step launch: %s", cudaGetErrorString(e));
+  return 0;
+}
+
+int qwen_b200_batched_step_prefix(void *handle, int rows, const int *seq_ids, const int *positions,
+                                  const int *tokens_in, int *tokens_out, float *logits, long long ld,
+                                  float *norm_out, const int *plan_header, void *plan, void *workspace,
+                                  long long workspace_bytes, int max_length, float attn_scale, void *stream) {
+  qb200_clear_error();
+  Plan *p = static_cast<Plan *>(handle);
+  if ((tokens_out == nullptr) == (logits == nullptr)) return fail(13, "give tokens_out or logits, one of the two");
+  const void *out = tokens_out != nullptr ? static_cast<const void *>(tokens_out) : logits;
+  if (int rc = check_step(p, rows, seq_ids, positions, tokens_in, out, 0)) return rc;
+  if (p->kg.page_table == nullptr) return fail(10, "a shared prefix needs paged pools");
+  if (max_length < 1 || max_length > p->max_seq)
+    return fail(11, "max_length=%d outside the KV cache (max_seq=%d)", max_length, p->max_seq);
+  if (logits != nullptr && (ld < VOCAB || (ld & 3) != 0 || !al16(logits)))
+    return fail(14, "logits: ld=%lld must be >= %d and a multiple of 4, pointer 16-byte aligned", ld, VOCAB);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const Workspace &w = p->ws;
+  QwenPrefixAttention a{};
+  a.q = w.qrot;
+  a.out = w.attn;
+  a.k_pool = p->k_pool;
+  a.v_pool = p->v_pool;
+  a.page_table = p->kg.page_table;
+  a.seq_ids = seq_ids;
+  a.lengths = positions;
+  a.length_bias = 1;
+  a.plan_header = plan_header;
+  a.plan = plan;
+  a.workspace = workspace;
+  a.workspace_bytes = workspace_bytes;
+  a.q_row_stride = a.out_row_stride = QS;
+  a.q_head_stride = a.out_head_stride = HD;
+  a.token_stride = HD;
+  a.head_stride = static_cast<long long>(PAGE) * HD;
+  a.page_stride = static_cast<long long>(p->num_layers) * NKV * PAGE * HD;
+  a.table_pitch = p->kg.max_pages;
+  a.rows = rows;
+  a.heads = NQ;
+  a.kv_heads = NKV;
+  a.dim = HD;
+  a.num_pages = p->kg.num_pages;
+  a.page_tokens = PAGE;
+  a.num_seqs = p->num_seqs;
+  a.max_pages = p->kg.max_pages;
+  a.max_length = max_length;
+  a.scale = attn_scale;
+  // Checked before the first launch, not at the first layer's attention.
+  if (int rc = qb200_prefix_check(&a)) return rc;
+  if (int rc = step_layers(p, rows, seq_ids, positions, tokens_in, norm_out, 0, attn_scale, st, &a)) return rc;
+  GemmArgs g{};
+  g.M = rows;
+  g.err = w.err;
+  g.pdl = 1;
+  if (logits != nullptr) {
+    g.out = logits;
+    g.ldo = static_cast<int>(ld);
+    if (int rc = qb200_gemm_run(p->g_lm, qb200tc::EPI_F32, g, st)) return rc;
+  } else {
+    g.ldo = 1;
+    g.part_val = w.arg_val;
+    g.part_idx = w.arg_idx;
+    if (int rc = qb200_gemm_run_argmax(p->g_lm, g, st)) return rc;
+    if (int rc = qb200_argmax_reduce(w.arg_val, w.arg_idx, p->lm_tiles, rows, tokens_out, st, true)) return rc;
+  }
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return fail(20, "batched step launch: %s", cudaGetErrorString(e));
   return 0;

@@ -13,3 +13,7 @@ int qb200_set_error(int code, const char *msg);
 // Returns 0 or an error code with the message recorded (ops.cu).
 int qb200_encode_f16_2d(CUtensorMap *m, const void *ptr, long long inner, long long outer,
                         long long pitch, int box_inner, int box_outer, int swizzle128);
+
+// The argument checks of qwen_b200_prefix_attention (prefix_attn.cu).
+struct QwenPrefixAttention;
+int qb200_prefix_check(const QwenPrefixAttention *a);

@@ -1281,6 +1281,39 @@ int launch(const QwenPrefixAttention &u, const Args &a, const CUtensorMap &mk, c
 
 }  // namespace
 
+int qb200_prefix_check(const QwenPrefixAttention *u) {
+  if (u == nullptr) return fail(13, "null argument");
+  const int *h = u->plan_header;
+  if (!plan_ok(h)) return fail(13, "plan: not the words of qwen_b200_prefix_plan");
+  if (u->rows != h[PW_ROWS] || u->heads != h[PW_HEADS] || u->kv_heads != h[PW_KV_HEADS])
+    return fail(10, "the plan is for %d rows, %d / %d heads; called with %d rows, %d / %d heads", h[PW_ROWS],
+                h[PW_HEADS], h[PW_KV_HEADS], u->rows, u->heads, u->kv_heads);
+  if (u->dim != 64 && u->dim != 128) return fail(10, "dim=%d: 64 or 128", u->dim);
+  if (u->dtype != 0 && u->dtype != 1) return fail(10, "dtype=%d: 0 (fp16) or 1 (bf16)", u->dtype);
+  if (u->num_pages < 1 || u->page_tokens < 16 || u->page_tokens % 16 != 0)
+    return fail(10, "num_pages=%d page_tokens=%d: pages of a multiple of 16 tokens", u->num_pages, u->page_tokens);
+  if (u->num_seqs < 1 || u->max_pages < 1 || u->table_pitch < u->max_pages)
+    return fail(10, "page table: num_seqs=%d max_pages=%d pitch=%lld", u->num_seqs, u->max_pages, u->table_pitch);
+  if (static_cast<long long>(u->max_pages) * u->page_tokens > 0x7fff0000ll)
+    return fail(10, "page table rows of over 2^31 tokens");
+  if (!(u->scale > 0.f) || u->scale > 1e30f) return fail(10, "scale=%g must be positive", static_cast<double>(u->scale));
+  if (u->max_length < 0) return fail(10, "max_length=%d", u->max_length);
+  const void *need[] = {u->q, u->out, u->k_pool, u->v_pool, u->page_table, u->seq_ids, u->lengths, u->plan, u->workspace};
+  for (const void *p : need)
+    if (p == nullptr) return fail(13, "null pointer argument");
+  for (const void *p : {u->q, static_cast<const void *>(u->out), u->k_pool, u->v_pool, static_cast<const void *>(u->plan),
+                        static_cast<const void *>(u->workspace)})
+    if (!al16(p)) return fail(14, "q, out, pools, plan and workspace must be 16-byte aligned");
+  for (long long s : {u->q_row_stride, u->q_head_stride, u->out_row_stride, u->out_head_stride, u->page_stride,
+                      u->head_stride, u->token_stride})
+    if (s < 0 || s % 8 != 0 || s > (1ll << 38)) return fail(14, "stride of %lld elements: must be a multiple of 8", s);
+  if (u->token_stride < u->dim || (u->kv_heads > 1 && u->head_stride < u->dim) || (u->num_pages > 1 && u->page_stride < u->dim))
+    return fail(14, "pool strides overlap");
+  const long long ws = qwen_b200_prefix_workspace(h, u->dim, u->max_length);
+  if (u->workspace_bytes < ws) return fail(15, "workspace of %lld bytes, need %lld", u->workspace_bytes, ws);
+  return 0;
+}
+
 extern "C" {
 
 int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_lens, int heads, int kv_heads, int ctas,
@@ -1423,35 +1456,8 @@ long long qwen_b200_prefix_workspace(const int *h, int dim, int max_length) {
 
 int qwen_b200_prefix_attention(const QwenPrefixAttention *u, void *stream) {
   qb200_clear_error();
-  if (u == nullptr) return fail(13, "null argument");
+  if (int rc = qb200_prefix_check(u)) return rc;
   const int *h = u->plan_header;
-  if (!plan_ok(h)) return fail(13, "plan: not the words of qwen_b200_prefix_plan");
-  if (u->rows != h[PW_ROWS] || u->heads != h[PW_HEADS] || u->kv_heads != h[PW_KV_HEADS])
-    return fail(10, "the plan is for %d rows, %d / %d heads; called with %d rows, %d / %d heads", h[PW_ROWS],
-                h[PW_HEADS], h[PW_KV_HEADS], u->rows, u->heads, u->kv_heads);
-  if (u->dim != 64 && u->dim != 128) return fail(10, "dim=%d: 64 or 128", u->dim);
-  if (u->dtype != 0 && u->dtype != 1) return fail(10, "dtype=%d: 0 (fp16) or 1 (bf16)", u->dtype);
-  if (u->num_pages < 1 || u->page_tokens < 16 || u->page_tokens % 16 != 0)
-    return fail(10, "num_pages=%d page_tokens=%d: pages of a multiple of 16 tokens", u->num_pages, u->page_tokens);
-  if (u->num_seqs < 1 || u->max_pages < 1 || u->table_pitch < u->max_pages)
-    return fail(10, "page table: num_seqs=%d max_pages=%d pitch=%lld", u->num_seqs, u->max_pages, u->table_pitch);
-  if (static_cast<long long>(u->max_pages) * u->page_tokens > 0x7fff0000ll)
-    return fail(10, "page table rows of over 2^31 tokens");
-  if (!(u->scale > 0.f) || u->scale > 1e30f) return fail(10, "scale=%g must be positive", static_cast<double>(u->scale));
-  if (u->max_length < 0) return fail(10, "max_length=%d", u->max_length);
-  const void *need[] = {u->q, u->out, u->k_pool, u->v_pool, u->page_table, u->seq_ids, u->lengths, u->plan, u->workspace};
-  for (const void *p : need)
-    if (p == nullptr) return fail(13, "null pointer argument");
-  for (const void *p : {u->q, static_cast<const void *>(u->out), u->k_pool, u->v_pool, static_cast<const void *>(u->plan),
-                        static_cast<const void *>(u->workspace)})
-    if (!al16(p)) return fail(14, "q, out, pools, plan and workspace must be 16-byte aligned");
-  for (long long s : {u->q_row_stride, u->q_head_stride, u->out_row_stride, u->out_head_stride, u->page_stride,
-                      u->head_stride, u->token_stride})
-    if (s < 0 || s % 8 != 0 || s > (1ll << 38)) return fail(14, "stride of %lld elements: must be a multiple of 8", s);
-  if (u->token_stride < u->dim || (u->kv_heads > 1 && u->head_stride < u->dim) || (u->num_pages > 1 && u->page_stride < u->dim))
-    return fail(14, "pool strides overlap");
-  const long long ws = qwen_b200_prefix_workspace(h, u->dim, u->max_length);
-  if (u->workspace_bytes < ws) return fail(15, "workspace of %lld bytes, need %lld", u->workspace_bytes, ws);
   Args a{};
   a.q = u->q;
   a.out = u->out;
