@@ -84,7 +84,6 @@ constexpr int THREADS = 384; // 3 warpgroups: TMA and MMA warps (two idle), two 
 // no L1 to spill to (a spilled value comes back from L2).
 constexpr int REGS_WORK = 88, REGS_SOFT = 208;
 static_assert(REGS_WORK + 2 * REGS_SOFT <= 3 * 168, "the split fits what the block was launched with");
-constexpr int OWN_THREADS = 128;
 
 struct Args {
   const void *q;
@@ -104,7 +103,7 @@ struct Args {
   unsigned long long *err;
   int rows, heads, kv_heads, ratio;
   int num_pages, page_tokens, box, box_shift, num_seqs, max_pages;
-  int length_bias, own_splits;
+  int length_bias, own_splits, own_per, run_rows;
   int after_prefix;    // the own kernel follows a prefix kernel of the same call
   float scale_log2;
 };
@@ -839,13 +838,16 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-__device__ __forceinline__ uint4 ld_kv(const void *p, bool on) {
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (on)
-    asm volatile("ld.global.L1::no_allocate.L2::128B.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p));
-  return v;
+// 16 bytes to shared memory without a register, zeros when `on` is false (the
+// source is then not read).
+__device__ __forceinline__ void copy16(void *dst, const void *src, bool on) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(on ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
@@ -876,6 +878,7 @@ struct PrefixParts {
   int first, count, ql;  // first stream slot (one slot holds two), slots, query within the stream
 };
 __device__ __forceinline__ PrefixParts prefix_parts(const Args &a, const RowPlan &rp, int head) {
+  // (the plan is constant: this may run before the prefix kernel is done)
   const int kvh = head / a.ratio, qi = rp.query + head % a.ratio;
   const int tile = rp.tile0 + (qi / (2 * QT)) * a.kv_heads + kvh;
   const int s0 = a.tile_slot[tile], s1 = a.tile_slot[tile + 1];
@@ -889,14 +892,14 @@ __device__ __forceinline__ PrefixParts prefix_parts(const Args &a, const RowPlan
 }
 
 // Joins partials k0, k0 + dk, ... of a query's prefix, dims 4 d4 .. 4 d4 + 3;
-// four are requested before the first is used.
-template <int D>
+// U are requested before the first is used.
+template <int D, int U>
 __device__ __forceinline__ void join_prefix(const Args &a, const PrefixParts &p, int d4, int k0, int dk, Joined &j) {
-  for (int k = k0; k < p.count; k += 4 * dk) {
-    float m[4], l[4];
-    float4 v[4];
+  for (int k = k0; k < p.count; k += U * dk) {
+    float m[U], l[U];
+    float4 v[U];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < U; ++u) {
       m[u] = -INFINITY;
       l[u] = 0.f;
       v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -908,7 +911,7 @@ __device__ __forceinline__ void join_prefix(const Args &a, const PrefixParts &p,
       }
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) j.add(m[u], l[u], v[u]);
+    for (int u = 0; u < U; ++u) j.add(m[u], l[u], v[u]);
   }
 }
 
@@ -932,49 +935,85 @@ __device__ __forceinline__ void put_result(const Args &a, int row, int head, int
   if (d4 == 0 && a.lse != nullptr) a.lse[static_cast<size_t>(row) * a.heads + head] = lse;
 }
 
-// grid (splits, kv heads x head tiles of 8, rows), 4 warps.  The CTA takes
-// positions [start + split * per, ...) of its row, its warps blocks of 16
-// tokens in turn, each with its own online softmax; the four join through
-// shared memory.  Per block, with tokens on the M side of the products:
-//   S^T[16 tokens, 8 heads] = K Q^T, O^T[D dims, 8 heads] += V^T P^T.
-// K fragments come straight from global memory: lane (g, c) = (lane / 4,
-// lane % 4) reads 16 bytes at dims 32 i + 8 c of tokens g and g + 8, and the
-// contraction runs over the dims in that order on both sides.  V likewise:
-// the lane reads tokens 2c, 2c+1, 2c+8, 2c+9 at dims 64 i + 8 g and pairs
-// tokens with byte permutes, which is the transposed operand.  With one split the CTA also joins the prefix's partial results
-// and writes the output; else it leaves partial results to the join kernel.
-template <typename T, int D>
-__global__ void __launch_bounds__(OWN_THREADS, 5) own_kernel(const Args a) {
+// grid (splits, kv heads x head tiles of 8, rows), 4 warps.  A CTA takes a run
+// of rows of one sequence (draft tokens, a piece of a prompt; one row in plain
+// decoding) within a block of run_rows rows, as many as fit 8 columns of
+// (row, head): they read the same keys, and the products are 8 columns wide
+// anyway.  It takes positions [start + split * own_per, ...) of the sequence,
+// its warps blocks of BT tokens in turn, each with its own online softmax; the
+// four join through shared memory.  Per 16 tokens, with tokens on the M side:
+//   S^T[16 tokens, 8 columns] = K Q^T, O^T[D dims, 8 columns] += V^T P^T.
+// What bounds it are the bytes of K and V and the latency of getting at them
+// (length, page, tokens: three round trips), so the copies go to shared memory
+// without registers (16 rows of K and of V per warp at D = 128) and six CTAs
+// fit an SM; a block's K is replaced as soon as it has been multiplied, its V
+// likewise.  Lane (g, c) = (lane / 4, lane % 4) reads K at dims 32 i + 8 c of
+// tokens g and g + 8 (the contraction runs over the dims in that order on both
+// sides) and V at dims 64 i + 8 g of tokens 2c, 2c+1, 2c+8, 2c+9, pairing tokens
+// with byte permutes, which is the transposed operand; the 16-byte chunks of a
+// row are exchanged by its number so that neither read has bank conflicts.
+// With one split the CTA also joins the prefix's partial results and writes the
+// output; else it leaves partial results to the join kernel.
+template <typename T, int D, int W>
+__global__ void __launch_bounds__(32 * W, W == 1 ? 11 : 3) own_kernel(const Args a) {
   // Behind a prefix kernel of the same call nothing that this part reads is
   // new: the prefix kernel's CTAs have all passed their own wait for whatever
   // came before.  Its results are waited for where they are read, below.
   if (!a.after_prefix) qb200::griddep_wait();
   qb200::griddep_launch_dependents();
-  constexpr int KI = D / 32;  // 16-byte chunks of a token per lane (scores)
-  constexpr int VI = D / 64;  // 16-byte chunks of a token per lane (values)
-  __shared__ float s_m[4][8], s_l[4][8];
-  __shared__ __align__(16) float s_o[4][8][D + 4];
-  constexpr int QP = D + 32;  // pitch of a query row: the fragment reads of two rows take all banks
+  constexpr int KI = D / 32;       // 16-byte chunks of a token per lane (scores)
+  constexpr int VI = D / 64;       // 16-byte chunks of a token per lane (values)
+  constexpr int NB = 128 / D;      // 16-token steps of a block
+  constexpr int BT = 16 * NB;      // tokens of a warp's block: 4 KB of K and of V
+  constexpr int CPR = D / 8;       // 16-byte chunks of a token
+  constexpr int RPI = 32 / CPR;    // tokens that a warp copies at a time
+  constexpr int QP = D + 32;       // pitch of a query row: the fragment reads of two rows take all banks
+  constexpr int OP = D + 4;        // pitch of an output column
+  constexpr int R = W == 1 ? 2 : 1;  // blocks of a warp in shared memory
+  constexpr int NT = 32 * W;
+  __shared__ __align__(128) T s_kv[W][R][2][BT * D];
   __shared__ __align__(16) T s_q[8 * QP];
-  const int split = blockIdx.x, row = blockIdx.z;
+  __shared__ float s_m[W][8], s_l[W][8];
+  static_assert(8 * OP * 4 <= sizeof(s_kv) / W, "a warp's output columns fit its copies' place");
+  const int split = blockIdx.x;
   const int htiles = (a.ratio + 7) >> 3;
   const int kvh = blockIdx.y / htiles, h0 = (blockIdx.y % htiles) * 8;
   const int nh = min(8, a.ratio - h0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  int seq;
-  const int len = row_length(a, row, &seq);
-  const RowPlan rp = a.row_plan[row];
-  if (len < 0 && threadIdx.x == 0) record(a.err, 3);
-  const int start = len >= rp.prefix ? rp.prefix : 0;
-  const int count = max(0, len - start);
-  // Tokens of one split: a multiple of 64 that covers the row.
-  const int per = ((count + a.own_splits - 1) / a.own_splits + 63) / 64 * 64;
-  const int lo = start + split * per, hi = min(len, lo + per);
-  const bool fused = a.own_splits == 1;
 
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // heads 2c, 2c + 1
+  // Lane i looks at row i of the block of rows: which of them run together
+  // (same sequence, same start of the own part), and whether this row leads.
+  const int row = blockIdx.z, me = row % a.run_rows;
+  int seq = -1, len = -1, start = 0;
+  if (lane < a.run_rows && row - me + lane < a.rows) {
+    len = row_length(a, row - me + lane, &seq);
+    const int prefix = a.row_plan[row - me + lane].prefix;
+    start = len >= prefix ? prefix : 0;
+    if (len < 0) seq = -2 - lane;  // runs with no other row
+  }
+  const int my_seq = __shfl_sync(0xffffffffu, seq, me), my_start = __shfl_sync(0xffffffffu, start, me);
+  const uint32_t same = __ballot_sync(0xffffffffu, lane < a.run_rows && seq == my_seq && start == my_start);
+  if (me > 0 && ((same >> (me - 1)) & 1u)) return;      // the row before takes this one along
+  const int nrun = __ffs(~(same >> me)) - 1;            // rows of the run
+  const int nc = nrun * nh;                             // columns: run_rows > 1 only when nh is all heads
+  len = __shfl_sync(0xffffffffu, len, min(me + lane, 31));  // lane i: row i of the run
+  const int max_len = __reduce_max_sync(0xffffffffu, lane < nrun ? len : -1);
+  const int min_len = __reduce_min_sync(0xffffffffu, lane < nrun ? len : 0x7fffffff);
+  if (max_len < 0 && threadIdx.x == 0) record(a.err, 3);
+  const int lo = my_start + split * a.own_per;
+  const int hi = split + 1 == a.own_splits ? max_len : min(max_len, lo + a.own_per);
+  const bool fused = a.own_splits == 1;
+  // Lengths of this lane's columns 2c, 2c + 1 (0: no such column).
+  int clen[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int v = __shfl_sync(0xffffffffu, len, min((2 * c + h) / nh, 31));
+    clen[h] = 2 * c + h < nc ? v : 0;
+  }
+
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   // O^T tile (i, e): rows g = dims 64 i + 8 g + e, rows g + 8 = those + 4;
-  // columns = heads 2c, 2c + 1.
+  // columns 2c, 2c + 1.
   float o[VI][4][4];
 #pragma unroll
   for (int i = 0; i < VI; ++i)
@@ -982,14 +1021,15 @@ __global__ void __launch_bounds__(OWN_THREADS, 5) own_kernel(const Args a) {
     for (int e = 0; e < 4; ++e)
 #pragma unroll
       for (int x = 0; x < 4; ++x) o[i][e][x] = 0.f;
-  bool seen = false;
-  const int b0 = lo + 16 * warp;
-  const int *trow = a.page_table + (len < 0 ? 0 : seq * a.table_pitch);
-  // Element offset of block j of this warp in the pools; -1: its page is not
-  // mapped.  The pages of 32 blocks are looked up at once.
+  bool seen[2] = {false, false};
+  const int b0 = lo + BT * warp;
+  const int *trow = a.page_table + (my_seq < 0 ? 0 : my_seq * a.table_pitch);
+  const int nb = b0 < hi ? (hi - b0 + W * BT - 1) / (W * BT) : 0;
+  // Element offset of the warp's j-th 16 tokens in the pools; -1: their page
+  // is not mapped.  The pages of 32 steps are looked up at once.
   long long where = -1;
   const auto lookup = [&](int j) {
-    const int b = b0 + 64 * (j + lane);
+    const int b = b0 + W * BT * ((j + lane) / NB) + 16 * ((j + lane) % NB);
     where = -1;
     if (b < hi) {
       const int pi = b / a.page_tokens, page = trow[pi];
@@ -1000,126 +1040,223 @@ __global__ void __launch_bounds__(OWN_THREADS, 5) own_kernel(const Args a) {
     }
   };
   lookup(0);
-  // Q^T, the B operand of the scores, waits in shared memory: n = head g, k =
-  // dims in the order of the K loads.
-  for (int x = threadIdx.x; x < D; x += OWN_THREADS) {
-    const int h = x / (D / 8), d = 8 * (x % (D / 8));
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (h < nh)
-      v = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + row * a.q_row + (kvh * a.ratio + h0 + h) * a.q_head + d);
-    *reinterpret_cast<uint4 *>(s_q + h * QP + d) = v;
+  uint32_t ready = 0;  // bit (step % 32): the page of a step that has been fetched is mapped
+  // Q^T, the B operand of the scores, on its way to shared memory: n = column,
+  // k = dims in the order of the K reads.
+  constexpr int QC = (8 * CPR + NT - 1) / NT;  // 16-byte chunks per thread
+  uint4 qv0[QC];
+#pragma unroll
+  for (int i = 0; i < QC; ++i) {
+    const int x = threadIdx.x + i * NT, col = x / CPR;
+    qv0[i] = make_uint4(0, 0, 0, 0);
+    if (col < nc)
+      qv0[i] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (row + col / nh) * a.q_row +
+                                                (kvh * a.ratio + h0 + col % nh) * a.q_head + 8 * (x % CPR));
+  }
+  // Copies block j of K or V (xk: the exchange of K's chunks, else V's), and
+  // closes the group of copies (an empty one behind the last block).
+  const auto fetch = [&](const void *pool, int j, bool xk) {
+    if (j >= nb) {
+      copy_commit();
+      return;
+    }
+    T *dst = s_kv[warp][j % R][xk ? 0 : 1];
+    if (xk && j > 0 && (j * NB & 31) == 0) lookup(j * NB);
+    const int ch = lane % CPR, t0 = lane / CPR;  // chunk; token within a step of RPI
+    const T *src = static_cast<const T *>(pool) + kvh * a.head_stride + 8 * ch;
+    const int left = hi - (b0 + W * BT * j);
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      const long long at = __shfl_sync(0xffffffffu, where, (j * NB + k) & 31);
+      const uint32_t bit = 1u << ((j * NB + k) & 31);
+      if (xk) ready = at >= 0 ? ready | bit : ready & ~bit;
+      const int n = at >= 0 ? left - 16 * k : 0;
+      const T *from = src + (at >= 0 ? at : 0) + t0 * a.token_stride;
+#pragma unroll
+      for (int i = 0; i < 16 / RPI; ++i) {
+        const int t = i * RPI + t0;
+        const int x = xk ? (t & 1) << 2 : ((t >> 1) & 3) << 1;
+        copy16(dst + (16 * k + t) * D + 8 * (ch ^ x), t < n ? from + i * RPI * a.token_stride : src, t < n);
+      }
+    }
+    copy_commit();
+  };
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    fetch(a.k_pool, j, true);
+    fetch(a.v_pool, j, false);
+  }
+#pragma unroll
+  for (int i = 0; i < QC; ++i) {
+    const int x = threadIdx.x + i * NT;
+    if (x < 8 * CPR) *reinterpret_cast<uint4 *>(s_q + (x / CPR) * QP + 8 * (x % CPR)) = qv0[i];
+  }
+  // Where the prefix's partial results of this thread's outputs lie.
+  constexpr int Q4 = D / 4;
+  PrefixParts parts{};
+  if (fused && my_start > 0 && static_cast<int>(threadIdx.x) < nc * Q4) {
+    const int col = threadIdx.x % nc;
+    parts = prefix_parts(a, a.row_plan[row + col / nh], kvh * a.ratio + h0 + col % nh);
   }
   __syncthreads();
-  if (b0 < hi) {
-    const T *kp = static_cast<const T *>(a.k_pool) + kvh * a.head_stride + g * a.token_stride + 8 * c;
-    const T *vp = static_cast<const T *>(a.v_pool) + kvh * a.head_stride + 2 * c * a.token_stride + 8 * g;
-    const int nb = (hi - b0 + 63) / 64;
-    uint4 kv[2][KI], vv[4][VI];
-    const auto load_k = [&](long long at, int n) {
+  for (int j = 0; j < nb; ++j) {
+    const int b = b0 + W * BT * j;
+    const T *sk = s_kv[warp][j % R][0], *sv = s_kv[warp][j % R][1];
+    // Visible steps of the block (its pages are mapped).
+    bool mapped[NB];
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
+    for (int k = 0; k < NB; ++k) mapped[k] = (ready >> ((j * NB + k) & 31)) & 1u;
+    copy_wait<2 * R - 1>();
+    __syncwarp();
+    float s[NB][4];  // (token g, columns 2c, 2c+1), (token g + 8, ...)
 #pragma unroll
-        for (int i = 0; i < KI; ++i) kv[x][i] = ld_kv(kp + at + 8 * x * a.token_stride + 32 * i, g + 8 * x < n);
-    };
-    const auto load_v = [&](long long at, int n) {
+    for (int k = 0; k < NB; ++k) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int t = (x & 1) + 8 * (x >> 1);
-#pragma unroll
-        for (int i = 0; i < VI; ++i) vv[x][i] = ld_kv(vp + at + t * a.token_stride + 64 * i, 2 * c + t < n);
-      }
-    };
-    // Tokens of block j that count: none behind the row or of an unmapped page.
-    const auto tokens = [&](int j, long long at) { return at < 0 ? 0 : min(16, hi - (b0 + 64 * j)); };
-    for (int j = 0; j < nb; ++j) {
-      if (j > 0 && (j & 31) == 0) lookup(j);
-      const long long at = __shfl_sync(0xffffffffu, where, j & 31);
-      const int n = tokens(j, at);
-      load_k(at, n);
-      load_v(at, n);
-      float s[4] = {0.f, 0.f, 0.f, 0.f};  // (token g, heads 2c, 2c+1), (token g + 8, ...)
+      for (int x = 0; x < 4; ++x) s[k][x] = 0.f;
 #pragma unroll
       for (int i = 0; i < KI; ++i) {
+        const int t = 16 * k + g, ch = (4 * i + c) ^ ((g & 1) << 2);
+        const uint4 k0 = *reinterpret_cast<const uint4 *>(sk + t * D + 8 * ch);
+        const uint4 k1 = *reinterpret_cast<const uint4 *>(sk + (t + 8) * D + 8 * ch);
         const uint4 qv = *reinterpret_cast<const uint4 *>(s_q + g * QP + 32 * i + 8 * c);
-        mma16816<T>(s, kv[0][i].x, kv[1][i].x, kv[0][i].y, kv[1][i].y, qv.x, qv.y);
-        mma16816<T>(s, kv[0][i].z, kv[1][i].z, kv[0][i].w, kv[1][i].w, qv.z, qv.w);
+        mma16816<T>(s[k], k0.x, k1.x, k0.y, k1.y, qv.x, qv.y);
+        mma16816<T>(s[k], k0.z, k1.z, k0.w, k1.w, qv.z, qv.w);
       }
-      float p[4];
+    }
+    __syncwarp();
+    fetch(a.k_pool, j + R, true);
+    uint32_t pb[NB][2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float s0 = g < n ? s[h] * a.scale_log2 : -INFINITY, s1 = g + 8 < n ? s[2 + h] * a.scale_log2 : -INFINITY;
-        float mx = fmaxf(s0, s1);
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        const float mn = fmaxf(m[h], mx);
-        const float mu = mn == -INFINITY ? 0.f : mn;
-        const float f = ex2_approx(m[h] - mu);
-        p[h] = ex2_approx(s0 - mu);
-        p[2 + h] = ex2_approx(s1 - mu);
-        l[h] = l[h] * f + (p[h] + p[2 + h]);
-        m[h] = mn;
+    for (int h = 0; h < 2; ++h) {
+      float mx = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < VI; ++i)
+      for (int k = 0; k < NB; ++k)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            o[i][e][h] *= f;
-            o[i][e][2 + h] *= f;
-          }
+        for (int x = 0; x < 2; ++x) {
+          float &v = s[k][2 * x + h];
+          v = mapped[k] && b + 16 * k + g + 8 * x < min(clen[h], hi) ? v * a.scale_log2 : -INFINITY;
+          mx = fmaxf(mx, v);
+          seen[h] = seen[h] || (mapped[k] && b + 16 * k < min(clen[h], hi));
+        }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+      const float mn = fmaxf(m[h], mx);
+      const float mu = mn == -INFINITY ? 0.f : mn;
+      const float f = ex2_approx(m[h] - mu);
+      l[h] *= f;
+#pragma unroll
+      for (int k = 0; k < NB; ++k) {
+        s[k][h] = ex2_approx(s[k][h] - mu);
+        s[k][2 + h] = ex2_approx(s[k][2 + h] - mu);
+        l[h] += s[k][h] + s[k][2 + h];
       }
-      seen = seen || n > 0;
-      // P^T as the B operand (n = head g, k = tokens 2c, 2c+1 / 2c+8, 2c+9).
-      // The weights are rounded to the input type for the product (half a
-      // step each, as the values they weigh); their sum is not.
-      const uint32_t pb0 = transpose8x8(Type<T>::pack(p[0], p[1]));
-      const uint32_t pb1 = transpose8x8(Type<T>::pack(p[2], p[3]));
+      m[h] = mn;
 #pragma unroll
       for (int i = 0; i < VI; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          // A rows g: dim 8 g + e; rows g + 8: dim 8 g + e + 4.
-          const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
-          const int w0 = e >> 1, w1 = 2 + (e >> 1);
-          const uint32_t a0 = __byte_perm(word(vv[0][i], w0), word(vv[1][i], w0), sel);
-          const uint32_t a1 = __byte_perm(word(vv[0][i], w1), word(vv[1][i], w1), sel);
-          const uint32_t a2 = __byte_perm(word(vv[2][i], w0), word(vv[3][i], w0), sel);
-          const uint32_t a3 = __byte_perm(word(vv[2][i], w1), word(vv[3][i], w1), sel);
-          mma16816<T>(o[i][e], a0, a1, a2, a3, pb0, pb1);
+          o[i][e][h] *= f;
+          o[i][e][2 + h] *= f;
         }
     }
+    // P^T as the B operand (n = column g, k = tokens 2c, 2c+1 / 2c+8, 2c+9).
+    // The weights are rounded to the input type for the product (half a step
+    // each, as the values they weigh); their sum is not.
+#pragma unroll
+    for (int k = 0; k < NB; ++k) {
+      pb[k][0] = transpose8x8(Type<T>::pack(s[k][0], s[k][1]));
+      pb[k][1] = transpose8x8(Type<T>::pack(s[k][2], s[k][3]));
+    }
+    copy_wait<2 * R - 1>();
+    __syncwarp();
+    // o += V^T P^T; with `limit`, V counts as zero from that position on and
+    // only the columns of row `only` of the run are added: a value that one
+    // row sees and another does not may be anything (0 x NaN).
+    const auto values = [&](int limit, int only) {
+#pragma unroll
+      for (int k = 0; k < NB; ++k)
+#pragma unroll
+        for (int i = 0; i < VI; ++i) {
+          uint4 vv[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int t = 16 * k + 2 * c + (x & 1) + 8 * (x >> 1);
+            vv[x] = *reinterpret_cast<const uint4 *>(sv + t * D + 8 * ((8 * i + g) ^ (c << 1)));
+            if (only >= 0 && b + t >= limit) vv[x] = make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            // A rows g: dim 8 g + e; rows g + 8: dim 8 g + e + 4.
+            const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
+            const int w0 = e >> 1, w1 = 2 + (e >> 1);
+            const uint32_t a0 = __byte_perm(word(vv[0], w0), word(vv[1], w0), sel);
+            const uint32_t a1 = __byte_perm(word(vv[0], w1), word(vv[1], w1), sel);
+            const uint32_t a2 = __byte_perm(word(vv[2], w0), word(vv[3], w0), sel);
+            const uint32_t a3 = __byte_perm(word(vv[2], w1), word(vv[3], w1), sel);
+            if (only < 0) {
+              mma16816<T>(o[i][e], a0, a1, a2, a3, pb[k][0], pb[k][1]);
+            } else {
+              float d[4] = {0.f, 0.f, 0.f, 0.f};
+              mma16816<T>(d, a0, a1, a2, a3, pb[k][0], pb[k][1]);
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                if ((2 * c + h) / nh == only) {
+                  o[i][e][h] += d[h];
+                  o[i][e][2 + h] += d[2 + h];
+                }
+            }
+          }
+        }
+    };
+    if (b + BT <= min_len || nrun == 1) {
+      values(0, -1);
+    } else {
+#pragma unroll 1
+      for (int r = 0; r < nrun; ++r) values(__shfl_sync(0xffffffffu, len, r), r);
+    }
+    __syncwarp();
+    fetch(a.v_pool, j + R, false);
   }
+  copy_wait<0>();
+  __syncwarp();
+  float *so = reinterpret_cast<float *>(s_kv[warp]);  // [column][OP]
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 4);
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 8);
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 16);
     // Seen tokens whose scores are all -inf: as in the prefix kernel.
-    if (m[h] == -INFINITY) l[h] = seen ? 1.f : 0.f;
+    if (m[h] == -INFINITY) l[h] = seen[h] ? 1.f : 0.f;
     if (g == 0) {
       s_m[warp][2 * c + h] = m[h];
       s_l[warp][2 * c + h] = l[h];
     }
 #pragma unroll
     for (int i = 0; i < VI; ++i) {
-      float *d = &s_o[warp][2 * c + h][64 * i + 8 * g];
+      float *d = so + (2 * c + h) * OP + 64 * i + 8 * g;
       *reinterpret_cast<float4 *>(d) = make_float4(o[i][0][h], o[i][1][h], o[i][2][h], o[i][3][h]);
       *reinterpret_cast<float4 *>(d + 4) = make_float4(o[i][0][2 + h], o[i][1][2 + h], o[i][2][2 + h], o[i][3][2 + h]);
     }
   }
   __syncthreads();
   if (a.after_prefix) qb200::griddep_wait();
-  constexpr int Q4 = D / 4;
-  for (int x = threadIdx.x; x < nh * Q4; x += OWN_THREADS) {
-    // Neighbouring threads take the heads of one row: their prefix partials are adjacent.
-    const int h = x % nh, d4 = x / nh, head = kvh * a.ratio + h0 + h;
+  for (int x = threadIdx.x; x < nc * Q4; x += NT) {
+    // Neighbouring threads take the columns: their prefix partials are adjacent.
+    const int col = x % nc, d4 = x / nc, r = row + col / nh, head = kvh * a.ratio + h0 + col % nh;
     Joined j;
-    if (fused && rp.prefix > 0 && len >= rp.prefix) join_prefix<D>(a, prefix_parts(a, rp, head), d4, 0, 1, j);
+    if (fused && my_start > 0) {
+      if (x >= NT) parts = prefix_parts(a, a.row_plan[r], head);
+      join_prefix<D, W == 1 ? 8 : 4>(a, parts, d4, 0, 1, j);
+    }
 #pragma unroll
-    for (int w = 0; w < 4; ++w) j.add(s_m[w][h], s_l[w][h], *reinterpret_cast<const float4 *>(&s_o[w][h][4 * d4]));
+    for (int w = 0; w < W; ++w)
+      j.add(s_m[w][col], s_l[w][col],
+            *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(s_kv[w]) + col * OP + 4 * d4));
     if (fused) {
-      put_result<T>(a, row, head, d4, j);
+      put_result<T>(a, r, head, d4, j);
     } else {
-      float *part = a.own + ((static_cast<size_t>(row) * a.heads + head) * a.own_splits + split) * (D + 4);
+      float *part = a.own + ((static_cast<size_t>(r) * a.heads + head) * a.own_splits + split) * (D + 4);
       *reinterpret_cast<float4 *>(part + 4 * d4) = j.acc;
       if (d4 == 0) {
         part[D] = j.m;
@@ -1145,11 +1282,10 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args a) {
   const int len = row_length(a, row, &seq);
   const RowPlan rp = a.row_plan[row];
   Joined j;
-  if (rp.prefix > 0 && len >= rp.prefix) join_prefix<D>(a, prefix_parts(a, rp, head), d4, grp, NG, j);
+  if (rp.prefix > 0 && len >= rp.prefix) join_prefix<D, 8>(a, prefix_parts(a, rp, head), d4, grp, NG, j);
   if (len > 0) {
     const int count = len - (len >= rp.prefix ? rp.prefix : 0);
-    const int per = ((count + a.own_splits - 1) / a.own_splits + 63) / 64 * 64;
-    const int ns = count > 0 ? (count + per - 1) / per : 0;
+    const int ns = min(a.own_splits, (count + a.own_per - 1) / a.own_per);
     const float *own = a.own + (static_cast<size_t>(row) * a.heads + head) * a.own_splits * (D + 4);
     for (int s = grp; s < ns; s += NG) {
       const float *p = own + static_cast<size_t>(s) * (D + 4);
@@ -1204,9 +1340,13 @@ int own_splits(int rows, int kv_heads, int ratio, int own_tokens) {
   return s < 1 ? 1 : static_cast<int>(s);
 }
 
+int own_tokens(const int *h, int max_length) { return max_length > h[PW_MIN_PREFIX] ? max_length - h[PW_MIN_PREFIX] : 1; }
+
+// Tokens of one split (the last one takes whatever is left of a row).
+int own_part(int own, int splits) { return ((own + splits - 1) / splits + 127) / 128 * 128; }
+
 int plan_splits(const int *h, int max_length) {
-  const int own = max_length - h[PW_MIN_PREFIX];
-  return own_splits(h[PW_ROWS], h[PW_KV_HEADS], h[PW_HEADS] / h[PW_KV_HEADS], own < 1 ? 1 : own);
+  return own_splits(h[PW_ROWS], h[PW_KV_HEADS], h[PW_HEADS] / h[PW_KV_HEADS], own_tokens(h, max_length));
 }
 
 long long up256(long long b) { return (b + 255) / 256 * 256; }
@@ -1249,6 +1389,11 @@ int encode_pool(CUtensorMap *m, const QwenPrefixAttention &a, const void *pool, 
   return 0;
 }
 
+// Warps of an own CTA.
+int own_warps(const Args &a) {
+  return static_cast<long long>(a.rows) * a.kv_heads * ((a.ratio + 7) / 8) * a.own_splits >= 1480 ? 1 : 4;
+}
+
 template <typename T, int D>
 int launch(const QwenPrefixAttention &u, const Args &a, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t st) {
   const int *h = u.plan_header;
@@ -1270,8 +1415,9 @@ int launch(const QwenPrefixAttention &u, const Args &a, const CUtensorMap &mk, c
                                        mk, mv, a);
     if (e != cudaSuccess) return fail(20, "prefix attention launch: %s", cudaGetErrorString(e));
   }
-  cudaError_t e = qb200_launch(own_kernel<T, D>, dim3(a.own_splits, a.kv_heads * ((a.ratio + 7) / 8), a.rows),
-                               dim3(OWN_THREADS), 0, st, true, a);
+  const dim3 grid(a.own_splits, a.kv_heads * ((a.ratio + 7) / 8), a.rows);
+  cudaError_t e = own_warps(a) == 1 ? qb200_launch(own_kernel<T, D, 1>, grid, dim3(32), 0, st, true, a)
+                                    : qb200_launch(own_kernel<T, D, 4>, grid, dim3(128), 0, st, true, a);
   if (e != cudaSuccess) return fail(20, "own attention launch: %s", cudaGetErrorString(e));
   if (a.own_splits == 1) return 0;  // the own kernel has joined both parts
   e = qb200_launch(join_kernel<T, D>, dim3(a.heads, a.rows), dim3(JOIN_THREADS), 0, st, true, a);
@@ -1493,6 +1639,8 @@ int qwen_b200_prefix_attention(const QwenPrefixAttention *u, void *stream) {
   a.max_pages = u->max_pages;
   a.length_bias = u->length_bias;
   a.own_splits = plan_splits(h, u->max_length);
+  a.own_per = own_part(own_tokens(h, u->max_length), a.own_splits);
+  a.run_rows = a.ratio >= 8 ? 1 : 8 / a.ratio;
   a.after_prefix = h[PW_SEGS] > 0;
   a.scale_log2 = u->scale * 1.4426950408889634f;
   a.box = u->page_tokens % 128 == 0 ? 128 : u->page_tokens % 64 == 0 ? 64 : u->page_tokens % 32 == 0 ? 32 : 16;
