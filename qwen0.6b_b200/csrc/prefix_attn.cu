@@ -849,7 +849,21 @@ template <int N>
 __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ uint32_t word(const uint4 &v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+// Four 8 x 8 matrices of 16-bit values whose rows are the 16 bytes at the
+// lanes' addresses, as fragments; transposed ones with `trans`.
+template <bool kTrans>
+__device__ __forceinline__ void load_matrices(uint32_t (&r)[4], const void *p) {
+  if constexpr (kTrans)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(smem_u32(p))
+                 : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(smem_u32(p))
+                 : "memory");
+}
 
 // The running join of partial results (m, l, a) of four dims of a query.
 struct Joined {
@@ -944,14 +958,13 @@ __device__ __forceinline__ void put_result(const Args &a, int row, int head, int
 // four join through shared memory.  Per 16 tokens, with tokens on the M side:
 //   S^T[16 tokens, 8 columns] = K Q^T, O^T[D dims, 8 columns] += V^T P^T.
 // What bounds it are the bytes of K and V and the latency of getting at them
-// (length, page, tokens: three round trips), so the copies go to shared memory
-// without registers (16 rows of K and of V per warp at D = 128) and six CTAs
-// fit an SM; a block's K is replaced as soon as it has been multiplied, its V
-// likewise.  Lane (g, c) = (lane / 4, lane % 4) reads K at dims 32 i + 8 c of
-// tokens g and g + 8 (the contraction runs over the dims in that order on both
-// sides) and V at dims 64 i + 8 g of tokens 2c, 2c+1, 2c+8, 2c+9, pairing tokens
-// with byte permutes, which is the transposed operand; the 16-byte chunks of a
-// row are exchanged by its number so that neither read has bank conflicts.
+// (length, page, tokens: three round trips), and, as one warp's instructions
+// depend on one another, their number.  The copies go to shared memory without
+// registers, a block's K is replaced as soon as it has been multiplied, its V
+// likewise; fragments are loaded as 8 x 8 matrices, V transposed on the way
+// (its 16-byte chunks are exchanged by the token's number, so that no read has
+// bank conflicts); the maximum moves only when a column has outgrown it by 2^8,
+// as in the prefix kernel.
 // With one split the CTA also joins the prefix's partial results and writes the
 // output; else it leaves partial results to the join kernel.
 template <typename T, int D, int W>
@@ -961,17 +974,15 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? 11 : 3) own_kernel(const Args
   // came before.  Its results are waited for where they are read, below.
   if (!a.after_prefix) qb200::griddep_wait();
   qb200::griddep_launch_dependents();
-  constexpr int KI = D / 32;       // 16-byte chunks of a token per lane (scores)
-  constexpr int VI = D / 64;       // 16-byte chunks of a token per lane (values)
-  constexpr int NB = 128 / D;      // 16-token steps of a block
-  constexpr int BT = 16 * NB;      // tokens of a warp's block: 4 KB of K and of V
+  constexpr int DT = D / 16;       // 16-dim steps
+  constexpr int NB = (W == 1 ? 2 : 1) * 128 / D;  // 16-token steps of a block
+  constexpr int BT = 16 * NB;      // tokens of a warp's block: 8 KB of K and of V (4 KB with four warps)
   constexpr int CPR = D / 8;       // 16-byte chunks of a token
   constexpr int RPI = 32 / CPR;    // tokens that a warp copies at a time
-  constexpr int QP = D + 32;       // pitch of a query row: the fragment reads of two rows take all banks
+  constexpr int QP = D + 8;        // pitch of a query row: the fragment reads of eight rows take all banks
   constexpr int OP = D + 4;        // pitch of an output column
-  constexpr int R = W == 1 ? 2 : 1;  // blocks of a warp in shared memory
   constexpr int NT = 32 * W;
-  __shared__ __align__(128) T s_kv[W][R][2][BT * D];
+  __shared__ __align__(128) T s_kv[W][2][BT * D];
   __shared__ __align__(16) T s_q[8 * QP];
   __shared__ float s_m[W][8], s_l[W][8];
   static_assert(8 * OP * 4 <= sizeof(s_kv) / W, "a warp's output columns fit its copies' place");
@@ -1012,15 +1023,13 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? 11 : 3) own_kernel(const Args
   }
 
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  // O^T tile (i, e): rows g = dims 64 i + 8 g + e, rows g + 8 = those + 4;
-  // columns 2c, 2c + 1.
-  float o[VI][4][4];
+  // O^T step i: rows g = dims 16 i + g, rows g + 8 = dims 16 i + 8 + g; columns
+  // 2c, 2c + 1.
+  float o[DT][4];
 #pragma unroll
-  for (int i = 0; i < VI; ++i)
+  for (int i = 0; i < DT; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) o[i][e][x] = 0.f;
+    for (int x = 0; x < 4; ++x) o[i][x] = 0.f;
   bool seen[2] = {false, false};
   const int b0 = lo + BT * warp;
   const int *trow = a.page_table + (my_seq < 0 ? 0 : my_seq * a.table_pitch);
@@ -1053,39 +1062,42 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? 11 : 3) own_kernel(const Args
       qv0[i] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (row + col / nh) * a.q_row +
                                                 (kvh * a.ratio + h0 + col % nh) * a.q_head + 8 * (x % CPR));
   }
-  // Copies block j of K or V (xk: the exchange of K's chunks, else V's), and
-  // closes the group of copies (an empty one behind the last block).
-  const auto fetch = [&](const void *pool, int j, bool xk) {
-    if (j >= nb) {
-      copy_commit();
-      return;
-    }
-    T *dst = s_kv[warp][j % R][xk ? 0 : 1];
-    if (xk && j > 0 && (j * NB & 31) == 0) lookup(j * NB);
-    const int ch = lane % CPR, t0 = lane / CPR;  // chunk; token within a step of RPI
-    const T *src = static_cast<const T *>(pool) + kvh * a.head_stride + 8 * ch;
-    const int left = hi - (b0 + W * BT * j);
+  // Copies block j of K or V and closes the group of copies (an empty one
+  // behind the last block).
+  const int ch = lane % CPR, t0 = lane / CPR;  // this lane's chunk, and token of every RPI
+  const T *kfrom = static_cast<const T *>(a.k_pool) + kvh * a.head_stride + t0 * a.token_stride + 8 * ch;
+  const T *vfrom = static_cast<const T *>(a.v_pool) + kvh * a.head_stride + t0 * a.token_stride + 8 * ch;
+  const auto fetch = [&](bool is_k, int j) {
+    if (j < nb) {
+      if (is_k && j > 0 && (j * NB & 31) == 0) lookup(j * NB);
+      const int left = hi - (b0 + W * BT * j);
+      const T *pool = is_k ? kfrom : vfrom;
+      T *dst = s_kv[warp][is_k ? 0 : 1] + t0 * D;
 #pragma unroll
-    for (int k = 0; k < NB; ++k) {
-      const long long at = __shfl_sync(0xffffffffu, where, (j * NB + k) & 31);
-      const uint32_t bit = 1u << ((j * NB + k) & 31);
-      if (xk) ready = at >= 0 ? ready | bit : ready & ~bit;
-      const int n = at >= 0 ? left - 16 * k : 0;
-      const T *from = src + (at >= 0 ? at : 0) + t0 * a.token_stride;
+      for (int k = 0; k < NB; ++k) {
+        const long long at = __shfl_sync(0xffffffffu, where, (j * NB + k) & 31);
+        const uint32_t bit = 1u << ((j * NB + k) & 31);
+        if (is_k) ready = at >= 0 ? ready | bit : ready & ~bit;
+        const int n = at >= 0 ? left - 16 * k : 0;
+        const T *from = pool + (at >= 0 ? at : 0);
+        if (n >= 16) {
 #pragma unroll
-      for (int i = 0; i < 16 / RPI; ++i) {
-        const int t = i * RPI + t0;
-        const int x = xk ? (t & 1) << 2 : ((t >> 1) & 3) << 1;
-        copy16(dst + (16 * k + t) * D + 8 * (ch ^ x), t < n ? from + i * RPI * a.token_stride : src, t < n);
+          for (int i = 0; i < 16 / RPI; ++i)
+            copy16(dst + (16 * k + i * RPI) * D + 8 * (ch ^ ((i * RPI + t0) & 7)), from + i * RPI * a.token_stride, true);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16 / RPI; ++i) {
+            const bool on = i * RPI + t0 < n;
+            copy16(dst + (16 * k + i * RPI) * D + 8 * (ch ^ ((i * RPI + t0) & 7)),
+                   on ? from + i * RPI * a.token_stride : pool, on);
+          }
+        }
       }
     }
     copy_commit();
   };
-#pragma unroll
-  for (int j = 0; j < R; ++j) {
-    fetch(a.k_pool, j, true);
-    fetch(a.v_pool, j, false);
-  }
+  fetch(true, 0);
+  fetch(false, 0);
 #pragma unroll
   for (int i = 0; i < QC; ++i) {
     const int x = threadIdx.x + i * NT;
@@ -1099,14 +1111,15 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? 11 : 3) own_kernel(const Args
     parts = prefix_parts(a, a.row_plan[row + col / nh], kvh * a.ratio + h0 + col % nh);
   }
   __syncthreads();
+  uint32_t qf[DT][2];
+#pragma unroll
+  for (int i = 0; i < DT; ++i)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) qf[i][x] = *reinterpret_cast<const uint32_t *>(s_q + g * QP + 16 * i + 8 * x + 2 * c);
+  const T *sk = s_kv[warp][0], *sv = s_kv[warp][1];
   for (int j = 0; j < nb; ++j) {
     const int b = b0 + W * BT * j;
-    const T *sk = s_kv[warp][j % R][0], *sv = s_kv[warp][j % R][1];
-    // Visible steps of the block (its pages are mapped).
-    bool mapped[NB];
-#pragma unroll
-    for (int k = 0; k < NB; ++k) mapped[k] = (ready >> ((j * NB + k) & 31)) & 1u;
-    copy_wait<2 * R - 1>();
+    copy_wait<1>();
     __syncwarp();
     float s[NB][4];  // (token g, columns 2c, 2c+1), (token g + 8, ...)
 #pragma unroll
@@ -1114,109 +1127,117 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? 11 : 3) own_kernel(const Args
 #pragma unroll
       for (int x = 0; x < 4; ++x) s[k][x] = 0.f;
 #pragma unroll
-      for (int i = 0; i < KI; ++i) {
-        const int t = 16 * k + g, ch = (4 * i + c) ^ ((g & 1) << 2);
-        const uint4 k0 = *reinterpret_cast<const uint4 *>(sk + t * D + 8 * ch);
-        const uint4 k1 = *reinterpret_cast<const uint4 *>(sk + (t + 8) * D + 8 * ch);
-        const uint4 qv = *reinterpret_cast<const uint4 *>(s_q + g * QP + 32 * i + 8 * c);
-        mma16816<T>(s[k], k0.x, k1.x, k0.y, k1.y, qv.x, qv.y);
-        mma16816<T>(s[k], k0.z, k1.z, k0.w, k1.w, qv.z, qv.w);
+      for (int i = 0; i < DT; ++i) {
+        const int t = 16 * k + (lane & 15);
+        uint32_t f[4];
+        load_matrices<false>(f, sk + t * D + 8 * ((2 * i + (lane >> 4)) ^ (lane & 7)));
+        mma16816<T>(s[k], f[0], f[1], f[2], f[3], qf[i][0], qf[i][1]);
       }
+    }
+    // Masks: none for a block that every column sees whole.
+    uint32_t mapped = ready >> ((j * NB) & 31);
+    const bool whole = b + BT <= min(hi, min_len) && (~mapped & ((1u << NB) - 1u)) == 0;
+    if (!whole) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int end = min(clen[h], hi);
+#pragma unroll
+        for (int k = 0; k < NB; ++k) {
+          const bool on = (mapped >> k) & 1u;
+          if (!(on && b + 16 * k + g < end)) s[k][h] = -INFINITY;
+          if (!(on && b + 16 * k + g + 8 < end)) s[k][2 + h] = -INFINITY;
+          seen[h] = seen[h] || (on && b + 16 * k < end);
+        }
+      }
+    } else {
+      seen[0] = seen[1] = true;
     }
     __syncwarp();
-    fetch(a.k_pool, j + R, true);
-    uint32_t pb[NB][2];
+    fetch(true, j + 1);
+    float mx[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float mx = -INFINITY;
+      mx[h] = fmaxf(s[0][h], s[0][2 + h]);
 #pragma unroll
-      for (int k = 0; k < NB; ++k)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          float &v = s[k][2 * x + h];
-          v = mapped[k] && b + 16 * k + g + 8 * x < min(clen[h], hi) ? v * a.scale_log2 : -INFINITY;
-          mx = fmaxf(mx, v);
-          seen[h] = seen[h] || (mapped[k] && b + 16 * k < min(clen[h], hi));
-        }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-      const float mn = fmaxf(m[h], mx);
-      const float mu = mn == -INFINITY ? 0.f : mn;
-      const float f = ex2_approx(m[h] - mu);
-      l[h] *= f;
-#pragma unroll
-      for (int k = 0; k < NB; ++k) {
-        s[k][h] = ex2_approx(s[k][h] - mu);
-        s[k][2 + h] = ex2_approx(s[k][2 + h] - mu);
-        l[h] += s[k][h] + s[k][2 + h];
-      }
-      m[h] = mn;
-#pragma unroll
-      for (int i = 0; i < VI; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          o[i][e][h] *= f;
-          o[i][e][2 + h] *= f;
-        }
+      for (int k = 1; k < NB; ++k) mx[h] = fmaxf(mx[h], fmaxf(s[k][h], s[k][2 + h]));
+      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 4));
+      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 8));
+      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 16)) * a.scale_log2;
     }
+    if (__any_sync(0xffffffffu, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f)) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float mn = fmaxf(m[h], mx[h]);
+        const float f = mn == -INFINITY ? 1.f : ex2_approx(m[h] - mn);
+        m[h] = mn;
+        l[h] *= f;
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+          o[i][h] *= f;
+          o[i][2 + h] *= f;
+        }
+      }
+    }
+    const float mu0 = m[0] == -INFINITY ? 0.f : m[0], mu1 = m[1] == -INFINITY ? 0.f : m[1];
     // P^T as the B operand (n = column g, k = tokens 2c, 2c+1 / 2c+8, 2c+9).
     // The weights are rounded to the input type for the product (half a step
     // each, as the values they weigh); their sum is not.
+    uint32_t pb[NB][2];
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
+      s[k][0] = ex2_approx(fmaf(s[k][0], a.scale_log2, -mu0));
+      s[k][1] = ex2_approx(fmaf(s[k][1], a.scale_log2, -mu1));
+      s[k][2] = ex2_approx(fmaf(s[k][2], a.scale_log2, -mu0));
+      s[k][3] = ex2_approx(fmaf(s[k][3], a.scale_log2, -mu1));
+      l[0] += s[k][0] + s[k][2];
+      l[1] += s[k][1] + s[k][3];
       pb[k][0] = transpose8x8(Type<T>::pack(s[k][0], s[k][1]));
       pb[k][1] = transpose8x8(Type<T>::pack(s[k][2], s[k][3]));
     }
-    copy_wait<2 * R - 1>();
+    copy_wait<1>();
     __syncwarp();
-    // o += V^T P^T; with `limit`, V counts as zero from that position on and
-    // only the columns of row `only` of the run are added: a value that one
-    // row sees and another does not may be anything (0 x NaN).
-    const auto values = [&](int limit, int only) {
+    // V^T of 16 dims and 16 tokens: matrix q of a lane's eight is tokens 8 (q / 2)
+    // and dims 8 (q % 2) of them.
+    const int vt = (lane & 7) + ((lane >> 4) << 3), vc = (lane >> 3) & 1;
+    if (nrun == 1 || b + BT <= min_len) {
 #pragma unroll
       for (int k = 0; k < NB; ++k)
 #pragma unroll
-        for (int i = 0; i < VI; ++i) {
-          uint4 vv[4];
+        for (int i = 0; i < DT; ++i) {
+          uint32_t f[4];
+          load_matrices<true>(f, sv + (16 * k + vt) * D + 8 * ((2 * i + vc) ^ (lane & 7)));
+          mma16816<T>(o[i], f[0], f[1], f[2], f[3], pb[k][0], pb[k][1]);
+        }
+    } else {
+      // Tokens that some rows of the run see and others do not may be anything
+      // (0 x NaN): each row's columns are added by themselves, with V zero from
+      // the row's length on.
+#pragma unroll 1
+      for (int r = 0; r < nrun; ++r) {
+        const int limit = __shfl_sync(0xffffffffu, len, r) - b;  // tokens of the block that row r sees
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int t = 16 * k + 2 * c + (x & 1) + 8 * (x >> 1);
-            vv[x] = *reinterpret_cast<const uint4 *>(sv + t * D + 8 * ((8 * i + g) ^ (c << 1)));
-            if (only >= 0 && b + t >= limit) vv[x] = make_uint4(0, 0, 0, 0);
-          }
+        for (int k = 0; k < NB; ++k) {
+          // Both halves, the lower or none of the pairs at tokens 2c and 2c + 8.
+          const int n0 = limit - 16 * k - 2 * c, n1 = n0 - 8;
+          const uint32_t w0 = n0 >= 2 ? ~0u : n0 == 1 ? 0xffffu : 0u, w1 = n1 >= 2 ? ~0u : n1 == 1 ? 0xffffu : 0u;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            // A rows g: dim 8 g + e; rows g + 8: dim 8 g + e + 4.
-            const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
-            const int w0 = e >> 1, w1 = 2 + (e >> 1);
-            const uint32_t a0 = __byte_perm(word(vv[0], w0), word(vv[1], w0), sel);
-            const uint32_t a1 = __byte_perm(word(vv[0], w1), word(vv[1], w1), sel);
-            const uint32_t a2 = __byte_perm(word(vv[2], w0), word(vv[3], w0), sel);
-            const uint32_t a3 = __byte_perm(word(vv[2], w1), word(vv[3], w1), sel);
-            if (only < 0) {
-              mma16816<T>(o[i][e], a0, a1, a2, a3, pb[k][0], pb[k][1]);
-            } else {
-              float d[4] = {0.f, 0.f, 0.f, 0.f};
-              mma16816<T>(d, a0, a1, a2, a3, pb[k][0], pb[k][1]);
+          for (int i = 0; i < DT; ++i) {
+            uint32_t f[4];
+            load_matrices<true>(f, sv + (16 * k + vt) * D + 8 * ((2 * i + vc) ^ (lane & 7)));
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            mma16816<T>(d, f[0] & w0, f[1] & w0, f[2] & w1, f[3] & w1, pb[k][0], pb[k][1]);
 #pragma unroll
-              for (int h = 0; h < 2; ++h)
-                if ((2 * c + h) / nh == only) {
-                  o[i][e][h] += d[h];
-                  o[i][e][2 + h] += d[2 + h];
-                }
-            }
+            for (int h = 0; h < 2; ++h)
+              if ((2 * c + h) / nh == r) {
+                o[i][h] += d[h];
+                o[i][2 + h] += d[2 + h];
+              }
           }
         }
-    };
-    if (b + BT <= min_len || nrun == 1) {
-      values(0, -1);
-    } else {
-#pragma unroll 1
-      for (int r = 0; r < nrun; ++r) values(__shfl_sync(0xffffffffu, len, r), r);
+      }
     }
     __syncwarp();
-    fetch(a.v_pool, j + R, false);
+    fetch(false, j + 1);
   }
   copy_wait<0>();
   __syncwarp();
@@ -1233,10 +1254,9 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? 11 : 3) own_kernel(const Args
       s_l[warp][2 * c + h] = l[h];
     }
 #pragma unroll
-    for (int i = 0; i < VI; ++i) {
-      float *d = so + (2 * c + h) * OP + 64 * i + 8 * g;
-      *reinterpret_cast<float4 *>(d) = make_float4(o[i][0][h], o[i][1][h], o[i][2][h], o[i][3][h]);
-      *reinterpret_cast<float4 *>(d + 4) = make_float4(o[i][0][2 + h], o[i][1][2 + h], o[i][2][2 + h], o[i][3][2 + h]);
+    for (int i = 0; i < DT; ++i) {
+      so[(2 * c + h) * OP + 16 * i + g] = o[i][h];
+      so[(2 * c + h) * OP + 16 * i + 8 + g] = o[i][2 + h];
     }
   }
   __syncthreads();
