@@ -84,12 +84,14 @@ int qwen_b200_paged_status(uint64_t *detail);
  * Plan of a batch's groups (host arrays; sum of group_rows = rows): fills
  * `words` (host, int32) and returns how many it wrote, which the caller
  * copies to 16-byte aligned device memory; with words NULL only returns the
- * number.  0: bad arguments (qwen_b200_last_error).  ctas: CTAs that share
- * the prefix work (the device's SM count).  The first
+ * number.  0: bad arguments (qwen_b200_last_error).  max_length: about the
+ * longest row (it weighs the prefix work against the rows' own).  ctas: CTAs
+ * that share the prefix work at most (the device's SM count).  The first
  * QWEN_PREFIX_HEADER words are also the host's view of the plan. */
 #define QWEN_PREFIX_HEADER 16
 int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_lens, int heads,
-                          int kv_heads, int ctas, int *words, int capacity);
+                          int kv_heads, int dim, int max_length, int ctas, int *words,
+                          int capacity);
 
 typedef struct QwenPrefixAttention {
   const void *q;            /* [rows, heads, dim], last dimension contiguous */

@@ -1482,8 +1482,8 @@ int qb200_prefix_check(const QwenPrefixAttention *u) {
 
 extern "C" {
 
-int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_lens, int heads, int kv_heads, int ctas,
-                          int *words, int capacity) {
+int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_lens, int heads, int kv_heads,
+                          int dim, int max_length, int ctas, int *words, int capacity) {
   qb200_clear_error();
   const auto bad = [](int code, const char *msg) {
     qb200_set_error(code, msg);
@@ -1492,6 +1492,8 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
   if (groups < 1 || group_rows == nullptr || prefix_lens == nullptr) return bad(13, "plan: no groups");
   if (kv_heads < 1 || heads < kv_heads || heads % kv_heads != 0 || heads / kv_heads > 128 || kv_heads > 4096)
     return bad(10, "plan: heads must be a multiple of kv_heads, at most 128 per kv head");
+  if (max_length < 0) return bad(10, "plan: negative max_length");
+  if (dim != 64 && dim != 128) return bad(10, "plan: dim 64 or 128");
   if (ctas < 1 || ctas > 4096) return bad(10, "plan: ctas outside [1, 4096]");
   const int ratio = heads / kv_heads;
   long long rows = 0, tiles = 0, weight = 0;
@@ -1545,6 +1547,17 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
       if (parts_at(2 * mid) <= ctas) hi = mid; else lo = mid + 1;
     }
     if (2 * lo <= (weight + ctas - 1) / ctas + kSegWeight) part = 2 * lo;
+  }
+  if (part > 0) {
+    // The prefix kernel leaves DRAM idle, and the own kernel runs on the SMs
+    // that it leaves: when the own part is the longer one, the prefix takes
+    // fewer CTAs for longer, up to half of the own part's time (rows of half
+    // the longest own length at 4.5 TB/s, and 8 us), at 8 us and 1.1 us per
+    // weight (256 rows behind 2048 tokens: 64 CTAs 44.4 us in all, 128 50.1,
+    // 32 53.0).
+    const double own = rows * 0.5 * (max_length > max_prefix ? max_length - max_prefix : 0) * kv_heads * dim * 4 / 4.5e6 + 8;
+    const long long most = static_cast<long long>((0.5 * own - 8) / 1.1) / 2 * 2;
+    if (most > part) part = most;
   }
   if (part > 0) ctas = static_cast<int>(parts_at(part));
   if (ctas > weight) ctas = weight > 0 ? static_cast<int>(weight) : 1;

@@ -34,7 +34,7 @@ def lib() -> ctypes.CDLL:
             raise RuntimeError(f"{path} is missing: build it with qwen0.6b_b200/build.py")
         L = ctypes.CDLL(path)
         vp, i, ll, u64p = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.POINTER(ctypes.c_uint64)
-        for name, res, args in [("paged_status", i, [u64p]), ("prefix_plan", i, [i, vp, vp, i, i, i, vp, i]),
+        for name, res, args in [("paged_status", i, [u64p]), ("prefix_plan", i, [i, vp, vp, i, i, i, i, i, vp, i]),
                                 ("prefix_workspace", ll, [vp, i, i]), ("prefix_status", i, [vp, vp, u64p]),
                                 ("last_error", i, [ctypes.c_char_p, i])]:
             f = getattr(L, "qwen_b200_" + name)
@@ -153,7 +153,7 @@ class PrefixPlan:
             raise ValueError(f"a plan lives on a CUDA device, not {self.device}")
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
-        words = plan_words(rows, lens, num_q_heads, num_kv_heads,
+        words = plan_words(rows, lens, num_q_heads, num_kv_heads, head_dim, max_length,
                            torch.cuda.get_device_properties(self.device).multi_processor_count)
         self.rows = int(words[1])
         self.num_q_heads, self.num_kv_heads, self.head_dim = num_q_heads, num_kv_heads, head_dim
@@ -171,9 +171,10 @@ class PrefixPlan:
 
 
 def plan_words(group_rows: torch.Tensor, prefix_lens: torch.Tensor, num_q_heads: int, num_kv_heads: int,
-               ctas: int) -> torch.Tensor:
+               head_dim: int, max_length: int, ctas: int) -> torch.Tensor:
     """The int32 words of a plan (host), as ``qwen_b200_prefix_plan`` fills them."""
-    args = (group_rows.numel(), group_rows.data_ptr(), prefix_lens.data_ptr(), num_q_heads, num_kv_heads, ctas)
+    args = (group_rows.numel(), group_rows.data_ptr(), prefix_lens.data_ptr(), num_q_heads, num_kv_heads, head_dim,
+            max_length, ctas)
     n = lib().qwen_b200_prefix_plan(*args, None, 0)
     if n <= 0:
         raise ValueError(f"PrefixPlan: {_last_error()}")

@@ -110,7 +110,7 @@ def test_empty_lists_are_no_calls(name, k):
 
 
 def _attention(**kw):
-    words = paged.plan_words(torch.tensor([4], dtype=torch.int32), torch.tensor([256], dtype=torch.int32), 4, 2, 148)
+    words = paged.plan_words(torch.tensor([4], dtype=torch.int32), torch.tensor([256], dtype=torch.int32), 4, 2, 128, 512, 148)
     header = words[:16].clone()
     kw = dict(kw)
     if kw.pop("bad_plan", False):
@@ -159,7 +159,7 @@ def test_attention_arguments_are_refused(kw, what):
 ])
 def test_plan_arguments_are_refused(rows, lens, heads, kv, ctas):
     with pytest.raises(ValueError, match="plan"):
-        paged.plan_words(torch.tensor(rows, dtype=torch.int32), torch.tensor(lens, dtype=torch.int32), heads, kv, ctas)
+        paged.plan_words(torch.tensor(rows, dtype=torch.int32), torch.tensor(lens, dtype=torch.int32), heads, kv, 64, 512, ctas)
 
 
 def test_python_refusals_without_a_gpu():
@@ -183,9 +183,9 @@ def test_python_refusals_without_a_gpu():
         paged._host_list([1 << 40], "x")
 
 
-def _plan(rows, lens, heads, kv, ctas):
+def _plan(rows, lens, heads, kv, longest, ctas):
     w = paged.plan_words(torch.tensor(rows, dtype=torch.int32), torch.tensor(lens, dtype=torch.int32), heads, kv,
-                         ctas).tolist()
+                         128, longest, ctas).tolist()
     h = w[:16]
     cta = [w[h[8] + 16 * i:h[8] + 16 * i + 16] for i in range(h[3])]  # what each CTA reads first
     return dict(rows=h[1], cta=cta,
@@ -203,7 +203,7 @@ def test_plans_cover_every_tile_once(seed):
     rows = [r.choice([0, 1, 2, 3, 17, 64, 100]) for _ in range(n)] + [3]
     lens = [r.choice([0, 1, 15, 16, 127, 128, 129, 1000, 5000]) for _ in rows]
     ctas = r.choice([1, 3, 148])
-    p = _plan(rows, lens, kv * ratio, kv, ctas)
+    p = _plan(rows, lens, kv * ratio, kv, r.choice([0, 200, 6000, 60000]), ctas)
     assert p["rows"] == sum(rows) and len(p["cta"]) <= ctas
     assert [c[0] for c in p["cta"]] + [len(p["segs"])] == [0] + [c[1] for c in p["cta"]]
     for first, last, *_, in p["cta"]:
