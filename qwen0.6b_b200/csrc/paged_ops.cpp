@@ -54,14 +54,26 @@ QwenPageTable table_of(const Tensor &t) {
                        t.size(0) > 1 ? t.stride(0) : t.size(1)};
 }
 
-// A host list: contiguous int32 on the CPU (paged.py makes it one).
-const int *list_of(const Tensor &t, const Tensor &first, const char *name) {
-  TORCH_CHECK_VALUE(t.device().is_cpu() && t.dim() == 1 && t.scalar_type() == torch::kInt && t.is_contiguous(), name,
-                    " must be a contiguous int32 list on the host");
-  TORCH_CHECK_VALUE(t.numel() == first.numel(), name, " has ", t.numel(), " entries, the other lists ", first.numel());
-  TORCH_CHECK_VALUE(t.numel() < (1ll << 31), name, " has over 2^31 entries");
-  return t.data_ptr<int>();
-}
+// A list of integers on the host, as contiguous int32.
+struct HostList {
+  Tensor t;
+  HostList(const Tensor &given, const char *name, int64_t n = -1) : t(given) {
+    TORCH_CHECK_VALUE(t.device().is_cpu() && t.dim() == 1 && at::isIntegralType(t.scalar_type(), false), name,
+                      " must be a one-dimensional list of integers on the host");
+    TORCH_CHECK_VALUE(n < 0 || t.numel() == n, name, " has ", t.numel(), " entries, the other lists ", n);
+    TORCH_CHECK_VALUE(t.numel() < (1ll << 31), name, " has over 2^31 entries");
+    if (t.scalar_type() != torch::kInt) {
+      const Tensor wide = t.to(torch::kLong);
+      TORCH_CHECK_VALUE(wide.numel() == 0 || (wide.min().item<int64_t>() >= -(1ll << 31) &&
+                                              wide.max().item<int64_t>() < (1ll << 31)),
+                        name, " holds a value outside 32 bits");
+      t = wide.to(torch::kInt);
+    }
+    t = t.contiguous();
+  }
+  const int *data() const { return t.data_ptr<int>(); }
+  int size() const { return static_cast<int>(t.numel()); }
+};
 
 void same_device(const Tensor &t, const Tensor &k) {
   TORCH_CHECK_VALUE(t.device() == k.device(), "page_table is on ", t.device(), ", the pools on ", k.device());
@@ -70,11 +82,11 @@ void same_device(const Tensor &t, const Tensor &k) {
 void copy_pages(const Tensor &k, const Tensor &v, const Tensor &src, const Tensor &dst,
                 const std::optional<Tensor> &tokens) {
   const QwenPagePools p = pools_of(k, v);
+  const HostList s(src, "src"), d(dst, "dst", s.size());
+  std::optional<HostList> t;
+  if (tokens) t.emplace(*tokens, "tokens", s.size());
   const c10::cuda::CUDAGuard guard(k.device());
-  check_rc(qwen_b200_pages_copy(&p, list_of(src, src, "src"), list_of(dst, src, "dst"),
-                                tokens ? list_of(*tokens, src, "tokens") : nullptr, static_cast<int>(src.numel()),
-                                stream_of(k)),
-           "copy_pages");
+  check_rc(qwen_b200_pages_copy(&p, s.data(), d.data(), t ? t->data() : nullptr, s.size(), stream_of(k)), "copy_pages");
 }
 
 void fork_pages(const Tensor &table, const Tensor &k, const Tensor &v, const Tensor &parents, const Tensor &children,
@@ -82,10 +94,10 @@ void fork_pages(const Tensor &table, const Tensor &k, const Tensor &v, const Ten
   const QwenPagePools p = pools_of(k, v);
   const QwenPageTable t = table_of(table);
   same_device(table, k);
+  const HostList from(parents, "parents"), to(children, "children", from.size()), n(lengths, "lengths", from.size()),
+      pages(new_pages, "new_pages", from.size());
   const c10::cuda::CUDAGuard guard(k.device());
-  check_rc(qwen_b200_pages_fork(&p, &t, list_of(parents, parents, "parents"), list_of(children, parents, "children"),
-                                list_of(lengths, parents, "lengths"), list_of(new_pages, parents, "new_pages"),
-                                static_cast<int>(parents.numel()), stream_of(k)),
+  check_rc(qwen_b200_pages_fork(&p, &t, from.data(), to.data(), n.data(), pages.data(), from.size(), stream_of(k)),
            "fork_pages");
 }
 
@@ -93,17 +105,16 @@ void compact_pages(const Tensor &table, const Tensor &k, const Tensor &v, const 
   const QwenPagePools p = pools_of(k, v);
   const QwenPageTable t = table_of(table);
   same_device(table, k);
+  const HostList s(src, "src"), d(dst, "dst", s.size());
   const c10::cuda::CUDAGuard guard(k.device());
-  check_rc(qwen_b200_pages_compact(&p, &t, list_of(src, src, "src"), list_of(dst, src, "dst"),
-                                   static_cast<int>(src.numel()), stream_of(k)),
-           "compact_pages");
+  check_rc(qwen_b200_pages_compact(&p, &t, s.data(), d.data(), s.size(), stream_of(k)), "compact_pages");
 }
 
 void free_pages(const Tensor &table, const Tensor &seqs) {
   const QwenPageTable t = table_of(table);
+  const HostList s(seqs, "seqs");
   const c10::cuda::CUDAGuard guard(table.device());
-  check_rc(qwen_b200_pages_free(&t, list_of(seqs, seqs, "seqs"), static_cast<int>(seqs.numel()), stream_of(table)),
-           "free_pages");
+  check_rc(qwen_b200_pages_free(&t, s.data(), s.size(), stream_of(table)), "free_pages");
 }
 
 // Stride of a dimension; that of a one-element dimension, which torch leaves

@@ -65,21 +65,13 @@ def _ext():
 
 # ------------------------------------------------------------------- pages
 def _host_list(values, name: str) -> torch.Tensor:
-    """`values` (a sequence or a CPU integer tensor) as contiguous int32 on the host."""
-    if isinstance(values, torch.Tensor):
-        t = values
-        if t.dtype == torch.int32 and t.device.type == "cpu" and t.dim() == 1 and t.is_contiguous():
-            return t
-        if t.device.type != "cpu" or t.dim() != 1 or t.is_floating_point() or t.dtype == torch.bool:
-            raise ValueError(f"{name} must be a one-dimensional list of integers on the host")
-    else:
-        values = list(values)
-        if any(not -2**31 <= v < 2**31 for v in values):
-            raise ValueError(f"{name} holds a value outside 32 bits")
-        return torch.tensor(values, dtype=torch.int32)
-    if t.numel() and (int(t.min()) < -2**31 or int(t.max()) >= 2**31):
+    """A sequence of integers as an int32 tensor on the host; a tensor as it is (the extension checks it)."""
+    if type(values) is torch.Tensor:
+        return values
+    values = list(values)
+    if any(not -2**31 <= v < 2**31 for v in values):
         raise ValueError(f"{name} holds a value outside 32 bits")
-    return t.to(torch.int32).contiguous()
+    return torch.tensor(values, dtype=torch.int32)
 
 
 def copy_pages(k_pool: torch.Tensor, v_pool: torch.Tensor, src, dst, tokens=None) -> None:
@@ -140,8 +132,8 @@ class PrefixPlan:
 
     def __init__(self, group_rows, prefix_lens, num_q_heads: int, num_kv_heads: int, head_dim: int, max_length: int,
                  device=None):
-        rows = _host_list(group_rows, "group_rows")
-        lens = _host_list(prefix_lens, "prefix_lens")
+        rows = torch.as_tensor(_host_list(group_rows, "group_rows"), dtype=torch.int32, device="cpu").contiguous()
+        lens = torch.as_tensor(_host_list(prefix_lens, "prefix_lens"), dtype=torch.int32, device="cpu").contiguous()
         if lens.numel() != rows.numel():
             raise ValueError(f"prefix_lens has {lens.numel()} entries, group_rows {rows.numel()}")
         if head_dim not in (64, 128):

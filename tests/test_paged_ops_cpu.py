@@ -176,9 +176,6 @@ def test_python_refusals_without_a_gpu():
         paged.PrefixPlan([2], [16], 4, 2, 96, max_length=32)
     with pytest.raises(ValueError, match="entries"):
         paged.PrefixPlan([2, 1], [16], 4, 2, 64, max_length=32)
-    for bad in (torch.zeros(2, 2, dtype=torch.int32), torch.zeros(2), torch.tensor([True])):
-        with pytest.raises(ValueError, match="list of integers"):
-            paged._host_list(bad, "x")
     with pytest.raises(ValueError, match="32 bits"):
         paged._host_list([1 << 40], "x")
 

@@ -190,3 +190,32 @@ def test_offsets_past_32_bits():
     copy_pages(k, v, [69], [68], [100])
     assert bool((k[68, :, :, :100] == 1).all()) and bool((v[68, :, :, :100] == 2).all())
     assert not bool(k[68, :, :, 100:].any()) and not bool(k[:68].any())
+
+
+def test_refusals_leave_the_pools_alone():
+    from paged import compact_pages, copy_pages, fork_pages, free_pages
+    geo = (10, 1, 2, 16, 64, torch.float16)
+    raw, (k, v) = _pools(geo, 7)
+    table = torch.tensor([[0, 1], [-1, -1]], dtype=torch.int32, device="cuda")
+    for call, what in [
+            (lambda: copy_pages(k, v, [0], [1, 2]), "entries"),
+            (lambda: copy_pages(k, v, [0, 1], [1, 2]), "also a source"),
+            (lambda: copy_pages(k, v, [0], [10]), "outside the pool"),
+            (lambda: copy_pages(k, v, [0], [1 << 40]), "32 bits"),
+            (lambda: copy_pages(k, v, torch.tensor([0]), torch.tensor([1 << 40])), "32 bits"),
+            (lambda: copy_pages(k, v, torch.tensor([0.0]), [1]), "list of integers"),
+            (lambda: copy_pages(k, v, torch.tensor([0], device="cuda"), [1]), "list of integers"),
+            (lambda: copy_pages(k, v, torch.tensor([[0]]), [1]), "list of integers"),
+            (lambda: copy_pages(k[:, :, :, :8], v[:, :, :, :8], [0], [1]), "contiguous"),
+            (lambda: copy_pages(k, v[:5], [0], [1]), "same shape"),
+            (lambda: copy_pages(k, k, [0], [1]), "same pool"),
+            (lambda: copy_pages(k[..., :4].contiguous(), v[..., :4].contiguous(), [0], [1]), "multiple of 16"),
+            (lambda: fork_pages(table, k, v, [0], [0], [20], [5]), "also a parent"),
+            (lambda: fork_pages(table.long(), k, v, [0], [1], [20], [5]), "int32"),
+            (lambda: fork_pages(table.cpu(), k, v, [0], [1], [20], [5]), "CUDA"),
+            (lambda: compact_pages(table, k, v, [5, 5], [2, 3]), "moves twice"),
+            (lambda: free_pages(table, [2]), "outside the table")]:
+        with pytest.raises(ValueError, match=what):
+            call()
+    assert table.cpu().tolist() == [[0, 1], [-1, -1]]
+    _same(raw, (k, v))
