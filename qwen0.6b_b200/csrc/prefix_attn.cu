@@ -1287,46 +1287,65 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? 11 : 3) own_kernel(const Args
 }
 
 // -------------------------------------------------------------- join kernel
-// grid (heads, rows), 128 threads: D / 4 threads per partial result, several
-// partials at a time; the groups meet in shared memory in a fixed order.
-constexpr int JOIN_THREADS = 128;
+// grid (kv heads, rows): the partial results of one row's heads, several at a
+// time; the groups of threads that share them meet in shared memory in a fixed
+// order.  Neighbouring threads take the heads, whose prefix partials are
+// adjacent (with a CTA per head a warp's loads fell on 32 lines: 13 us behind
+// 60000 shared tokens, XX now).
+constexpr int JOIN_THREADS = 512;
 template <typename T, int D>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args a) {
+  constexpr int Q4 = D / 4;
+  __shared__ float s_m[JOIN_THREADS], s_l[JOIN_THREADS], s_none[JOIN_THREADS];
+  __shared__ __align__(16) float4 s_acc[JOIN_THREADS];
+  const int kvh = blockIdx.x, row = blockIdx.y;
+  const RowPlan rp = a.row_plan[row];
+  const int nout = a.ratio * Q4, used = min(nout, JOIN_THREADS), ng = JOIN_THREADS / used;
+  const int grp = threadIdx.x / used;
   qb200::griddep_wait();
   qb200::griddep_launch_dependents();
-  constexpr int Q4 = D / 4, NG = JOIN_THREADS / Q4;
-  __shared__ float s_m[NG], s_l[NG], s_none[NG];
-  __shared__ __align__(16) float4 s_acc[NG][Q4];
-  const int head = blockIdx.x, row = blockIdx.y, grp = threadIdx.x / Q4, d4 = threadIdx.x % Q4;
   int seq;
   const int len = row_length(a, row, &seq);
-  const RowPlan rp = a.row_plan[row];
-  Joined j;
-  if (rp.prefix > 0 && len >= rp.prefix) join_prefix<D, 8>(a, prefix_parts(a, rp, head), d4, grp, NG, j);
-  if (len > 0) {
-    const int count = len - (len >= rp.prefix ? rp.prefix : 0);
-    const int ns = min(a.own_splits, (count + a.own_per - 1) / a.own_per);
-    const float *own = a.own + (static_cast<size_t>(row) * a.heads + head) * a.own_splits * (D + 4);
-    for (int s = grp; s < ns; s += NG) {
-      const float *p = own + static_cast<size_t>(s) * (D + 4);
-      j.add(p[D], p[D + 1], *reinterpret_cast<const float4 *>(p + 4 * d4));
-    }
-  }
-  if (d4 == 0) {
-    s_m[grp] = j.m;
-    s_l[grp] = j.l;
-    s_none[grp] = j.none;
-  }
-  s_acc[grp][d4] = j.acc;
-  __syncthreads();
-  if (grp != 0) return;
-  Joined r;
+  const bool shared = rp.prefix > 0 && len >= rp.prefix;
+  const int count = len - (shared ? rp.prefix : 0);
+  const int ns = count > 0 ? min(a.own_splits, (count + a.own_per - 1) / a.own_per) : 0;
+  for (int x0 = 0; x0 < nout; x0 += used) {
+    const int x = x0 + threadIdx.x % used, h = x % a.ratio, d4 = x / a.ratio, head = kvh * a.ratio + h;
+    Joined j;
+    if (grp < ng && x < nout) {
+      if (shared) join_prefix<D, 8>(a, prefix_parts(a, rp, head), d4, grp, ng, j);
+      const float *own = a.own + (static_cast<size_t>(row) * a.heads + head) * a.own_splits * (D + 4);
+      for (int s = grp; s < ns; s += 4 * ng) {
+        float m[4], l[4];
+        float4 v[4];
 #pragma unroll
-  for (int k = 0; k < NG; ++k) {
-    r.add(s_m[k], s_l[k], s_acc[k][d4]);
-    r.none += s_none[k];
+        for (int u = 0; u < 4; ++u) {
+          const bool on = s + u * ng < ns;
+          const float *p = own + static_cast<size_t>(on ? s + u * ng : 0) * (D + 4);
+          m[u] = on ? p[D] : -INFINITY;
+          l[u] = on ? p[D + 1] : 0.f;
+          v[u] = *reinterpret_cast<const float4 *>(p + 4 * d4);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) j.add(m[u], l[u], v[u]);
+      }
+    }
+    if (ng > 1) {
+      s_m[threadIdx.x] = j.m;
+      s_l[threadIdx.x] = j.l;
+      s_none[threadIdx.x] = j.none;
+      s_acc[threadIdx.x] = j.acc;
+      __syncthreads();
+      if (grp == 0) {
+        for (int k = 1; k < ng; ++k) {
+          j.add(s_m[k * used + threadIdx.x], s_l[k * used + threadIdx.x], s_acc[k * used + threadIdx.x]);
+          j.none += s_none[k * used + threadIdx.x];
+        }
+      }
+    }
+    if (grp == 0 && x < nout) put_result<T>(a, row, head, d4, j);
+    if (x0 + used < nout) __syncthreads();
   }
-  put_result<T>(a, row, head, d4, r);
 }
 
 }  // namespace qb200x
@@ -1440,7 +1459,7 @@ int launch(const QwenPrefixAttention &u, const Args &a, const CUtensorMap &mk, c
                                     : qb200_launch(own_kernel<T, D, 4>, grid, dim3(128), 0, st, true, a);
   if (e != cudaSuccess) return fail(20, "own attention launch: %s", cudaGetErrorString(e));
   if (a.own_splits == 1) return 0;  // the own kernel has joined both parts
-  e = qb200_launch(join_kernel<T, D>, dim3(a.heads, a.rows), dim3(JOIN_THREADS), 0, st, true, a);
+  e = qb200_launch(join_kernel<T, D>, dim3(a.kv_heads, a.rows), dim3(JOIN_THREADS), 0, st, true, a);
   if (e != cudaSuccess) return fail(20, "attention join launch: %s", cudaGetErrorString(e));
   return 0;
 }
