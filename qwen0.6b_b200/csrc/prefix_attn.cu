@@ -51,7 +51,7 @@ using qb200tc::tmem_ld64;
 // Header words, then the arrays they point at (offsets in words).
 enum PlanWord : int {
   PW_MAGIC = 0, PW_ROWS, PW_GROUPS, PW_CTAS, PW_SEGS, PW_TILES, PW_HEADS, PW_KV_HEADS,
-  PW_CTA, PW_SEG, PW_TILE_SLOT, PW_ROW, PW_ERR, PW_WORDS, PW_MIN_PREFIX, PW_MAX_PREFIX
+  PW_CTA, PW_SEG, PW_TILE_SLOT, PW_ROW, PW_ERR, PW_WORDS, PW_MAX_PREFIX, PW_SPARE
 };
 constexpr int PLAN_MAGIC = 0x51503031;
 // A segment is a CTA's run of token tiles of one query tile (up to 256
@@ -968,7 +968,7 @@ __device__ __forceinline__ void put_result(const Args &a, int row, int head, int
 // With one split the CTA also joins the prefix's partial results and writes the
 // output; else it leaves partial results to the join kernel.
 template <typename T, int D, int W>
-__global__ void __launch_bounds__(32 * W, W == 1 ? 11 : 3) own_kernel(const Args a) {
+__global__ void __launch_bounds__(32 * W, W == 1 ? 11 : 6) own_kernel(const Args a) {
   // Behind a prefix kernel of the same call nothing that this part reads is
   // new: the prefix kernel's CTAs have all passed their own wait for whatever
   // came before.  Its results are waited for where they are read, below.
@@ -1103,13 +1103,11 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? 11 : 3) own_kernel(const Args
     const int x = threadIdx.x + i * NT;
     if (x < 8 * CPR) *reinterpret_cast<uint4 *>(s_q + (x / CPR) * QP + 8 * (x % CPR)) = qv0[i];
   }
-  // Where the prefix's partial results of this thread's outputs lie.
+  // Where the prefix's partial results of each column lie (lane = column).
   constexpr int Q4 = D / 4;
-  PrefixParts parts{};
-  if (fused && my_start > 0 && static_cast<int>(threadIdx.x) < nc * Q4) {
-    const int col = threadIdx.x % nc;
-    parts = prefix_parts(a, a.row_plan[row + col / nh], kvh * a.ratio + h0 + col % nh);
-  }
+  const bool shared = fused && my_start > 0;
+  PrefixParts mine{};
+  if (shared && lane < nc) mine = prefix_parts(a, a.row_plan[row + lane / nh], kvh * a.ratio + h0 + lane % nh);
   __syncthreads();
   uint32_t qf[DT][2];
 #pragma unroll
@@ -1261,14 +1259,17 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? 11 : 3) own_kernel(const Args
   }
   __syncthreads();
   if (a.after_prefix) qb200::griddep_wait();
-  for (int x = threadIdx.x; x < nc * Q4; x += NT) {
+  for (int x0 = 0; x0 < nc * Q4; x0 += NT) {
     // Neighbouring threads take the columns: their prefix partials are adjacent.
-    const int col = x % nc, d4 = x / nc, r = row + col / nh, head = kvh * a.ratio + h0 + col % nh;
+    const int x = x0 + threadIdx.x, col = x % nc, d4 = x / nc;
+    PrefixParts parts;
+    parts.first = __shfl_sync(0xffffffffu, mine.first, col);
+    parts.count = __shfl_sync(0xffffffffu, mine.count, col);
+    parts.ql = __shfl_sync(0xffffffffu, mine.ql, col);
+    if (x >= nc * Q4) continue;
+    const int r = row + col / nh, head = kvh * a.ratio + h0 + col % nh;
     Joined j;
-    if (fused && my_start > 0) {
-      if (x >= NT) parts = prefix_parts(a, a.row_plan[r], head);
-      join_prefix<D, W == 1 ? 8 : 4>(a, parts, d4, 0, 1, j);
-    }
+    if (shared) join_prefix<D, W == 1 ? 8 : 4>(a, parts, d4, 0, 1, j);
 #pragma unroll
     for (int w = 0; w < W; ++w)
       j.add(s_m[w][col], s_l[w][col],
@@ -1379,7 +1380,8 @@ int own_splits(int rows, int kv_heads, int ratio, int own_tokens) {
   return s < 1 ? 1 : static_cast<int>(s);
 }
 
-int own_tokens(const int *h, int max_length) { return max_length > h[PW_MIN_PREFIX] ? max_length - h[PW_MIN_PREFIX] : 1; }
+// The longest own part expected: the longest row behind the longest prefix.
+int own_tokens(const int *h, int max_length) { return max_length > h[PW_MAX_PREFIX] ? max_length - h[PW_MAX_PREFIX] : 1; }
 
 // Tokens of one split (the last one takes whatever is left of a row).
 int own_part(int own, int splits) { return ((own + splits - 1) / splits + 127) / 128 * 128; }
@@ -1430,7 +1432,7 @@ int encode_pool(CUtensorMap *m, const QwenPrefixAttention &a, const void *pool, 
 
 // Warps of an own CTA.
 int own_warps(const Args &a) {
-  return static_cast<long long>(a.rows) * a.kv_heads * ((a.ratio + 7) / 8) * a.own_splits >= 1480 ? 1 : 4;
+  return static_cast<long long>(a.rows) * a.kv_heads * ((a.ratio + 7) / 8) * a.own_splits >= 1480 ? 1 : 2;
 }
 
 template <typename T, int D>
@@ -1456,7 +1458,7 @@ int launch(const QwenPrefixAttention &u, const Args &a, const CUtensorMap &mk, c
   }
   const dim3 grid(a.own_splits, a.kv_heads * ((a.ratio + 7) / 8), a.rows);
   cudaError_t e = own_warps(a) == 1 ? qb200_launch(own_kernel<T, D, 1>, grid, dim3(32), 0, st, true, a)
-                                    : qb200_launch(own_kernel<T, D, 4>, grid, dim3(128), 0, st, true, a);
+                                    : qb200_launch(own_kernel<T, D, 2>, grid, dim3(64), 0, st, true, a);
   if (e != cudaSuccess) return fail(20, "own attention launch: %s", cudaGetErrorString(e));
   if (a.own_splits == 1) return 0;  // the own kernel has joined both parts
   e = qb200_launch(join_kernel<T, D>, dim3(a.kv_heads, a.rows), dim3(JOIN_THREADS), 0, st, true, a);
@@ -1516,7 +1518,7 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
   if (ctas < 1 || ctas > 4096) return bad(10, "plan: ctas outside [1, 4096]");
   const int ratio = heads / kv_heads;
   long long rows = 0, tiles = 0, weight = 0;
-  int min_prefix = 0x7fffffff, max_prefix = 0;
+  int max_prefix = 0;
   // A group of one row shares nothing: its row runs on its own pages.  The
   // prefix is cut to whole steps of 16 tokens of the products; the tokens
   // behind the cut count as each row's own.
@@ -1525,7 +1527,6 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
     if (group_rows[g] < 0 || prefix_lens[g] < 0) return bad(10, "plan: negative group size or prefix");
     rows += group_rows[g];
     const int p = prefix_of(g);
-    if (group_rows[g] > 0 && p < min_prefix) min_prefix = p;
     if (p > max_prefix) max_prefix = p;
     if (p == 0) continue;
     const long long nq = static_cast<long long>(group_rows[g]) * ratio, nt = (p + TN - 1) / TN;
@@ -1536,7 +1537,6 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
   }
   if (rows < 1 || rows > 65535) return bad(10, "plan: rows outside [1, 65535]");
   if (tiles > (1 << 20)) return bad(10, "plan: over 2^20 query tiles");
-  if (min_prefix == 0x7fffffff) min_prefix = 0;
   // Two ways to share the token tiles out, by weight (a dual tile's products
   // count twice): every query tile cut into equal parts, one part per CTA; or
   // contiguous shares of all of them, where a CTA's share may end in the next
@@ -1641,7 +1641,7 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
   const int head[QWEN_PREFIX_HEADER] = {PLAN_MAGIC, static_cast<int>(rows), groups, ctas, nseg, ntile, heads, kv_heads,
                                         static_cast<int>(o_cta), static_cast<int>(o_seg), static_cast<int>(o_tile),
                                         static_cast<int>(o_row), static_cast<int>(o_err), static_cast<int>(total),
-                                        min_prefix, max_prefix};
+                                        max_prefix, 0};
   for (int i = 0; i < QWEN_PREFIX_HEADER; ++i) words[i] = head[i];
   return static_cast<int>(total);
 }
