@@ -296,41 +296,11 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// NaN if any is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// 2^x of two values on the FMA pipe: x = n + f with n the nearest integer
-// (added and taken off again at 1.5 x 2^23), 2^f by a polynomial of degree 4
-// fitted to it over [-1/2, 1/2] with equal relative errors (2.7e-6 in fp32, a
-// ninetieth of an fp16 half step), n added to the exponent.  Below -126 it
-// gives 2^-126.  The special function unit makes 16 results a clock and SM,
-// which alone would take as long as the tile's products; kPolyOf8 of eight
-// pairs go this way instead.
-constexpr int kPolyOf8 = 0;
-__device__ __forceinline__ void exp2_poly2(uint64_t x2, float &a, float &b) {
-  float x, y;
-  unpair2(x2, x, y);
-  x = fmaxf(x, -126.f);
-  y = fmaxf(y, -126.f);
-  x2 = pair2(x, y);
-  const uint64_t big = pair2(12582912.f, 12582912.f);
-  const uint64_t t2 = add2(x2, big);
-  const uint64_t n2 = add2(t2, pair2(-12582912.f, -12582912.f));
-  const uint64_t f2 = fma2(n2, pair2(-1.f, -1.f), x2);
-  uint64_t p = fma2(f2, pair2(0.009570102207362652f, 0.009570102207362652f), pair2(0.05591786280274391f, 0.05591786280274391f));
-  p = fma2(p, f2, pair2(0.240247443318367f, 0.240247443318367f));
-  p = fma2(p, f2, pair2(0.6931217908859253f, 0.6931217908859253f));
-  p = fma2(p, f2, pair2(0.9999992847442627f, 0.9999992847442627f));
-  float t, u;
-  unpair2(p, a, b);
-  unpair2(t2, t, u);
-  a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(t) << 23));
-  b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(u) << 23));
-}
-
 // Instruction descriptor of kind::f16: fp32 accumulator, M = 128, N = n, both
 // operands fp16 or both bf16, A K-major, B K-major or MN-major.
 template <typename T>
@@ -384,7 +354,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[2 * s], 4);
+      mbar_init(&p_full[2 * s], 5);      // four softmax warps and the tile warp
       mbar_init(&p_full[2 * s + 1], 4);
     }
     mbar_init(q_full, 8);
@@ -546,7 +516,6 @@ __global__ void __launch_bounds__(THREADS, 1)
         // Both tiles of the step are waited for while the tensor cores still
         // work on the last one.
         const int place = ring0 + v_place(dual, t, nt), stage = place % ST;
-        ok = wait_bar(&kv_full[stage], (place / ST) & 1, abort, a.err) && k_ready(i + 2);
         const uint32_t pa = tmem + S_COL + st * 128;
         const uint64_t vd = sw128_mn_desc(smem_u32(ring + stage * TILE), TN * 128);
         // Only the 16-token steps inside the prefix: what lies behind it in a
@@ -578,6 +547,29 @@ __global__ void __launch_bounds__(THREADS, 1)
     commit_elect(drained);
     wait_bar(drained, 0, abort + 1, a.err);
     __syncwarp();
+  } else if (warp == 2) {
+    // ---- tiles: waits for a step's V and the next K ahead of the MMA warp
+    int ring0 = 0, steps[2] = {0, 0};
+    bool ok = true;
+    for (int si = seg0; si < seg1 && ok; ++si) {
+      const Seg s = segment(si);
+      const bool dual = s.dual != 0;
+      const int nt = s.t1 - s.t0, n = dual ? 2 * nt : nt;
+      for (int i = 0; i < n && ok; ++i) {
+        const int pv = ring0 + v_place(dual, dual ? i >> 1 : i, nt);
+        ok = wait_bar(&kv_full[pv % ST], (pv / ST) & 1, abort, a.err);
+        if (ok && i + 2 < n) {
+          const int pk = ring0 + k_place(dual, dual ? (i + 2) >> 1 : i + 2);
+          ok = wait_bar(&kv_full[pk % ST], (pk / ST) & 1, abort, a.err);
+        }
+        // (One arrival per phase: the stream's step before has to be complete.)
+        if (ok && steps[i & 1] > 0) ok = wait_bar(&p_full[2 * (i & 1)], (steps[i & 1] - 1) & 1, abort, a.err);
+        ++steps[i & 1];
+        if (lane == 0) mbar_arrive(&p_full[2 * (i & 1)]);
+        __syncwarp();
+      }
+      ring0 += 2 * nt;
+    }
   }
   __syncwarp();
   tc_fence_before();
@@ -711,20 +703,16 @@ __global__ void __launch_bounds__(THREADS, 1)
               const int c = c0 + 2 * k;
               const uint64_t x2 = fma2(pair2(v[c >> 6][c & 63], v[c >> 6][(c & 63) + 1]), sc2, mu2);
               float x, y;
-              if (k % 8 < kPolyOf8) {
-                exp2_poly2(x2, x, y);
-              } else {
-                unpair2(x2, x, y);
-                x = ex2_approx(x);
-                y = ex2_approx(y);
-              }
+              unpair2(x2, x, y);
+              x = ex2_approx(x);
+              y = ex2_approx(y);
               sum[k & 1] = add2(sum[k & 1], pair2(x, y));
               // The weights enter the second product rounded to the input type
               // (half a step each, as the values they weigh); their sum is not.
               w[k] = Type<T>::pack(x, y);
             }
             tmem_st16(ts + c0 / 2, w);
-            if (c0 == 64) {  // announces the first half without a pause for its stores
+            if (c0 == 32) {
               tmem_wait_st();
               tc_fence_before();
               __syncwarp();
