@@ -497,6 +497,8 @@ class BatchedDecoder:
         prompts = [list(prefix) + list(s) for s in suffixes]
         if not 1 <= n <= min(self.max_rows, self.num_seqs) or any(len(p) < 1 for p in prompts):
             raise ValueError(f"{n} prompts: 1 to {min(self.max_rows, self.num_seqs)}, none of them empty")
+        if any(p >= 0 for row in self.pages.table[:n] for p in row):
+            raise ValueError(f"sequences 0..{n - 1} must hold no pages (release them first)")
         longest = max(len(p) for p in prompts) - 1 + max_tokens
         if max_tokens < 1 or longest > self.max_seq:
             raise ValueError("generation would run past max_seq")

@@ -1499,8 +1499,8 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
     return 0;
   };
   if (groups < 1 || group_rows == nullptr || prefix_lens == nullptr) return bad(13, "plan: no groups");
-  if (kv_heads < 1 || heads < kv_heads || heads % kv_heads != 0 || heads / kv_heads > 128 || kv_heads > 4096)
-    return bad(10, "plan: heads must be a multiple of kv_heads, at most 128 per kv head");
+  if (kv_heads < 1 || heads < kv_heads || heads % kv_heads != 0 || heads / kv_heads > 128 || kv_heads > 1024)
+    return bad(10, "plan: heads must be a multiple of kv_heads (at most 1024), at most 128 per kv head");
   if (max_length < 0) return bad(10, "plan: negative max_length");
   if (dim != 64 && dim != 128) return bad(10, "plan: dim 64 or 128");
   if (ctas < 1 || ctas > 4096) return bad(10, "plan: ctas outside [1, 4096]");

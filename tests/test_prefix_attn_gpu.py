@@ -30,6 +30,13 @@ CASES = [
     (F16, 128, 2, 2, 128, [4], [0], [1, 700, 2000, 128], 1),   # nothing shared: paged attention
     (F16, 128, 1, 2, 128, [3], [9000], [2100, 1, 77], 1),      # long, few rows: split over many CTAs
     (F16, 64, 1, 1, 256, [2], [512], [256, 1], 1),             # pages of two tiles
+    # Batches of over 1480 (row, kv head) pairs: one-warp CTAs for the own parts.
+    (F16, 128, 8, 2, 128, [190], [256], [1, 130, 33, 32, 64, 257], 1),
+    (BF16, 64, 8, 4, 16, [100, 90], [48, 160], [1, 95, 16, 63, 64, 65, 300], 1),
+    (F16, 128, 8, 2, 64, [25], [200], [9, 40, 70, 128], 8),    # runs of four rows
+    (BF16, 128, 4, 3, 32, [60, 1, 20], [128, 100, 64], [6, 41, 12], 5),  # runs of two, an odd row left
+    (F16, 64, 8, 16, 16, [95], [32], [3, 80], 1),              # two head tiles
+    (F16, 128, 8, 1, 128, [200], [0], [1, 2, 100], 1),         # nothing shared
 ]
 
 
@@ -104,6 +111,24 @@ def test_infinities_and_nan_stay_in_their_rows():
     c.lengths[4] = 32                                   # sees page 0 alone
     out, _ = c.run(plan)
     assert bool(torch.isnan(out[:4]).all()) and not bool(torch.isnan(out[4]).any())
+
+
+@pytest.mark.parametrize("seqs", [3, 60])                   # two-warp and one-warp CTAs
+def test_nan_of_a_later_token_stays_out_of_earlier_rows(seqs):
+    """Rows of one sequence run together; a token that only the later ones see
+    may hold anything."""
+    c = Case(BF16, 128, 8, 2, 32, [seqs], [64], [45, 60], tokens=6, seed=14)
+    plan = c.plan()
+    before, lse0 = c.run(plan)
+    last = int(c.lengths[5]) - 1                        # only row 5 of sequence 0 sees it
+    page, at = int(c.table[0, last // 32]), last % 32
+    c.v_pool[page, :, at] = math.nan
+    c.v_pool[page, :, at - 1] = math.inf
+    c.k_pool[page, :, at] = math.inf
+    out, lse = c.run(plan)
+    assert torch.equal(out[:4], before[:4]) and torch.equal(out[6:], before[6:])
+    assert torch.equal(lse[:5], lse0[:5]) and torch.equal(lse[6:], lse0[6:])
+    assert not bool(torch.isfinite(out[4]).any()) and bool(torch.isnan(out[5]).all())
 
 
 def test_scores_of_minus_infinity():

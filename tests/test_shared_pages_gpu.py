@@ -214,3 +214,6 @@ def test_refusals(weights_2l):
         bd.generate_shared([1, 2], [[], []], 5000)
     with pytest.raises(ValueError, match="none of them empty"):
         bd.generate_shared([], [[], []], 5)
+    bd.reserve(1, 3)
+    with pytest.raises(ValueError, match="hold no pages"):
+        bd.generate_shared([1, 2], [[], []], 5)
