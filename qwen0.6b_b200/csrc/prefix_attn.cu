@@ -50,8 +50,8 @@ using qb200tc::tmem_ld64;
 // ------------------------------------------------------------ plan (int32)
 // Header words, then the arrays they point at (offsets in words).
 enum PlanWord : int {
-  PW_MAGIC = 0, PW_ROWS, PW_GROUPS, PW_CTAS, PW_SEGS, PW_TILES, PW_HEADS, PW_KV_HEADS,
-  PW_CTA, PW_SEG, PW_TILE_SLOT, PW_ROW, PW_ERR, PW_WORDS, PW_MAX_PREFIX, PW_SPARE
+  PW_MAGIC = 0, PW_ROWS, PW_MIN_PREFIX, PW_CTAS, PW_SEGS, PW_TILES, PW_HEADS, PW_KV_HEADS,
+  PW_CTA, PW_SEG, PW_TILE_SLOT, PW_ROW, PW_ERR, PW_WORDS, PW_MAX_PREFIX, PW_MAX_SLOTS
 };
 constexpr int PLAN_MAGIC = 0x51503031;
 // A segment is a CTA's run of token tiles of one query tile (up to 256
@@ -103,7 +103,8 @@ struct Args {
   unsigned long long *err;
   int rows, heads, kv_heads, ratio;
   int num_pages, page_tokens, box, box_shift, num_seqs, max_pages;
-  int length_bias, own_splits, own_per, run_rows;
+  int length_bias, own_splits, run_rows;
+  int fused;           // the own kernel joins both parts and writes the output
   int after_prefix;    // the own kernel follows a prefix kernel of the same call
   float scale_log2;
 };
@@ -941,7 +942,7 @@ __device__ __forceinline__ void put_result(const Args &a, int row, int head, int
 // of rows of one sequence (draft tokens, a piece of a prompt; one row in plain
 // decoding) within a block of run_rows rows, as many as fit 8 columns of
 // (row, head): they read the same keys, and the products are 8 columns wide
-// anyway.  It takes positions [start + split * own_per, ...) of the sequence,
+// anyway.  It takes positions [start + split * per, ...) of the sequence,
 // its warps blocks of BT tokens in turn, each with its own online softmax; the
 // four join through shared memory.  Per 16 tokens, with tokens on the M side:
 //   S^T[16 tokens, 8 columns] = K Q^T, O^T[D dims, 8 columns] += V^T P^T.
@@ -999,9 +1000,9 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? 11 : 6) own_kernel(const Args
   const int max_len = __reduce_max_sync(0xffffffffu, lane < nrun ? len : -1);
   const int min_len = __reduce_min_sync(0xffffffffu, lane < nrun ? len : 0x7fffffff);
   if (max_len < 0 && threadIdx.x == 0) record(a.err, 3);
-  const int lo = my_start + split * a.own_per;
-  const int hi = split + 1 == a.own_splits ? max_len : min(max_len, lo + a.own_per);
-  const bool fused = a.own_splits == 1;
+  const int per = max(128, ((max_len - my_start + a.own_splits - 1) / a.own_splits + 15) / 16 * 16);
+  const int lo = my_start + split * per, hi = min(max_len, lo + per);
+  const bool fused = a.fused;
   // Lengths of this lane's columns 2c, 2c + 1 (0: no such column).
   int clen[2];
 #pragma unroll
@@ -1280,8 +1281,8 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? 11 : 6) own_kernel(const Args
 // time; the groups of threads that share them meet in shared memory in a fixed
 // order.  Neighbouring threads take the heads, whose prefix partials are
 // adjacent (with a CTA per head a warp's loads fell on 32 lines: 13 us behind
-// 60000 shared tokens, XX now).
-constexpr int JOIN_THREADS = 512;
+// 60000 shared tokens, 8 now).
+constexpr int JOIN_THREADS = 512;  // at most
 template <typename T, int D>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args a) {
   constexpr int Q4 = D / 4;
@@ -1289,27 +1290,25 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args a) {
   __shared__ __align__(16) float4 s_acc[JOIN_THREADS];
   const int kvh = blockIdx.x, row = blockIdx.y;
   const RowPlan rp = a.row_plan[row];
-  const int nout = a.ratio * Q4, used = min(nout, JOIN_THREADS), ng = JOIN_THREADS / used;
+  const int threads = blockDim.x, nout = a.ratio * Q4, used = min(nout, threads), ng = threads / used;
   const int grp = threadIdx.x / used;
   qb200::griddep_wait();
   qb200::griddep_launch_dependents();
   int seq;
   const int len = row_length(a, row, &seq);
   const bool shared = rp.prefix > 0 && len >= rp.prefix;
-  const int count = len - (shared ? rp.prefix : 0);
-  const int ns = count > 0 ? min(a.own_splits, (count + a.own_per - 1) / a.own_per) : 0;
   for (int x0 = 0; x0 < nout; x0 += used) {
     const int x = x0 + threadIdx.x % used, h = x % a.ratio, d4 = x / a.ratio, head = kvh * a.ratio + h;
     Joined j;
     if (grp < ng && x < nout) {
       if (shared) join_prefix<D, 8>(a, prefix_parts(a, rp, head), d4, grp, ng, j);
       const float *own = a.own + (static_cast<size_t>(row) * a.heads + head) * a.own_splits * (D + 4);
-      for (int s = grp; s < ns; s += 4 * ng) {
+      for (int s = grp; s < a.own_splits; s += 4 * ng) {  // (an idle split left m = -inf, l = 0)
         float m[4], l[4];
         float4 v[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const bool on = s + u * ng < ns;
+          const bool on = s + u * ng < a.own_splits;
           const float *p = own + static_cast<size_t>(on ? s + u * ng : 0) * (D + 4);
           m[u] = on ? p[D] : -INFINITY;
           l[u] = on ? p[D + 1] : 0.f;
@@ -1358,24 +1357,18 @@ bool al16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 constexpr int MAX_SPLITS = 64;
 
 // Splits of a row's own part: enough CTAs for a few per SM when the batch is
-// small, at least 128 tokens each.
-int own_splits(int rows, int kv_heads, int ratio, int own_tokens) {
-  const long long ctas = static_cast<long long>(rows) * kv_heads * ((ratio + 7) / 8);
+// small, at least 128 tokens each (the longest row behind the longest prefix
+// is the usual own part), and no more than about 4096 tokens in any case (the
+// longest row behind the shortest prefix).
+int plan_splits(const int *h, int max_length) {
+  const int ratio = h[PW_HEADS] / h[PW_KV_HEADS];
+  const long long ctas = static_cast<long long>(h[PW_ROWS]) * h[PW_KV_HEADS] * ((ratio + 7) / 8);
+  const long long usual = max_length - h[PW_MAX_PREFIX], longest = max_length - h[PW_MIN_PREFIX];
   long long s = (592 + ctas - 1) / ctas;
-  const long long most = (own_tokens + 127) / 128;
-  if (s > most) s = most;
+  if (s > (usual + 127) / 128) s = (usual + 127) / 128;
+  if (s < longest / 4096) s = longest / 4096;
   if (s > MAX_SPLITS) s = MAX_SPLITS;
   return s < 1 ? 1 : static_cast<int>(s);
-}
-
-// The longest own part expected: the longest row behind the longest prefix.
-int own_tokens(const int *h, int max_length) { return max_length > h[PW_MAX_PREFIX] ? max_length - h[PW_MAX_PREFIX] : 1; }
-
-// Tokens of one split (the last one takes whatever is left of a row).
-int own_part(int own, int splits) { return ((own + splits - 1) / splits + 127) / 128 * 128; }
-
-int plan_splits(const int *h, int max_length) {
-  return own_splits(h[PW_ROWS], h[PW_KV_HEADS], h[PW_HEADS] / h[PW_KV_HEADS], own_tokens(h, max_length));
 }
 
 long long up256(long long b) { return (b + 255) / 256 * 256; }
@@ -1448,8 +1441,12 @@ int launch(const QwenPrefixAttention &u, const Args &a, const CUtensorMap &mk, c
   cudaError_t e = own_warps(a) == 1 ? qb200_launch(own_kernel<T, D, 1>, grid, dim3(32), 0, st, true, a)
                                     : qb200_launch(own_kernel<T, D, 2>, grid, dim3(64), 0, st, true, a);
   if (e != cudaSuccess) return fail(20, "own attention launch: %s", cudaGetErrorString(e));
-  if (a.own_splits == 1) return 0;  // the own kernel has joined both parts
-  e = qb200_launch(join_kernel<T, D>, dim3(a.kv_heads, a.rows), dim3(JOIN_THREADS), 0, st, true, a);
+  if (a.fused) return 0;
+  // Threads for eight partial results each.
+  const int parts = h[PW_MAX_SLOTS] > a.own_splits ? h[PW_MAX_SLOTS] : a.own_splits;
+  int threads = (a.ratio * (D / 4) * ((parts + 7) / 8) + 31) / 32 * 32;
+  if (threads > JOIN_THREADS) threads = JOIN_THREADS;
+  e = qb200_launch(join_kernel<T, D>, dim3(a.kv_heads, a.rows), dim3(threads), 0, st, true, a);
   if (e != cudaSuccess) return fail(20, "attention join launch: %s", cudaGetErrorString(e));
   return 0;
 }
@@ -1506,16 +1503,18 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
   if (ctas < 1 || ctas > 4096) return bad(10, "plan: ctas outside [1, 4096]");
   const int ratio = heads / kv_heads;
   long long rows = 0, tiles = 0, weight = 0;
-  int max_prefix = 0;
-  // A group of one row shares nothing: its row runs on its own pages.  The
-  // prefix is cut to whole steps of 16 tokens of the products; the tokens
-  // behind the cut count as each row's own.
-  const auto prefix_of = [&](int g) { return group_rows[g] > 1 ? prefix_lens[g] / 16 * 16 : 0; };
+  int min_prefix = 0x7fffffff, max_prefix = 0;
+  // A group of one row shares nothing, but a long prefix is better spread over
+  // the SMs here than in the own kernel.  The prefix is cut to whole steps of
+  // 16 tokens of the products; the tokens behind the cut count as each row's
+  // own.
+  const auto prefix_of = [&](int g) { return group_rows[g] > 1 || prefix_lens[g] >= 1024 ? prefix_lens[g] / 16 * 16 : 0; };
   for (int g = 0; g < groups; ++g) {
     if (group_rows[g] < 0 || prefix_lens[g] < 0) return bad(10, "plan: negative group size or prefix");
     rows += group_rows[g];
     const int p = prefix_of(g);
     if (p > max_prefix) max_prefix = p;
+    if (group_rows[g] > 0 && p < min_prefix) min_prefix = p;
     if (p == 0) continue;
     const long long nq = static_cast<long long>(group_rows[g]) * ratio, nt = (p + TN - 1) / TN;
     if (nq > (1ll << 24)) return bad(10, "plan: a group of over 2^24 queries");
@@ -1626,10 +1625,15 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
     cp[c].seg1 = c + 1 < ctas ? cp[c + 1].seg0 : nseg;
     if (cp[c].seg0 < cp[c].seg1) cp[c].first = segs[cp[c].seg0];
   }
-  const int head[QWEN_PREFIX_HEADER] = {PLAN_MAGIC, static_cast<int>(rows), groups, ctas, nseg, ntile, heads, kv_heads,
+  int max_slots = 0;
+  for (int t = 0; t < ntile; ++t) {
+    const int n = words[o_tile + t + 1] - words[o_tile + t];
+    if (n > max_slots) max_slots = n;
+  }
+  const int head[QWEN_PREFIX_HEADER] = {PLAN_MAGIC, static_cast<int>(rows), min_prefix, ctas, nseg, ntile, heads, kv_heads,
                                         static_cast<int>(o_cta), static_cast<int>(o_seg), static_cast<int>(o_tile),
                                         static_cast<int>(o_row), static_cast<int>(o_err), static_cast<int>(total),
-                                        max_prefix, 0};
+                                        max_prefix, max_slots};
   for (int i = 0; i < QWEN_PREFIX_HEADER; ++i) words[i] = head[i];
   return static_cast<int>(total);
 }
@@ -1679,9 +1683,14 @@ int qwen_b200_prefix_attention(const QwenPrefixAttention *u, void *stream) {
   a.max_pages = u->max_pages;
   a.length_bias = u->length_bias;
   a.own_splits = plan_splits(h, u->max_length);
-  a.own_per = own_part(own_tokens(h, u->max_length), a.own_splits);
   a.run_rows = a.ratio >= 8 ? 1 : 8 / a.ratio;
   a.after_prefix = h[PW_SEGS] > 0;
+  // The own kernel's threads take a column's four dims at a time and join
+  // their prefix partials in rounds of a memory latency each; the join kernel
+  // spreads them further but costs about 8 us.
+  const int nt = 32 * own_warps(a), cols = a.ratio < 8 ? a.run_rows * a.ratio : 8, unroll = nt == 32 ? 8 : 4;
+  const int rounds = (cols * u->dim / 4 + nt - 1) / nt * ((h[PW_MAX_SLOTS] + unroll - 1) / unroll);
+  a.fused = a.own_splits == 1 && rounds <= 8;
   a.scale_log2 = u->scale * 1.4426950408889634f;
   a.box = u->page_tokens % 128 == 0 ? 128 : u->page_tokens % 64 == 0 ? 64 : u->page_tokens % 32 == 0 ? 32 : 16;
   a.box_shift = a.box == 128 ? 7 : a.box == 64 ? 6 : a.box == 32 ? 5 : 4;

@@ -216,7 +216,7 @@ def test_plans_cover_every_tile_once(seed):
             seen.add((row0, q0, h, t))
     want, row0 = 0, 0
     for m, q in zip(rows, lens):
-        q = q // 16 * 16 if m > 1 else 0
+        q = q // 16 * 16 if m > 1 or (m == 1 and q >= 1024) else 0
         want += -(-q // 128) * kv * -(-m * ratio // 256) if q else 0
         for j in range(m):
             prefix, tile0, query, queries = p["row"][row0 + j]

@@ -37,6 +37,9 @@ CASES = [
     (BF16, 128, 4, 3, 32, [60, 1, 20], [128, 100, 64], [6, 41, 12], 5),  # runs of two, an odd row left
     (F16, 64, 8, 16, 16, [95], [32], [3, 80], 1),              # two head tiles
     (F16, 128, 8, 1, 128, [200], [0], [1, 2, 100], 1),         # nothing shared
+    (F16, 128, 1, 2, 128, [1, 2, 1], [5000, 300, 1500], [20, 3], 1),     # long prefixes of single rows
+    (BF16, 128, 1, 4, 64, [40], [3000], [5, 60], 8),           # many partial results: a join of its own
+    (F16, 64, 1, 2, 32, [1, 3], [0, 64], [9500, 30, 200], 1),  # one row far longer than the others
 ]
 
 
