@@ -78,8 +78,8 @@ int qwen_b200_paged_status(uint64_t *detail);
  * q . k_t).  A row that sees nothing gives 0 and -inf.  The rows come in
  * groups: consecutive rows whose sequences hold the same tokens in their
  * first prefix_lens[g] positions.  Those are read and multiplied once for the
- * whole group, through the pages of the group's first row.  A row shorter
- * than its group's prefix runs on its own pages alone.
+ * whole group, through the pages of its first row that is as long as the
+ * prefix.  A row shorter than its group's prefix runs on its own pages alone.
  *
  * Plan of a batch's groups (host arrays; sum of group_rows = rows): fills
  * `words` (host, int32) and returns how many it wrote, which the caller

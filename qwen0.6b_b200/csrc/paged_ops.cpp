@@ -158,8 +158,10 @@ std::tuple<Tensor, std::optional<Tensor>> prefix_attention(
     out = *out_;
     TORCH_CHECK_VALUE(out.sizes() == q.sizes() && out.scalar_type() == type && out.device() == q.device(),
                       "out must have q's shape, type and device");
-    for (int d = 0; d < 2; ++d)
-      TORCH_CHECK_VALUE(out.size(d) == 1 || out.stride(d) >= dim, "out's rows or heads overlap");
+    // One of rows and heads lies within a step of the other.
+    const int64_t sr = out.size(0) > 1 ? out.stride(0) : 1ll << 60, sh = out.size(1) > 1 ? out.stride(1) : 1ll << 60;
+    const int64_t inner = sr < sh ? sr : sh, n = sr < sh ? out.size(0) : out.size(1);
+    TORCH_CHECK_VALUE(inner >= dim && (sr < sh ? sh : sr) >= inner * (n - 1) + dim, "out's rows or heads overlap");
   } else {
     out = torch::empty({rows, heads, dim}, q.options());
   }

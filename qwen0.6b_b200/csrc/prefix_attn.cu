@@ -12,7 +12,7 @@
 //                   read once per group: tcgen05, 128 or 256 queries per CTA;
 //   own_kernel      each row's own part, a few hundred tokens read by that
 //                   row alone: bound by their bytes, mma.sync on fragments
-//                   loaded straight from global memory;
+//                   of asynchronous copies in shared memory;
 //   join_kernel     the partial (m, l, a) of both, summed in a fixed order.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -78,7 +78,7 @@ struct RowPlan {
 
 constexpr int TN = 128;      // tokens of a tile
 constexpr int QT = 128;      // queries of a stream's tile
-constexpr int THREADS = 384; // 3 warpgroups: TMA and MMA warps (two idle), two streams of four softmax warps
+constexpr int THREADS = 384; // 3 warpgroups: copy, MMA and tile warps (one idle), two streams of four softmax warps
 // Registers after the split of the block's 384 x 168: the softmax warps hold a
 // query's 128 scores each, and with the shared memory taken by tiles there is
 // no L1 to spill to (a spilled value comes back from L2).
@@ -393,9 +393,14 @@ __global__ void __launch_bounds__(THREADS, 1)
     *bad = true;
     return a.num_pages;
   };
+  // The prefix's pages: those of the group's first row that holds all of it
+  // (rows ahead of it may be padding); null when none does, and then nobody
+  // reads what the segment leaves.
   auto table_row = [&](const Seg &s) -> const int * {
-    const int seq = a.seq_ids[s.row0];
-    return seq >= 0 && seq < a.num_seqs ? a.page_table + seq * a.table_pitch : nullptr;
+    int r = s.row0, seq;
+    while (row_length(a, r, &seq) < s.prefix)
+      if ((++r - s.row0) * a.ratio >= s.nq) return nullptr;
+    return a.page_table + seq * a.table_pitch;
   };
 
   if (warp < 4) {
@@ -416,7 +421,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       auto look = [&](int t, bool report) {
         bool bad = false;
         const int p = lane < wt * boxes ? page_of(row, s, (s.t0 + t) * boxes + lane, &bad) : a.num_pages;
-        if (bad && report && s.t0 + t + lane / boxes < s.t1) record(a.err, 3);
+        if (bad && report && row != nullptr && s.t0 + t + lane / boxes < s.t1) record(a.err, 3);
         return p;
       };
       cur[0] = cur[1] = look(0, true);
@@ -594,7 +599,6 @@ __global__ void __launch_bounds__(THREADS, 1)
       // rows past the group are zero.  A warp takes 32 rows (16 in a single
       // segment): each lane finds one row's address, then D / 8 lanes read a
       // row, eight reads of a lane in flight (all of a single segment's).
-      const int *row = table_row(s);
       {
         constexpr int CPR = D / 8, RPI = 32 / CPR;  // 16-byte chunks of a query, rows per step
         constexpr int U = 16 / RPI;                 // steps of a single segment
@@ -628,6 +632,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (lane == 0) mbar_arrive(q_full);
       }
       // Whether every page of the segment is mapped (else each tile looks).
+      const int *row = table_row(s);
       bool mapped = true;
       for (int x = s.t0 * boxes + lane; x < s.t1 * boxes; x += 32) {
         bool bad = false;
@@ -737,8 +742,9 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!ok) break;
       tc_fence_after();
       // A visible part whose scores are all -inf: the sum tells it from an
-      // empty one (the softmax of nothing but -inf is NaN).
-      if (my_steps > 0 && m == -INFINITY) l = 1.f;
+      // empty one (the softmax of nothing but -inf is NaN).  A NaN among them
+      // is in the sum already.
+      if (my_steps > 0 && m == -INFINITY && l == 0.f) l = 1.f;
       float f0 = 1.f, f1 = 0.f;
       const bool both = !dual && nt > 1;
       if (both) {
@@ -767,7 +773,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           } else {
             f0 = ex2_approx(m - mn);
             f1 = ex2_approx(m1 - mn);
-            l = (m == -INFINITY ? 0.f : l * f0) + (m1 == -INFINITY ? 0.f : l1 * f1);
+            l = l * f0 + l1 * f1;  // (f = 0 for a stream without a finite score)
           }
           m = mn;
         }
@@ -858,9 +864,9 @@ __device__ __forceinline__ void load_matrices(uint32_t (&r)[4], const void *p) {
 struct Joined {
   float m = -INFINITY, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float none = 0.f;  // visible parts whose scores are all -inf
+  float none = 0.f;  // visible parts without a finite maximum: all scores -inf, or NaN in the sum
   __device__ __forceinline__ void add(float mi, float li, const float4 &v) {
-    if (mi == -INFINITY) {
+    if (!(mi > -INFINITY)) {
       none += li;
       return;
     }
@@ -923,9 +929,10 @@ template <typename T>
 __device__ __forceinline__ void put_result(const Args &a, int row, int head, int d4, const Joined &j) {
   float lse = -INFINITY;
   float4 o;
-  if (j.m == -INFINITY) {  // nothing seen: 0; nothing but -inf: NaN
-    const float x = j.none > 0.f ? __int_as_float(0x7fffffff) : 0.f;
+  if (j.m == -INFINITY || j.none != j.none) {  // nothing seen: 0; nothing but -inf, or a NaN: NaN
+    const float x = j.none == 0.f ? 0.f : __int_as_float(0x7fffffff);
     o = make_float4(x, x, x, x);
+    if (j.none != j.none) lse = x;
   } else {
     const float inv = 1.f / j.l;
     o = make_float4(j.acc.x * inv, j.acc.y * inv, j.acc.z * inv, j.acc.w * inv);
@@ -1235,7 +1242,7 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? 11 : 6) own_kernel(const Args
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 8);
     l[h] += __shfl_xor_sync(0xffffffffu, l[h], 16);
     // Seen tokens whose scores are all -inf: as in the prefix kernel.
-    if (m[h] == -INFINITY) l[h] = seen[h] ? 1.f : 0.f;
+    if (m[h] == -INFINITY && l[h] == 0.f) l[h] = seen[h] ? 1.f : 0.f;
     if (g == 0) {
       s_m[warp][2 * c + h] = m[h];
       s_l[warp][2 * c + h] = l[h];
@@ -1270,7 +1277,7 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? 11 : 6) own_kernel(const Args
       *reinterpret_cast<float4 *>(part + 4 * d4) = j.acc;
       if (d4 == 0) {
         part[D] = j.m;
-        part[D + 1] = j.m == -INFINITY ? j.none : j.l;
+        part[D + 1] = j.m == -INFINITY ? j.none : j.l + 0.f * j.none;  // (a NaN stays)
       }
     }
   }

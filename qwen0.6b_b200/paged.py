@@ -15,6 +15,7 @@ allocates; every kernel lives in ``libqwen_b200.so``.
 from __future__ import annotations
 
 import ctypes
+import operator
 import os
 import sys
 
@@ -68,8 +69,11 @@ def _host_list(values, name: str) -> torch.Tensor:
     """A sequence of integers as an int32 tensor on the host; a tensor as it is (the extension checks it)."""
     if type(values) is torch.Tensor:
         return values
-    values = list(values)
-    if any(not -2**31 <= v < 2**31 for v in values):
+    try:
+        values = [operator.index(v) for v in values]
+    except TypeError as e:
+        raise ValueError(f"{name} must be a one-dimensional list of integers") from e
+    if values and not (min(values) >= -2**31 and max(values) < 2**31):
         raise ValueError(f"{name} holds a value outside 32 bits")
     return torch.tensor(values, dtype=torch.int32)
 
@@ -132,8 +136,8 @@ class PrefixPlan:
 
     def __init__(self, group_rows, prefix_lens, num_q_heads: int, num_kv_heads: int, head_dim: int, max_length: int,
                  device=None):
-        rows = torch.as_tensor(_host_list(group_rows, "group_rows"), dtype=torch.int32, device="cpu").contiguous()
-        lens = torch.as_tensor(_host_list(prefix_lens, "prefix_lens"), dtype=torch.int32, device="cpu").contiguous()
+        rows, lens = (_host_list(v.tolist() if isinstance(v, torch.Tensor) else v, name)
+                      for v, name in ((group_rows, "group_rows"), (prefix_lens, "prefix_lens")))
         if lens.numel() != rows.numel():
             raise ValueError(f"prefix_lens has {lens.numel()} entries, group_rows {rows.numel()}")
         if head_dim not in (64, 128):
@@ -189,9 +193,9 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     k_pool, v_pool [num_pages, kv heads, page_tokens, dim], any strides that are
     multiples of 8 elements (e.g. ``pool[:, layer]``), page_tokens a multiple
     of 16; page_table int32 [num_seqs, max_pages]; seq_ids, lengths int32
-    [rows].  The pages of a group's prefix are those of its first row's
-    sequence; a row shorter than its group's prefix runs on its own pages.  A
-    row of length 0 gives 0 (lse -inf).  scale defaults to dim ** -0.5.
+    [rows].  The pages of a group's prefix are those of its first row that is
+    as long as the prefix; a row shorter than that runs on its own pages.  A
+    row of length 0 gives 0 (lse -inf; with seq_id 0 a padding row).  scale defaults to dim ** -0.5.
 
     Returns out [rows, q heads, dim], with return_lse also the natural
     logarithm of each softmax sum, fp32 [rows, q heads].  A sequence, length or

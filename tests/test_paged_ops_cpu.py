@@ -178,6 +178,14 @@ def test_python_refusals_without_a_gpu():
         paged.PrefixPlan([2, 1], [16], 4, 2, 64, max_length=32)
     with pytest.raises(ValueError, match="32 bits"):
         paged._host_list([1 << 40], "x")
+    for bad in ([1.5], [[1, 2]], [torch.tensor([1, 2])]):
+        with pytest.raises(ValueError, match="list of integers"):
+            paged._host_list(bad, "x")
+    with pytest.raises(ValueError, match="32 bits"):
+        paged.PrefixPlan([2], torch.tensor([(1 << 32) + 16]), 4, 2, 64, max_length=32)
+    with pytest.raises(ValueError, match="list of integers"):
+        paged.PrefixPlan(torch.tensor([2.5]), [16], 4, 2, 64, max_length=32)
+    assert paged._host_list((), "x").numel() == 0
 
 
 def _plan(rows, lens, heads, kv, longest, ctas):

@@ -146,6 +146,66 @@ def test_scores_of_minus_infinity():
     assert bool(torch.isnan(out).all())
 
 
+@pytest.mark.parametrize("dtype,own", [(F16, [1, 70, 1]), (BF16, [300, 1, 30])])
+def test_a_visible_nan_reaches_its_row(dtype, own):
+    """Also where it is the only token of a part, whose other parts are finite."""
+    c = Case(dtype, 128, 2, 2, 32, [3], [160], own, seed=15)
+    plan = c.plan()
+    good, lse0 = c.run(plan)
+    r = own.index(1)
+    at = int(c.lengths[r]) - 1
+    page, at = int(c.table[r, at // 32]), at % 32
+    k = c.k_pool[page, :, at].clone()
+    c.k_pool[page, :, at] = math.nan                    # the row's one own token
+    out, lse = c.run(plan)
+    keep = [i for i in range(3) if i != r]
+    assert torch.equal(out[keep], good[keep]) and torch.equal(lse[keep], lse0[keep])
+    assert bool(torch.isnan(out[r]).all()) and bool(torch.isnan(lse[r]).all())
+    c.k_pool[page, :, at] = k
+    for x in c.table[0, :4].long().tolist():            # the first tile of the shared part
+        c.k_pool[x] = math.nan
+    out, lse = c.run(plan)
+    assert bool(torch.isnan(out).all()) and bool(torch.isnan(lse).all())
+
+
+@pytest.mark.parametrize("ahead", [1, 40])
+def test_padding_ahead_of_a_group(ahead):
+    """Rows of length 0, of no sequence or too short to hold the prefix, in
+    front of the rows whose pages are the group's."""
+    c = Case(F16, 128, 2, 2, 32, [ahead + 3], [300], [20, 70], seed=16)
+    plan = c.plan()
+    want, lse0 = c.run(plan)
+    c.lengths[:ahead] = torch.tensor([0, 5, 299], dtype=torch.int32, device="cuda").repeat(ahead)[:ahead]
+    c.table[0] = -1                                     # released
+    c.lengths[0] = 0
+    out, lse = c.run(plan)
+    assert torch.equal(out[ahead:], want[ahead:]) and torch.equal(lse[ahead:], lse0[ahead:])
+    assert bool((out[0] == 0).all()) and plan.status() == 0
+    c.check(out, lse)
+    c.seq_ids[0] = -1
+    again, _ = c.run(plan)
+    assert plan.status() == 3 and torch.equal(again, out)
+
+
+def test_rows_of_the_output_that_overlap_are_refused():
+    c = Case(F16, 128, 2, 2, 32, [3], [64], [5], seed=17)
+    plan = c.plan()
+    flat = torch.empty(3 * 4 * 128, dtype=F16, device="cuda")
+    for strides in [(128, 128, 1), (384, 128, 1), (128, 256, 1), (64, 192, 1), (512, 0, 1), (0, 128, 1)]:
+        with pytest.raises(ValueError, match="overlap"):
+            c.run(plan, out=flat.as_strided((3, 4, 128), strides))
+    c.check(*c.run(plan, out=flat.as_strided((3, 4, 128), (128, 384, 1))))   # heads outermost
+    c.check(*c.run(plan, out=c.q.clone()))
+
+
+def test_output_in_place_of_the_queries():
+    c = Case(BF16, 128, 4, 2, 64, [30, 5], [300, 64], [5, 90], seed=18)
+    plan = c.plan()
+    want, lse0 = c.run(plan)
+    out, lse = c.run(plan, out=c.q)
+    assert out.data_ptr() == c.q.data_ptr() and torch.equal(out, want) and torch.equal(lse, lse0)
+
+
 def test_bad_table_entries_are_skipped_and_recorded():
     c = Case(F16, 128, 2, 2, 32, [4], [128], [40], seed=11)
     plan = c.plan()
