@@ -126,23 +126,34 @@ class PagePool:
 
     def reserve(self, seq: int, upto_position: int) -> bool:
         """Maps pages for positions 0..upto_position; True if the row changed."""
-        need = upto_position // PAGE + 1
-        if not 0 <= seq < self.num_seqs or not 0 <= upto_position or need > self.max_pages:
-            raise ValueError(f"sequence {seq} / position {upto_position} outside the page table")
-        row = self.table[seq]
-        missing = [i for i in range(need) if row[i] < 0]
+        missing, row = self._missing(seq, upto_position), self.table[seq]
         self._enough(len(missing))
         for i in missing:
             row[i] = self._take()
         return bool(missing)
+
+    def _missing(self, seq: int, upto_position: int) -> list[int]:
+        need = upto_position // PAGE + 1
+        if not 0 <= seq < self.num_seqs or not 0 <= upto_position or need > self.max_pages:
+            raise ValueError(f"sequence {seq} / position {upto_position} outside the page table")
+        row = self.table[seq]
+        return [i for i in range(need) if row[i] < 0]
+
+    def _shared(self, seq: int, write_from: int, upto_position: int) -> list[int]:
+        row = self.table[seq]
+        return [i for i in range(write_from // PAGE, upto_position // PAGE + 1) if row[i] >= 0 and self.refs[row[i]] > 1]
+
+    def claim(self, seq: int, write_from: int, upto_position: int) -> tuple[bool, list[tuple[int, int, int]]]:
+        """reserve and unshare, both or (when the pool is exhausted) neither."""
+        self._enough(len(self._missing(seq, upto_position)) + len(self._shared(seq, write_from, upto_position)))
+        return self.reserve(seq, upto_position), self.unshare(seq, write_from, upto_position)
 
     def unshare(self, seq: int, write_from: int, upto_position: int) -> list[tuple[int, int, int]]:
         """Gives sequence `seq` pages of its own for the positions
         write_from..upto_position, which are about to be written, where it
         shares them with another one: (source, destination, tokens to copy) of
         each; the tokens before write_from stay, those behind it are dropped."""
-        row = self.table[seq]
-        shared = [i for i in range(write_from // PAGE, upto_position // PAGE + 1) if row[i] >= 0 and self.refs[row[i]] > 1]
+        row, shared = self.table[seq], self._shared(seq, write_from, upto_position)
         self._enough(len(shared))
         moves = []
         for i in shared:
@@ -305,8 +316,7 @@ class BatchedDecoder:
         write_from = upto_position if write_from is None else write_from
         if not 0 <= write_from <= upto_position:
             raise ValueError(f"write_from {write_from} outside [0, {upto_position}]")
-        changed = self.pages.reserve(seq, upto_position)
-        moves = self.pages.unshare(seq, write_from, upto_position)
+        changed, moves = self.pages.claim(seq, write_from, upto_position)
         if any(t for _, _, t in moves):
             copy_pages(self.k_pool, self.v_pool, *zip(*moves))
         if changed or moves:
@@ -317,7 +327,8 @@ class BatchedDecoder:
         pool, once no other sequence holds it (paged pools)."""
         if not self.paged:
             return
-        seqs = [seq] if isinstance(seq, int) else list(seq)
+        seqs = [seq] if hasattr(seq, "__index__") and not getattr(seq, "ndim", 0) else list(seq)
+        seqs = [range(self.num_seqs)[s] for s in seqs]  # what lies outside is refused before anything changes
         for s in seqs:
             self.pages.release(s)
         free_pages(self.page_table, seqs)
@@ -525,4 +536,6 @@ class BatchedDecoder:
             tok = self.step(ids, pos, tok, longest - 1, out=torch.empty(n, **dev), sampling=sampling, prefix=steps)
             outs.append(tok)
             pos = pos + 1
+        if code := steps.status():
+            raise RuntimeError(f"shared-prefix attention has recorded error {code}")
         return torch.stack(outs, 1).cpu().tolist()

@@ -57,6 +57,18 @@ def test_unshare_before_a_write():
     _consistent(pp)
 
 
+def test_claim_changes_nothing_when_the_pool_is_exhausted():
+    pp = PagePool(num_pages=3, num_seqs=2, max_pages=3)
+    pp.reserve(0, 2 * PAGE - 1)
+    pp.fork(0, [1], 2 * PAGE)
+    with pytest.raises(RuntimeError, match="exhausted"):
+        pp.claim(1, 2 * PAGE - 1, 2 * PAGE)                      # a page of its own and a new one; one is free
+    assert pp.table[1] == [0, 1, -1] and pp.in_use == 2
+    _consistent(pp)
+    assert pp.claim(1, 2 * PAGE, 2 * PAGE) == (True, []) and pp.table[1] == [0, 1, 2]
+    _consistent(pp)
+
+
 def test_shared_pages_are_freed_with_their_last_holder():
     pp = PagePool(num_pages=4, num_seqs=3, max_pages=2)
     pp.reserve(0, PAGE - 1)

@@ -131,6 +131,20 @@ def test_compaction_moves_what_is_in_use(weights_2l):
     assert bd.pages.table[0][0] == used                # the first free page
 
 
+def test_release_refuses_before_it_changes_anything(weights_2l):
+    bd = _decoder(weights_2l)
+    bd.reserve(1, 200)
+    for bad in ([1, 6], [1, -7], 6):
+        with pytest.raises(IndexError):
+            bd.release(bad)
+        assert bd.pages_in_use == 2 and bd.page_table.cpu().tolist() == bd.pages.table
+    bd.release(torch.tensor([1, 1]))
+    assert bd.pages_in_use == 0 and int(bd.page_table.max()) == -1
+    bd.reserve(5, 0)
+    bd.release(-1)                                     # as an index of a list
+    assert bd.pages_in_use == 0 and int(bd.page_table.max()) == -1
+
+
 @pytest.mark.parametrize("sampled", [False, True])
 def test_generate_shared(weights_2l, sampled):
     """Completions of one prompt and of prompts that begin alike: the greedy
