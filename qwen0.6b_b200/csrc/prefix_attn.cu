@@ -1418,9 +1418,16 @@ int encode_pool(CUtensorMap *m, const QwenPrefixAttention &a, const void *pool, 
   return 0;
 }
 
-// Warps of an own CTA.
-int own_warps(const Args &a) {
-  return static_cast<long long>(a.rows) * a.kv_heads * ((a.ratio + 7) / 8) * a.own_splits >= 1480 ? 1 : 2;
+// Warps of an own CTA.  An SM holds eleven one-warp CTAs or six of two warps,
+// which take half as long.  One warp for large batches (256 rows behind 2048
+// tokens: 43 us, two warps 50), and where the SMs that the prefix kernel
+// leaves hold all CTAs of one warp at once but not all of two (128 rows of 128
+// own tokens behind 512: 15.8 us, two warps 20.7; 160 rows of 500 behind 2048,
+// which they do not hold: 66 and 58).
+int own_warps(const Args &a, const int *h) {
+  const long long ctas = static_cast<long long>(a.rows) * a.kv_heads * ((a.ratio + 7) / 8) * a.own_splits;
+  const long long sms = 148 - (h[PW_SEGS] > 0 ? h[PW_CTAS] : 0);
+  return ctas >= 1480 || (ctas > 6 * sms && ctas <= 11 * sms) ? 1 : 2;
 }
 
 template <typename T, int D>
@@ -1445,7 +1452,7 @@ int launch(const QwenPrefixAttention &u, const Args &a, const CUtensorMap &mk, c
     if (e != cudaSuccess) return fail(20, "prefix attention launch: %s", cudaGetErrorString(e));
   }
   const dim3 grid(a.own_splits, a.kv_heads * ((a.ratio + 7) / 8), a.rows);
-  cudaError_t e = own_warps(a) == 1 ? qb200_launch(own_kernel<T, D, 1>, grid, dim3(32), 0, st, true, a)
+  cudaError_t e = own_warps(a, h) == 1 ? qb200_launch(own_kernel<T, D, 1>, grid, dim3(32), 0, st, true, a)
                                     : qb200_launch(own_kernel<T, D, 2>, grid, dim3(64), 0, st, true, a);
   if (e != cudaSuccess) return fail(20, "own attention launch: %s", cudaGetErrorString(e));
   if (a.fused) return 0;
@@ -1552,7 +1559,19 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
     return n;
   };
   long long part = 0;  // weight of a part; 0: contiguous shares
-  if (tiles > 0 && tiles <= ctas) {
+  // A short prefix has a CTA for each of its tiles, when they are enough and a
+  // query's partial results few: with two tiles to a CTA its streams wait for
+  // one another in the end (32 rows behind 512 tokens 8.8 us, parts of two
+  // 10.7; 64 rows behind 768 10.3 and 11.4, behind 1024 13.1 and 11.5).
+  long long token_tiles = 0, partials = 0;
+  for (int g = 0; g < groups; ++g) {
+    const long long p = prefix_of(g), nq = static_cast<long long>(group_rows[g]) * ratio, nt = (p + TN - 1) / TN;
+    token_tiles += (nq + 2 * QT - 1) / (2 * QT) * kv_heads * nt;
+    partials += nq * kv_heads * nt;
+  }
+  const bool lone = token_tiles <= ctas && max_prefix <= 8 * TN && partials <= 6144;
+  if (lone) part = 1;
+  if (part == 0 && tiles > 0 && tiles <= ctas) {
     long long lo = 1, hi = 1;
     while (parts_at(2 * hi) > ctas) hi *= 2;
     while (lo < hi) {
@@ -1561,7 +1580,7 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
     }
     if (2 * lo <= (weight + ctas - 1) / ctas + kSegWeight) part = 2 * lo;
   }
-  if (part > 0) {
+  if (part > 1) {
     // The prefix kernel leaves DRAM idle, and the own kernel runs on the SMs
     // that it leaves: when the own part is the longer one, the prefix takes
     // fewer CTAs for longer, up to half of the own part's time (rows of half
@@ -1572,7 +1591,8 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
     const long long most = static_cast<long long>((0.5 * own - 8) / 1.1) / 2 * 2;
     if (most > part) part = most;
   }
-  if (part > 0) ctas = static_cast<int>(parts_at(part));
+  if (lone) ctas = token_tiles > 0 ? static_cast<int>(token_tiles) : 1;
+  else if (part > 0) ctas = static_cast<int>(parts_at(part));
   if (ctas > weight) ctas = weight > 0 ? static_cast<int>(weight) : 1;
   const long long max_segs = part > 0 ? ctas : tiles + ctas;
   const long long o_cta = QWEN_PREFIX_HEADER, o_seg = o_cta + 16ll * ctas, o_tile = o_seg + max_segs * 8,
@@ -1595,15 +1615,15 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
       const int nq = group_rows[g] * ratio, nt = (p + TN - 1) / TN;
       for (int q0 = 0; q0 < nq; q0 += 2 * QT) {
         const int dual = nq - q0 > QT ? 1 : 0, w = dual ? 2 : 1;
-        const int parts = part > 0 ? static_cast<int>((tile_weight(nq, q0 / (2 * QT), nt) + part - 1) / part) : 0;
-        const int pairs = dual ? nt : (nt + 1) / 2;  // what the parts are made of: dual tiles, or two single ones
+        const int parts = lone ? nt : part > 0 ? static_cast<int>((tile_weight(nq, q0 / (2 * QT), nt) + part - 1) / part) : 0;
+        const int pairs = dual || lone ? nt : (nt + 1) / 2;  // what the parts are made of: dual tiles, or two single ones
         for (int h = 0; h < kv_heads; ++h) {
           words[o_tile + ntile++] = nseg;
           if (part > 0) {
             for (int k = 0; k < parts; ++k) {
               int t0 = static_cast<int>(static_cast<long long>(pairs) * k / parts);
               int t1 = static_cast<int>(static_cast<long long>(pairs) * (k + 1) / parts);
-              if (!dual) {
+              if (!dual && !lone) {
                 t0 *= 2;
                 t1 = 2 * t1 < nt ? 2 * t1 : nt;
               }
@@ -1695,7 +1715,7 @@ int qwen_b200_prefix_attention(const QwenPrefixAttention *u, void *stream) {
   // The own kernel's threads take a column's four dims at a time and join
   // their prefix partials in rounds of a memory latency each; the join kernel
   // spreads them further but costs about 8 us.
-  const int nt = 32 * own_warps(a), cols = a.ratio < 8 ? a.run_rows * a.ratio : 8, unroll = nt == 32 ? 8 : 4;
+  const int nt = 32 * own_warps(a, h), cols = a.ratio < 8 ? a.run_rows * a.ratio : 8, unroll = nt == 32 ? 8 : 4;
   const int rounds = (cols * u->dim / 4 + nt - 1) / nt * ((h[PW_MAX_SLOTS] + unroll - 1) / unroll);
   a.fused = a.own_splits == 1 && rounds <= 8;
   a.scale_log2 = u->scale * 1.4426950408889634f;
