@@ -115,26 +115,27 @@ __device__ __forceinline__ void record(unsigned long long *err, uint32_t code) {
 }
 
 // Bounded wait of a whole warp; false for all its lanes when it gave up (or
-// another role already did).  The lanes may leave the loop apart and meet
-// again in the vote: what follows a wait is warp-collective (tensor memory
-// accesses, elections, named barriers, which count a warp once per group of
-// lanes that arrives).  Inline like everything in the prefix kernel: a call
-// would keep the compiler from giving its warps different register counts.
+// another role already did).  The lanes go round together, by votes: what
+// follows a wait is warp-collective (tensor memory accesses, elections, named
+// barriers).  Inline like everything in the prefix kernel: a call would keep
+// the compiler from giving its warps different register counts.
 __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile uint32_t *abort,
                                          unsigned long long *err) {
-  bool ok = mbar_try_wait(bar, parity);
-  if (!ok) {
-    const uint64_t t0 = qb200::globaltimer_ns();
-    while (!(ok = mbar_try_wait(bar, parity))) {
-      if (*abort) break;
-      if (static_cast<long long>(qb200::globaltimer_ns() - t0) > qb200tc::WAIT_NS) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const uint64_t t0 = qb200::globaltimer_ns();
+  while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+    const bool late = static_cast<long long>(qb200::globaltimer_ns() - t0) > qb200tc::WAIT_NS;
+    if (__any_sync(0xffffffffu, late)) {
+      if ((threadIdx.x & 31) == 0) {
         *abort = 1;
         record(err, 1);
-        break;
       }
+      __syncwarp();
+      return false;
     }
+    if (__any_sync(0xffffffffu, *abort != 0)) return false;
   }
-  return __all_sync(0xffffffffu, ok);
+  return true;
 }
 
 template <typename T>
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&p_full[2 * s], 5);      // four softmax warps and the tile warp
       mbar_init(&p_full[2 * s + 1], 4);
     }
-    mbar_init(q_full, 8);
+    mbar_init(q_full, 9);                // eight softmax warps and the tile warp
     mbar_init(o_full, 1);
     mbar_init(drained, 1);
     *abort = 0;
@@ -476,19 +477,13 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
     // Every issued copy lands before the CTA may exit (matters after an abort).
-    for (int p = place > ST ? place - ST : 0; p < place; ++p) {
-      const uint64_t t0 = qb200::globaltimer_ns();
-      while (!mbar_try_wait(&kv_full[p % ST], (p / ST) & 1))
-        if (static_cast<long long>(qb200::globaltimer_ns() - t0) > qb200tc::WAIT_NS) {
-          if (lane == 0) record(a.err, 1);
-          break;
-        }
-    }
+    for (int p = place > ST ? place - ST : 0; p < place; ++p)
+      wait_bar(&kv_full[p % ST], (p / ST) & 1, abort + 1, a.err);
   } else if (warp == 1) {
     // ---- MMAs
     constexpr uint32_t id_s = idesc16<T>(TN, false), id_o = idesc16<T>(D, true);
     int ring0 = 0;            // ring place of the segment's first tile
-    int steps[2] = {0, 0};    // steps of each stream so far (phases of p_full)
+    uint32_t phase = 0;       // bit st: parity of stream st's next step (phases of p_full)
     bool ok = true;
     for (int si = seg0; si < seg1 && ok; ++si) {
       const Seg s = segment(si);
@@ -497,13 +492,6 @@ __global__ void __launch_bounds__(THREADS, 1)
       ok = wait_bar(q_full, (si - seg0) & 1, abort, a.err);
       if (!ok) break;
       tc_fence_after();
-      // The K tile of step i, if there is one (a copy has nothing to do with
-      // the tensor cores' own ordering: no fence).
-      auto k_ready = [&](int i) {
-        if (i >= n) return true;
-        const int place = ring0 + k_place(dual, dual ? i >> 1 : i);
-        return wait_bar(&kv_full[place % ST], (place / ST) & 1, abort, a.err);
-      };
       auto score = [&](int i) {  // S of step i
         const int st = i & 1, stage = (ring0 + k_place(dual, dual ? i >> 1 : i)) % ST;
         const uint64_t qd = sw128_desc(smem_u32(sq + (dual ? st * QB : 0))), kd = sw128_desc(smem_u32(ring + stage * TILE));
@@ -513,14 +501,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         commit_elect(&s_full[st]);
         if (!dual || st == 1) commit_elect(&kv_empty[stage]);
       };
-      ok = k_ready(0) && k_ready(1);
-      if (!ok) break;
       score(0);
       if (n > 1) score(1);
       for (int i = 0; i < n && ok; ++i) {
         const int st = i & 1, t = dual ? i >> 1 : i;
-        // Both tiles of the step are waited for while the tensor cores still
-        // work on the last one.
         const int place = ring0 + v_place(dual, t, nt), stage = place % ST;
         const uint32_t pa = tmem + S_COL + st * 128;
         const uint64_t vd = sw128_mn_desc(smem_u32(ring + stage * TILE), TN * 128);
@@ -530,7 +514,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int ks = min(TN, s.prefix - (s.t0 + t) * TN) / 16;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          ok = ok && wait_bar(&p_full[2 * st + half], steps[st] & 1, abort, a.err);
+          ok = ok && wait_bar(&p_full[2 * st + half], (phase >> st) & 1, abort, a.err);
           if (!ok) break;
           tc_fence_after();
           if (ks >= 4 * half + 4)
@@ -540,7 +524,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               mma_ts(tmem + O_COL + st * 128, pa + 8 * k, vd + 128 * k, id_o, k != 0 || i > 1);
         }
         if (!ok) break;
-        ++steps[st];
+        phase ^= 1u << st;
         if (!dual || st == 1) commit_elect(&kv_empty[stage]);
         if (i + 2 < n) score(i + 2);
       }
@@ -554,24 +538,36 @@ __global__ void __launch_bounds__(THREADS, 1)
     wait_bar(drained, 0, abort + 1, a.err);
     __syncwarp();
   } else if (warp == 2) {
-    // ---- tiles: waits for a step's V and the next K ahead of the MMA warp
-    int ring0 = 0, steps[2] = {0, 0};
+    // ---- tiles: waits for a step's V and the next K ahead of the MMA warp,
+    // which never looks at the tiles' barriers itself.  This warp waits for
+    // every tile of the ring in the ring's order: tiles land out of order, and
+    // a wait for one phase of a barrier would pass at once while the phase
+    // before it is still open.  Nothing is multiplied, and so no place filled
+    // again, before it has arrived (a segment's first two K tiles: at q_full),
+    // so it is never a phase behind either.
+    int ring0 = 0;
+    uint32_t phase = 0, begun = 0;  // bit st: parity of its next step, whether it has had one
     bool ok = true;
     for (int si = seg0; si < seg1 && ok; ++si) {
       const Seg s = segment(si);
       const bool dual = s.dual != 0;
       const int nt = s.t1 - s.t0, n = dual ? 2 * nt : nt;
+      const auto landed = [&](int place) {
+        return wait_bar(&kv_full[(ring0 + place) % ST], ((ring0 + place) / ST) & 1, abort, a.err);
+      };
+      ok = landed(0) && (dual || n < 2 || landed(1));
+      // (One arrival per phase, here and below: the one before has to be complete.)
+      if (ok && si > seg0) ok = wait_bar(q_full, (si - seg0 - 1) & 1, abort, a.err);
+      if (ok && lane == 0) mbar_arrive(q_full);
+      __syncwarp();
       for (int i = 0; i < n && ok; ++i) {
-        const int pv = ring0 + v_place(dual, dual ? i >> 1 : i, nt);
-        ok = wait_bar(&kv_full[pv % ST], (pv / ST) & 1, abort, a.err);
-        if (ok && i + 2 < n) {
-          const int pk = ring0 + k_place(dual, dual ? (i + 2) >> 1 : i + 2);
-          ok = wait_bar(&kv_full[pk % ST], (pk / ST) & 1, abort, a.err);
-        }
-        // (One arrival per phase: the stream's step before has to be complete.)
-        if (ok && steps[i & 1] > 0) ok = wait_bar(&p_full[2 * (i & 1)], (steps[i & 1] - 1) & 1, abort, a.err);
-        ++steps[i & 1];
-        if (lane == 0) mbar_arrive(&p_full[2 * (i & 1)]);
+        ok = landed(v_place(dual, dual ? i >> 1 : i, nt)) &&
+             (i + 2 >= n || landed(k_place(dual, dual ? (i + 2) >> 1 : i + 2)));
+        const int st = i & 1;
+        if (ok && ((begun >> st) & 1)) ok = wait_bar(&p_full[2 * st], ((phase >> st) & 1) ^ 1, abort, a.err);
+        phase ^= 1u << st;
+        begun |= 1u << st;
+        if (ok && lane == 0) mbar_arrive(&p_full[2 * st]);
         __syncwarp();
       }
       ring0 += 2 * nt;

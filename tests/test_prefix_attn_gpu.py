@@ -257,6 +257,21 @@ def test_same_bits_again_other_stream_and_graph():
     c.check(*want)
 
 
+def test_tiles_that_land_out_of_order():
+    """Many CTAs that start on new rows, their pages not cached and in no order:
+    the copies of a segment's first tiles return late and out of order."""
+    c = Case(F16, 128, 4, 2, 128, [1] * 40, [2048] * 40, [5, 70], seed=19)
+    plan = c.plan()
+    want = c.run(plan)
+    c.check(*want)
+    flush = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    for i in range(100):
+        flush.fill_(i)                                  # larger than the L2
+        out, lse = c.run(plan)
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+    assert plan.status() == 0
+
+
 def test_offsets_past_32_bits():
     """A pool of over 2^31 elements: pages at its far end."""
     page, d, kv = 128, 128, 8
