@@ -223,8 +223,9 @@ def test_plans_cover_every_tile_once(seed):
             assert (row0, q0, h, t) not in seen
             seen.add((row0, q0, h, t))
     want, row0 = 0, 0
+    any_shared = any(m > 1 and q >= 16 for m, q in zip(rows, lens))
     for m, q in zip(rows, lens):
-        q = q // 16 * 16 if m > 1 or (m == 1 and q >= 1024) else 0
+        q = q // 16 * 16 if m > 1 or (m == 1 and q >= 1024 and any_shared) else 0
         want += -(-q // 128) * kv * -(-m * ratio // 256) if q else 0
         for j in range(m):
             prefix, tile0, query, queries = p["row"][row0 + j]

@@ -39,6 +39,7 @@ CASES = [
     (F16, 128, 8, 1, 128, [200], [0], [1, 2, 100], 1),         # nothing shared
     (F16, 128, 1, 2, 128, [1, 2, 1], [5000, 300, 1500], [20, 3], 1),     # long prefixes of single rows
     (BF16, 128, 1, 4, 64, [40], [3000], [5, 60], 8),           # many partial results: a join of its own
+    (F16, 128, 2, 2, 16, [1, 1, 1], [4000, 30, 1500], [20, 3, 700], 1),  # single rows alone
     (F16, 64, 1, 2, 32, [1, 3], [0, 64], [9500, 30, 200], 1),  # one row far longer than the others
 ]
 
@@ -260,7 +261,7 @@ def test_same_bits_again_other_stream_and_graph():
 def test_tiles_that_land_out_of_order():
     """Many CTAs that start on new rows, their pages not cached and in no order:
     the copies of a segment's first tiles return late and out of order."""
-    c = Case(F16, 128, 4, 2, 128, [1] * 40, [2048] * 40, [5, 70], seed=19)
+    c = Case(F16, 128, 4, 2, 128, [1] * 39 + [2], [2048] * 40, [5, 70], seed=19)
     plan = c.plan()
     want = c.run(plan)
     c.check(*want)
