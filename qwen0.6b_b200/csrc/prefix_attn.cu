@@ -115,27 +115,30 @@ __device__ __forceinline__ void record(unsigned long long *err, uint32_t code) {
 }
 
 // Bounded wait of a whole warp; false for all its lanes when it gave up (or
-// another role already did).  The lanes go round together, by votes: what
-// follows a wait is warp-collective (tensor memory accesses, elections, named
-// barriers).  Inline like everything in the prefix kernel: a call would keep
-// the compiler from giving its warps different register counts.
+// another role already did).  The lanes may leave the loop apart and meet
+// again in the vote: what follows a wait is warp-collective (tensor memory
+// accesses, elections, named barriers).  (Going round by votes costs 2 us in
+// 44.)  Inline like everything in the prefix kernel: a call would keep the
+// compiler from giving its warps different register counts.
+//
+// A wait for a phase also passes while the phase before it is open (the
+// parities say no more), so whoever waits on a barrier waits for each of its
+// phases, in order, or for something that followed from them.
 __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile uint32_t *abort,
                                          unsigned long long *err) {
-  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-  const uint64_t t0 = qb200::globaltimer_ns();
-  while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
-    const bool late = static_cast<long long>(qb200::globaltimer_ns() - t0) > qb200tc::WAIT_NS;
-    if (__any_sync(0xffffffffu, late)) {
-      if ((threadIdx.x & 31) == 0) {
+  bool ok = mbar_try_wait(bar, parity);
+  if (!ok) {
+    const uint64_t t0 = qb200::globaltimer_ns();
+    while (!(ok = mbar_try_wait(bar, parity))) {
+      if (*abort) break;
+      if (static_cast<long long>(qb200::globaltimer_ns() - t0) > qb200tc::WAIT_NS) {
         *abort = 1;
         record(err, 1);
+        break;
       }
-      __syncwarp();
-      return false;
     }
-    if (__any_sync(0xffffffffu, *abort != 0)) return false;
   }
-  return true;
+  return __all_sync(0xffffffffu, ok);
 }
 
 template <typename T>
