@@ -171,7 +171,9 @@ __device__ __forceinline__ int row_length(const Args &a, int r, int *seq) {
 }
 
 // ------------------------------------------------------------ prefix kernel
-// Floats of one slot: two streams of acc[dim / 4][128 queries][4], m[128], l[128].
+// A slot (one per segment) is two of these, a stream's acc[dim / 4][128
+// queries][4], m[128], l[128]: neighbouring queries are adjacent, in the order
+// in which a softmax warp stores and a join reads them.  Floats of one:
 template <int D>
 constexpr int kStreamFloats = QT * D + 2 * QT;
 template <int D>
@@ -331,6 +333,21 @@ __device__ __forceinline__ int v_place(bool dual, int t, int n) {
 //   S_s = Q_s K^T       tcgen05, both operands in shared memory
 //   P_s = 2^(S_s - m)   rounded to the input type over S_s in tensor memory
 //   O_s += P_s V        tcgen05, P from tensor memory, V as it lies (MN-major)
+// The maximum m moves only when a row has outgrown it by 2^8, so the output is
+// hardly ever rescaled.  Warps: 0 copies K and V tiles (a ring of five of 32
+// KB; the pages of the next 32 boxes are looked up ahead), 1 issues every
+// product, 2 waits for tiles on its behalf, 4 to 7 and 8 to 11 are the
+// streams' softmax, one query per thread.
+//
+// What bounds it: with few rows the bytes of K and V (13 rows over 60000
+// tokens, 123 MB: 28 us, 4.4 TB/s with the queries' start and the results'
+// end; the ring holds 160 KB in flight per SM).  With many rows (64 x 8 rows
+// over 30000 tokens, 126 GFLOP) the softmax: a pair of tiles takes 3650 clocks,
+// of which the tensor cores work 48 %, its 256 x 128 exponentials half of the
+// rest; 113 us, 1.1 PFLOP/s where the products alone would allow 1.66.
+// Measured against it: exponentials half by a polynomial on the FMA pipe 143
+// us in all (140), weights announced at 64 or 96 columns of 128 142, two
+// threads per query 288 (they do not fit the registers).
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, 1)
     prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Args a) {
@@ -880,10 +897,10 @@ struct Joined {
   }
 };
 
-// Partial results of the prefix for one query: count of them, and where the
-// k-th lies.
+// Partial results of the prefix for one query: the k-th lies at stream slot
+// first + 2 k (a slot holds two streams), query ql of it.
 struct PrefixParts {
-  int first, count, ql;  // first stream slot (one slot holds two), slots, query within the stream
+  int first, count, ql;
 };
 __device__ __forceinline__ PrefixParts prefix_parts(const Args &a, const RowPlan &rp, int head) {
   // (the plan is constant: this may run before the prefix kernel is done)
@@ -944,13 +961,13 @@ __device__ __forceinline__ void put_result(const Args &a, int row, int head, int
   if (d4 == 0 && a.lse != nullptr) a.lse[static_cast<size_t>(row) * a.heads + head] = lse;
 }
 
-// grid (splits, kv heads x head tiles of 8, rows), 4 warps.  A CTA takes a run
+// grid (splits, kv heads x head tiles of 8, rows), W warps.  A CTA takes a run
 // of rows of one sequence (draft tokens, a piece of a prompt; one row in plain
 // decoding) within a block of run_rows rows, as many as fit 8 columns of
 // (row, head): they read the same keys, and the products are 8 columns wide
 // anyway.  It takes positions [start + split * per, ...) of the sequence,
-// its warps blocks of BT tokens in turn, each with its own online softmax; the
-// four join through shared memory.  Per 16 tokens, with tokens on the M side:
+// its warps blocks of BT tokens in turn, each with its own online softmax; they
+// join through shared memory.  Per 16 tokens, with tokens on the M side:
 //   S^T[16 tokens, 8 columns] = K Q^T, O^T[D dims, 8 columns] += V^T P^T.
 // What bounds it are the bytes of K and V and the latency of getting at them
 // (length, page, tokens: three round trips), and, as one warp's instructions
@@ -959,7 +976,9 @@ __device__ __forceinline__ void put_result(const Args &a, int row, int head, int
 // likewise; fragments are loaded as 8 x 8 matrices, V transposed on the way
 // (its 16-byte chunks are exchanged by the token's number, so that no read has
 // bank conflicts); the maximum moves only when a column has outgrown it by 2^8,
-// as in the prefix kernel.
+// as in the prefix kernel.  Measured: 256 rows of up to 256 own tokens, 142 MB,
+// 36 us beside the prefix kernel (4 TB/s); 112 rows of 1000 with no prefix 74
+// us (6.2 TB/s, 0.95 of a copy's rate).
 // With one split the CTA also joins the prefix's partial results and writes the
 // output; else it leaves partial results to the join kernel.
 template <typename T, int D, int W>
@@ -971,7 +990,7 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? 11 : 6) own_kernel(const Args
   qb200::griddep_launch_dependents();
   constexpr int DT = D / 16;       // 16-dim steps
   constexpr int NB = (W == 1 ? 2 : 1) * 128 / D;  // 16-token steps of a block
-  constexpr int BT = 16 * NB;      // tokens of a warp's block: 8 KB of K and of V (4 KB with four warps)
+  constexpr int BT = 16 * NB;      // tokens of a warp's block: 8 KB of K and of V (4 KB with two warps)
   constexpr int CPR = D / 8;       // 16-byte chunks of a token
   constexpr int RPI = 32 / CPR;    // tokens that a warp copies at a time
   constexpr int QP = D + 8;        // pitch of a query row: the fragment reads of eight rows take all banks
@@ -1045,8 +1064,8 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? 11 : 6) own_kernel(const Args
   };
   lookup(0);
   uint32_t ready = 0;  // bit (step % 32): the page of a step that has been fetched is mapped
-  // Q^T, the B operand of the scores, on its way to shared memory: n = column,
-  // k = dims in the order of the K reads.
+  // Q^T, the B operand of the scores (n = column, k = dims), on its way to
+  // shared memory.
   constexpr int QC = (8 * CPR + NT - 1) / NT;  // 16-byte chunks per thread
   uint4 qv0[QC];
 #pragma unroll
@@ -1287,7 +1306,8 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? 11 : 6) own_kernel(const Args
 // time; the groups of threads that share them meet in shared memory in a fixed
 // order.  Neighbouring threads take the heads, whose prefix partials are
 // adjacent (with a CTA per head a warp's loads fell on 32 lines: 13 us behind
-// 60000 shared tokens, 8 now).
+// 60000 shared tokens, 8 now).  Bound by latency: the kernel's start, the own
+// partials, the plan, then one round of loads (8 us for 2 MB).
 constexpr int JOIN_THREADS = 512;  // at most
 template <typename T, int D>
 __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args a) {
