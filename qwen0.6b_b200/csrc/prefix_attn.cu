@@ -1584,17 +1584,19 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
     return n;
   };
   long long part = 0;  // weight of a part; 0: contiguous shares
-  // A short prefix has a CTA for each of its tiles, when they are enough and a
-  // query's partial results few: with two tiles to a CTA its streams wait for
-  // one another in the end (32 rows behind 512 tokens 8.8 us, parts of two
-  // 10.7; 64 rows behind 768 10.3 and 11.4, behind 1024 13.1 and 11.5).
-  long long token_tiles = 0, partials = 0;
+  // A short prefix has a CTA for each of its tiles, when the SMs that are left
+  // hold the rows' own CTAs (six to an SM) and a query's partial results are
+  // few: with two tiles to a CTA its streams wait for one another in the end
+  // (32 rows behind 512 tokens 8.8 us, parts of two 10.7; behind 1408 10.8 and
+  // 11.6; 64 rows behind 768 10.3 and 11.4, but behind 1024, where 64 CTAs are
+  // in the way of the rows' own 512, 13.1 and 11.5).
+  long long token_tiles = 0;
   for (int g = 0; g < groups; ++g) {
     const long long p = prefix_of(g), nq = static_cast<long long>(group_rows[g]) * ratio, nt = (p + TN - 1) / TN;
     token_tiles += (nq + 2 * QT - 1) / (2 * QT) * kv_heads * nt;
-    partials += nq * kv_heads * nt;
   }
-  const bool lone = token_tiles <= ctas && max_prefix <= 8 * TN && partials <= 6144;
+  const bool lone = max_prefix <= 12 * TN && token_tiles <= ctas &&
+                    rows * kv_heads * ((ratio + 7) / 8) <= 6 * (ctas - token_tiles);
   if (lone) part = 1;
   if (part == 0 && tiles > 0 && tiles <= ctas) {
     long long lo = 1, hi = 1;
@@ -1742,7 +1744,7 @@ int qwen_b200_prefix_attention(const QwenPrefixAttention *u, void *stream) {
   // spreads them further but costs about 8 us.
   const int nt = 32 * own_warps(a, h), cols = a.ratio < 8 ? a.run_rows * a.ratio : 8, unroll = nt == 32 ? 8 : 4;
   const int rounds = (cols * u->dim / 4 + nt - 1) / nt * ((h[PW_MAX_SLOTS] + unroll - 1) / unroll);
-  a.fused = a.own_splits == 1 && rounds <= 8;
+  a.fused = a.own_splits == 1 && rounds <= 12;
   a.scale_log2 = u->scale * 1.4426950408889634f;
   a.box = u->page_tokens % 128 == 0 ? 128 : u->page_tokens % 64 == 0 ? 64 : u->page_tokens % 32 == 0 ? 32 : 16;
   a.box_shift = a.box == 128 ? 7 : a.box == 64 ? 6 : a.box == 32 ? 5 : 4;
