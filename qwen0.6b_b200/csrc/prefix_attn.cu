@@ -1283,7 +1283,7 @@ __global__ void __launch_bounds__(32 * W, W == 1 ? 11 : 6) own_kernel(const Args
     if (x >= nc * Q4) continue;
     const int r = row + col / nh, head = kvh * a.ratio + h0 + col % nh;
     Joined j;
-    if (shared) join_prefix<D, W == 1 ? 8 : 4>(a, parts, d4, 0, 1, j);
+    if (shared) join_prefix<D, 8>(a, parts, d4, 0, 1, j);
 #pragma unroll
     for (int w = 0; w < W; ++w)
       j.add(s_m[w][col], s_l[w][col],
@@ -1740,11 +1740,15 @@ int qwen_b200_prefix_attention(const QwenPrefixAttention *u, void *stream) {
   a.run_rows = a.ratio >= 8 ? 1 : 8 / a.ratio;
   a.after_prefix = h[PW_SEGS] > 0;
   // The own kernel's threads take a column's four dims at a time and join
-  // their prefix partials in rounds of a memory latency each; the join kernel
-  // spreads them further but costs about 8 us.
-  const int nt = 32 * own_warps(a, h), cols = a.ratio < 8 ? a.run_rows * a.ratio : 8, unroll = nt == 32 ? 8 : 4;
-  const int rounds = (cols * u->dim / 4 + nt - 1) / nt * ((h[PW_MAX_SLOTS] + unroll - 1) / unroll);
-  a.fused = a.own_splits == 1 && rounds <= 12;
+  // their prefix partials eight at a time, in rounds of a memory latency each
+  // (counted here for CTAs of eight columns; rows of different sequences have
+  // fewer); the join kernel spreads them further but starts after it.  128
+  // rows behind 1920 tokens (16 rounds) 20.7 us, with the join kernel 26.1; 16
+  // sequences of 4 rows behind 4096 22.6 and 20.5; 64 of 8 behind 30000 144
+  // and 142.
+  const int nt = 32 * own_warps(a, h), cols = a.ratio < 8 ? a.run_rows * a.ratio : 8;
+  const int rounds = (cols * u->dim / 4 + nt - 1) / nt * ((h[PW_MAX_SLOTS] + 7) / 8);
+  a.fused = a.own_splits == 1 && rounds <= 16;
   a.scale_log2 = u->scale * 1.4426950408889634f;
   a.box = u->page_tokens % 128 == 0 ? 128 : u->page_tokens % 64 == 0 ? 64 : u->page_tokens % 32 == 0 ? 32 : 16;
   a.box_shift = a.box == 128 ? 7 : a.box == 64 ? 6 : a.box == 32 ? 5 : 4;
