@@ -981,16 +981,22 @@ __device__ __forceinline__ void put_result(const Args &a, int row, int head, int
 // us (6.2 TB/s, 0.95 of a copy's rate).
 // With one split the CTA also joins the prefix's partial results and writes the
 // output; else it leaves partial results to the join kernel.
+// CTAs on an SM: one-warp CTAs in 128 registers and blocks of 16 tokens, for as
+// many rows at once as possible (256 rows of 130 tokens 26.4 us; eleven CTAs
+// with blocks of 32 tokens 30.5); of two warps six (eight in 128 registers: 13
+// rows over 60000 47.4 us, six 45.8).
+template <int W>
+constexpr int kOwnPerSm = W == 1 ? 14 : 6;
 template <typename T, int D, int W>
-__global__ void __launch_bounds__(32 * W, W == 1 ? 11 : 6) own_kernel(const Args a) {
+__global__ void __launch_bounds__(32 * W, kOwnPerSm<W>) own_kernel(const Args a) {
   // Behind a prefix kernel of the same call nothing that this part reads is
   // new: the prefix kernel's CTAs have all passed their own wait for whatever
   // came before.  Its results are waited for where they are read, below.
   if (!a.after_prefix) qb200::griddep_wait();
   qb200::griddep_launch_dependents();
   constexpr int DT = D / 16;       // 16-dim steps
-  constexpr int NB = (W == 1 ? 2 : 1) * 128 / D;  // 16-token steps of a block
-  constexpr int BT = 16 * NB;      // tokens of a warp's block: 8 KB of K and of V (4 KB with two warps)
+  constexpr int NB = 128 / D;      // 16-token steps of a block
+  constexpr int BT = 16 * NB;      // tokens of a warp's block: 4 KB of K and of V
   constexpr int CPR = D / 8;       // 16-byte chunks of a token
   constexpr int RPI = 32 / CPR;    // tokens that a warp copies at a time
   constexpr int QP = D + 8;        // pitch of a query row: the fragment reads of eight rows take all banks
@@ -1437,16 +1443,16 @@ int encode_pool(CUtensorMap *m, const QwenPrefixAttention &a, const void *pool, 
   return 0;
 }
 
-// Warps of an own CTA.  An SM holds eleven one-warp CTAs or six of two warps,
-// which take half as long.  One warp for large batches (256 rows behind 2048
-// tokens: 43 us, two warps 50), and where the SMs that the prefix kernel
-// leaves hold all CTAs of one warp at once but not all of two (128 rows of 128
-// own tokens behind 512: 15.8 us, two warps 20.7; 160 rows of 500 behind 2048,
-// which they do not hold: 66 and 58).
+// Warps of an own CTA; those of two take half as long, but an SM holds fewer.
+// One warp for large batches (256 rows behind 2048 tokens: 43 us, two warps
+// 50), and where the SMs that the prefix kernel leaves hold all CTAs of one
+// warp at once but not all of two (128 rows of 128 own tokens behind 512: 15
+// us, two warps 20.7; 160 rows of 500 behind 2048, which they do not hold: 66
+// and 58).
 int own_warps(const Args &a, const int *h) {
   const long long ctas = static_cast<long long>(a.rows) * a.kv_heads * ((a.ratio + 7) / 8) * a.own_splits;
   const long long sms = 148 - (h[PW_SEGS] > 0 ? h[PW_CTAS] : 0);
-  return ctas >= 1480 || (ctas > 6 * sms && ctas <= 11 * sms) ? 1 : 2;
+  return ctas >= 1480 || (ctas > kOwnPerSm<2> * sms && ctas <= kOwnPerSm<1> * sms) ? 1 : 2;
 }
 
 template <typename T, int D>
@@ -1596,7 +1602,7 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
     token_tiles += (nq + 2 * QT - 1) / (2 * QT) * kv_heads * nt;
   }
   const bool lone = max_prefix <= 12 * TN && token_tiles <= ctas &&
-                    rows * kv_heads * ((ratio + 7) / 8) <= 6 * (ctas - token_tiles);
+                    rows * kv_heads * ((ratio + 7) / 8) <= kOwnPerSm<2> * (ctas - token_tiles);
   if (lone) part = 1;
   if (part == 0 && tiles > 0 && tiles <= ctas) {
     long long lo = 1, hi = 1;
