@@ -895,6 +895,31 @@ struct Joined {
     acc.w = acc.w * f + v.w * h;
     m = mn;
   }
+  // The same for U at once: their weights do not wait for one another.
+  template <int U>
+  __device__ __forceinline__ void add(const float (&mi)[U], const float (&li)[U], const float4 (&v)[U]) {
+    float mn = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) mn = fmaxf(mn, mi[u]);
+    const float f = m > -INFINITY ? ex2_approx(m - mn) : 0.f;
+    l *= f;
+    acc.x *= f;
+    acc.y *= f;
+    acc.z *= f;
+    acc.w *= f;
+    m = mn;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool on = mi[u] > -INFINITY;
+      const float h = on ? ex2_approx(mi[u] - mn) : 0.f;
+      none += on ? 0.f : li[u];
+      l += on ? li[u] * h : 0.f;
+      acc.x += on ? v[u].x * h : 0.f;
+      acc.y += on ? v[u].y * h : 0.f;
+      acc.z += on ? v[u].z * h : 0.f;
+      acc.w += on ? v[u].w * h : 0.f;
+    }
+  }
 };
 
 // Partial results of the prefix for one query: the k-th lies at stream slot
@@ -935,8 +960,7 @@ __device__ __forceinline__ void join_prefix(const Args &a, const PrefixParts &p,
         v[u] = reinterpret_cast<const float4 *>(slot)[d4 * QT + p.ql];
       }
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) j.add(m[u], l[u], v[u]);
+    j.add(m, l, v);
   }
 }
 
@@ -1346,8 +1370,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args a) {
           l[u] = on ? p[D + 1] : 0.f;
           v[u] = *reinterpret_cast<const float4 *>(p + 4 * d4);
         }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) j.add(m[u], l[u], v[u]);
+        j.add(m, l, v);
       }
     }
     if (ng > 1) {
@@ -1443,16 +1466,27 @@ int encode_pool(CUtensorMap *m, const QwenPrefixAttention &a, const void *pool, 
   return 0;
 }
 
+// Rounds of a memory latency in which the threads of an own CTA of `warps`
+// warps join the prefix's partial results: a column's four dims at a time,
+// eight partials at once (counted for CTAs of eight columns; rows of different
+// sequences have fewer).
+int join_rounds(const Args &a, const int *h, int dim, int warps) {
+  const int cols = a.ratio < 8 ? a.run_rows * a.ratio : 8;
+  return (cols * dim / 4 + 32 * warps - 1) / (32 * warps) * ((h[PW_MAX_SLOTS] + 7) / 8);
+}
+
 // Warps of an own CTA; those of two take half as long, but an SM holds fewer.
 // One warp for large batches (256 rows behind 2048 tokens: 43 us, two warps
 // 50), and where the SMs that the prefix kernel leaves hold all CTAs of one
 // warp at once but not all of two (128 rows of 128 own tokens behind 512: 15
 // us, two warps 20.7; 160 rows of 500 behind 2048, which they do not hold: 66
-// and 58).
-int own_warps(const Args &a, const int *h) {
+// and 58) and there is not much to join (8 sequences of 4 rows behind 4096, 16
+// rounds: 28.4 and 20.8).
+int own_warps(const Args &a, const int *h, int dim) {
   const long long ctas = static_cast<long long>(a.rows) * a.kv_heads * ((a.ratio + 7) / 8) * a.own_splits;
   const long long sms = 148 - (h[PW_SEGS] > 0 ? h[PW_CTAS] : 0);
-  return ctas >= 1480 || (ctas > kOwnPerSm<2> * sms && ctas <= kOwnPerSm<1> * sms) ? 1 : 2;
+  if (ctas >= 1480) return 1;
+  return ctas > kOwnPerSm<2> * sms && ctas <= kOwnPerSm<1> * sms && join_rounds(a, h, dim, 1) <= 8 ? 1 : 2;
 }
 
 template <typename T, int D>
@@ -1477,7 +1511,7 @@ int launch(const QwenPrefixAttention &u, const Args &a, const CUtensorMap &mk, c
     if (e != cudaSuccess) return fail(20, "prefix attention launch: %s", cudaGetErrorString(e));
   }
   const dim3 grid(a.own_splits, a.kv_heads * ((a.ratio + 7) / 8), a.rows);
-  cudaError_t e = own_warps(a, h) == 1 ? qb200_launch(own_kernel<T, D, 1>, grid, dim3(32), 0, st, true, a)
+  cudaError_t e = own_warps(a, h, D) == 1 ? qb200_launch(own_kernel<T, D, 1>, grid, dim3(32), 0, st, true, a)
                                     : qb200_launch(own_kernel<T, D, 2>, grid, dim3(64), 0, st, true, a);
   if (e != cudaSuccess) return fail(20, "own attention launch: %s", cudaGetErrorString(e));
   if (a.fused) return 0;
@@ -1745,16 +1779,11 @@ int qwen_b200_prefix_attention(const QwenPrefixAttention *u, void *stream) {
   a.own_splits = plan_splits(h, u->max_length);
   a.run_rows = a.ratio >= 8 ? 1 : 8 / a.ratio;
   a.after_prefix = h[PW_SEGS] > 0;
-  // The own kernel's threads take a column's four dims at a time and join
-  // their prefix partials eight at a time, in rounds of a memory latency each
-  // (counted here for CTAs of eight columns; rows of different sequences have
-  // fewer); the join kernel spreads them further but starts after it.  128
-  // rows behind 1920 tokens (16 rounds) 20.7 us, with the join kernel 26.1; 16
-  // sequences of 4 rows behind 4096 22.6 and 20.5; 64 of 8 behind 30000 144
-  // and 142.
-  const int nt = 32 * own_warps(a, h), cols = a.ratio < 8 ? a.run_rows * a.ratio : 8;
-  const int rounds = (cols * u->dim / 4 + nt - 1) / nt * ((h[PW_MAX_SLOTS] + 7) / 8);
-  a.fused = a.own_splits == 1 && rounds <= 16;
+  // The own kernel joins by itself while that takes few rounds; the join
+  // kernel spreads them further but starts after it.  128 rows behind 1920
+  // tokens (16 rounds) 20.7 us, with the join kernel 26.1; 16 sequences of 4
+  // rows behind 4096 21.7 and 20.5.
+  a.fused = a.own_splits == 1 && join_rounds(a, h, u->dim, own_warps(a, h, u->dim)) <= 16;
   a.scale_log2 = u->scale * 1.4426950408889634f;
   a.box = u->page_tokens % 128 == 0 ? 128 : u->page_tokens % 64 == 0 ? 64 : u->page_tokens % 32 == 0 ? 32 : 16;
   a.box_shift = a.box == 128 ? 7 : a.box == 64 ? 6 : a.box == 32 ? 5 : 4;
