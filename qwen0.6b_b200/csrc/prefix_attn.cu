@@ -1414,13 +1414,16 @@ constexpr int MAX_SPLITS = 64;
 // Splits of a row's own part: enough CTAs for a few per SM when the batch is
 // small, at least 128 tokens each (the longest row behind the longest prefix
 // is the usual own part), and no more than about 4096 tokens in any case (the
-// longest row behind the shortest prefix).
+// longest row behind the shortest prefix).  Up to 256 tokens are not split:
+// two splits and the join kernel take as long or longer (2 rows of 136 tokens
+// 7.9 us, unsplit 6.7; of 256 8.0 and 8.6, but 2.4 us less on the host; 8 rows
+// of 200 behind 512 13.8 and 10.3).
 int plan_splits(const int *h, int max_length) {
   const int ratio = h[PW_HEADS] / h[PW_KV_HEADS];
   const long long ctas = static_cast<long long>(h[PW_ROWS]) * h[PW_KV_HEADS] * ((ratio + 7) / 8);
   const long long usual = max_length - h[PW_MAX_PREFIX], longest = max_length - h[PW_MIN_PREFIX];
   long long s = (592 + ctas - 1) / ctas;
-  if (s > (usual + 127) / 128) s = (usual + 127) / 128;
+  if (s > (usual + 127) / 128) s = usual <= 256 ? 1 : (usual + 127) / 128;
   if (s < longest / 4096) s = longest / 4096;
   if (s > MAX_SPLITS) s = MAX_SPLITS;
   return s < 1 ? 1 : static_cast<int>(s);
@@ -1583,9 +1586,20 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
   // row's long prefix is spread over the SMs here.  The prefix is cut to whole
   // steps of 16 tokens of the products; the tokens behind the cut count as
   // each row's own.
+  // Neither does a small batch of short rows (2 rows of 136 tokens, 128 of
+  // them shared: 6.7 us in the own kernel alone, 8.5 with this one; 32 rows of
+  // 256 8.9 and 8.8, with a launch less).
   bool any_shared = false;
-  for (int g = 0; g < groups; ++g) any_shared = any_shared || (group_rows[g] > 1 && prefix_lens[g] >= 16);
+  long long all_rows = 0;
+  int longest = max_length;
+  for (int g = 0; g < groups; ++g) {
+    any_shared = any_shared || (group_rows[g] > 1 && prefix_lens[g] >= 16);
+    all_rows += group_rows[g];
+    if (prefix_lens[g] > longest) longest = prefix_lens[g];
+  }
+  const bool small = longest <= 256 && all_rows * kv_heads * ((ratio + 7) / 8) <= 2 * 148;
   const auto prefix_of = [&](int g) {
+    if (small) return 0;
     return group_rows[g] > 1 || (any_shared && prefix_lens[g] >= 1024) ? prefix_lens[g] / 16 * 16 : 0;
   };
   for (int g = 0; g < groups; ++g) {

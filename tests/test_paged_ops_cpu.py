@@ -208,7 +208,8 @@ def test_plans_cover_every_tile_once(seed):
     rows = [r.choice([0, 1, 2, 3, 17, 64, 100]) for _ in range(n)] + [3]
     lens = [r.choice([0, 1, 15, 16, 127, 128, 129, 1000, 5000]) for _ in rows]
     ctas = r.choice([1, 3, 148])
-    p = _plan(rows, lens, kv * ratio, kv, r.choice([0, 200, 6000, 60000]), ctas)
+    longest = r.choice([0, 200, 6000, 60000])
+    p = _plan(rows, lens, kv * ratio, kv, longest, ctas)
     assert p["rows"] == sum(rows) and len(p["cta"]) <= ctas
     assert [c[0] for c in p["cta"]] + [len(p["segs"])] == [0] + [c[1] for c in p["cta"]]
     for first, last, *_, in p["cta"]:
@@ -224,6 +225,8 @@ def test_plans_cover_every_tile_once(seed):
             seen.add((row0, q0, h, t))
     want, row0 = 0, 0
     any_shared = any(m > 1 and q >= 16 for m, q in zip(rows, lens))
+    if max([longest] + lens) <= 256 and sum(rows) * kv * -(-ratio // 8) <= 296:
+        lens = [0] * len(lens)                           # a small batch of short rows: all their own
     for m, q in zip(rows, lens):
         q = q // 16 * 16 if m > 1 or (m == 1 and q >= 1024 and any_shared) else 0
         want += -(-q // 128) * kv * -(-m * ratio // 256) if q else 0

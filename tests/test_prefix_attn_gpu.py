@@ -44,10 +44,11 @@ CASES = [
 ]
 
 
+@pytest.mark.parametrize("longest", [None, 4000])           # as it is; told to be long (other plans, other splits)
 @pytest.mark.parametrize("i", range(len(CASES)))
-def test_matches_the_definition(i):
+def test_matches_the_definition(i, longest):
     c = Case(*CASES[i], seed=100 + i)
-    plan = c.plan()
+    plan = c.plan() if longest is None else c.plan(max_length=longest)
     c.check(*c.run(plan))
     assert plan.status() == 0
 
