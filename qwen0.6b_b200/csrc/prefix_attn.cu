@@ -1411,19 +1411,41 @@ bool al16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 constexpr int MAX_SPLITS = 64;
 
+// Rows of one sequence that an own CTA takes together.
+int rows_of_run(const int *h) {
+  const int ratio = h[PW_HEADS] / h[PW_KV_HEADS];
+  return ratio >= 8 ? 1 : 8 / ratio;
+}
+
+// Rounds of a memory latency in which the threads of an own CTA of `warps`
+// warps join the prefix's partial results: a column's four dims at a time,
+// eight partials at once (counted for CTAs of eight columns; rows of different
+// sequences have fewer where several would run together).
+int join_rounds(const int *h, int dim, int warps) {
+  const int ratio = h[PW_HEADS] / h[PW_KV_HEADS], cols = ratio < 8 ? rows_of_run(h) * ratio : 8;
+  return (cols * dim / 4 + 32 * warps - 1) / (32 * warps) * ((h[PW_MAX_SLOTS] + 7) / 8);
+}
+
 // Splits of a row's own part: enough CTAs for a few per SM when the batch is
 // small, at least 128 tokens each (the longest row behind the longest prefix
 // is the usual own part), and no more than about 4096 tokens in any case (the
 // longest row behind the shortest prefix).  Up to 256 tokens are not split:
 // two splits and the join kernel take as long or longer (2 rows of 136 tokens
 // 7.9 us, unsplit 6.7; of 256 8.0 and 8.6, but 2.4 us less on the host; 8 rows
-// of 200 behind 512 13.8 and 10.3).
-int plan_splits(const int *h, int max_length) {
+// of 200 behind 512 13.8 and 10.3).  Nor are parts of up to 600 tokens that
+// run beside the prefix kernel, on SMs that it leaves, for less than its time
+// (8 rows of 300 behind 1920 17.8 and 12.5, of 500 behind 60000 57.3 and 51.9).
+int plan_splits(const int *h, int dim, int max_length) {
   const int ratio = h[PW_HEADS] / h[PW_KV_HEADS];
   const long long ctas = static_cast<long long>(h[PW_ROWS]) * h[PW_KV_HEADS] * ((ratio + 7) / 8);
   const long long usual = max_length - h[PW_MAX_PREFIX], longest = max_length - h[PW_MIN_PREFIX];
   long long s = (592 + ctas - 1) / ctas;
   if (s > (usual + 127) / 128) s = usual <= 256 ? 1 : (usual + 127) / 128;
+  if (h[PW_SEGS] > 0 && ctas <= kOwnPerSm<2> * (148 - h[PW_CTAS]) && usual <= 600 && join_rounds(h, dim, 2) <= 12) {
+    const double tiles = 0.9 * h[PW_MAX_PREFIX] / TN / h[PW_MAX_SLOTS];
+    const double bytes = 4.0 * h[PW_MAX_PREFIX] * h[PW_KV_HEADS] * dim / 5.5e6;
+    if (0.02 * usual <= 6 + (tiles > bytes ? tiles : bytes)) s = 1;
+  }
   if (s < longest / 4096) s = longest / 4096;
   if (s > MAX_SPLITS) s = MAX_SPLITS;
   return s < 1 ? 1 : static_cast<int>(s);
@@ -1469,15 +1491,6 @@ int encode_pool(CUtensorMap *m, const QwenPrefixAttention &a, const void *pool, 
   return 0;
 }
 
-// Rounds of a memory latency in which the threads of an own CTA of `warps`
-// warps join the prefix's partial results: a column's four dims at a time,
-// eight partials at once (counted for CTAs of eight columns; rows of different
-// sequences have fewer).
-int join_rounds(const Args &a, const int *h, int dim, int warps) {
-  const int cols = a.ratio < 8 ? a.run_rows * a.ratio : 8;
-  return (cols * dim / 4 + 32 * warps - 1) / (32 * warps) * ((h[PW_MAX_SLOTS] + 7) / 8);
-}
-
 // Warps of an own CTA; those of two take half as long, but an SM holds fewer.
 // One warp for large batches (256 rows behind 2048 tokens: 43 us, two warps
 // 50), and where the SMs that the prefix kernel leaves hold all CTAs of one
@@ -1489,7 +1502,7 @@ int own_warps(const Args &a, const int *h, int dim) {
   const long long ctas = static_cast<long long>(a.rows) * a.kv_heads * ((a.ratio + 7) / 8) * a.own_splits;
   const long long sms = 148 - (h[PW_SEGS] > 0 ? h[PW_CTAS] : 0);
   if (ctas >= 1480) return 1;
-  return ctas > kOwnPerSm<2> * sms && ctas <= kOwnPerSm<1> * sms && join_rounds(a, h, dim, 1) <= 8 ? 1 : 2;
+  return ctas > kOwnPerSm<2> * sms && ctas <= kOwnPerSm<1> * sms && join_rounds(h, dim, 1) <= 8 ? 1 : 2;
 }
 
 template <typename T, int D>
@@ -1749,7 +1762,7 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
 long long qwen_b200_prefix_workspace(const int *h, int dim, int max_length) {
   if (!plan_ok(h) || (dim != 64 && dim != 128)) return 0;
   return slot_bytes(h, dim) +
-         up256(static_cast<long long>(h[PW_ROWS]) * h[PW_HEADS] * plan_splits(h, max_length) * (dim + 4) * 4);
+         up256(static_cast<long long>(h[PW_ROWS]) * h[PW_HEADS] * plan_splits(h, dim, max_length) * (dim + 4) * 4);
 }
 
 int qwen_b200_prefix_attention(const QwenPrefixAttention *u, void *stream) {
@@ -1790,14 +1803,15 @@ int qwen_b200_prefix_attention(const QwenPrefixAttention *u, void *stream) {
   a.num_seqs = u->num_seqs;
   a.max_pages = u->max_pages;
   a.length_bias = u->length_bias;
-  a.own_splits = plan_splits(h, u->max_length);
-  a.run_rows = a.ratio >= 8 ? 1 : 8 / a.ratio;
+  a.own_splits = plan_splits(h, u->dim, u->max_length);
+  a.run_rows = rows_of_run(h);
   a.after_prefix = h[PW_SEGS] > 0;
   // The own kernel joins by itself while that takes few rounds; the join
   // kernel spreads them further but starts after it.  128 rows behind 1920
-  // tokens (16 rounds) 20.7 us, with the join kernel 26.1; 16 sequences of 4
-  // rows behind 4096 21.7 and 20.5.
-  a.fused = a.own_splits == 1 && join_rounds(a, h, u->dim, own_warps(a, h, u->dim)) <= 16;
+  // tokens (16 rounds counted, 4 run) 20.7 us, with the join kernel 26.1; 16
+  // sequences of 4 rows behind 4096 (16) 21.7 and 20.5; 4 rows of eight heads
+  // per kv head behind 8192 (16) 27.9 and 18.6.
+  a.fused = a.own_splits == 1 && join_rounds(h, u->dim, own_warps(a, h, u->dim)) <= (a.run_rows > 1 ? 16 : 8);
   a.scale_log2 = u->scale * 1.4426950408889634f;
   a.box = u->page_tokens % 128 == 0 ? 128 : u->page_tokens % 64 == 0 ? 64 : u->page_tokens % 32 == 0 ? 32 : 16;
   a.box_shift = a.box == 128 ? 7 : a.box == 64 ? 6 : a.box == 32 ? 5 : 4;
