@@ -343,7 +343,7 @@ __device__ __forceinline__ int v_place(bool dual, int t, int n) {
 // tokens, 123 MB: 28 us, 4.4 TB/s with the queries' start and the results'
 // end; the ring holds 160 KB in flight per SM).  With many rows (64 x 8 rows
 // over 30000 tokens, 126 GFLOP) the softmax: a pair of tiles takes 3650 clocks,
-// of which the tensor cores work 48 %, its 256 x 128 exponentials half of the
+// of which the tensor cores work 47 %, its 256 x 128 exponentials half of the
 // rest; 113 us, 1.1 PFLOP/s where the products alone would allow 1.66.
 // Measured against it: exponentials half by a polynomial on the FMA pipe 143
 // us in all (140), weights announced at 64 or 96 columns of 128 142, two
