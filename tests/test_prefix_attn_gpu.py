@@ -68,6 +68,44 @@ def test_layouts_and_strides(dtype, layout):
     assert out.data_ptr() == big[:, 2:10].data_ptr()
 
 
+def test_tables_with_wider_rows_and_sequences_in_any_order():
+    """A window of a larger table, rows of sequences in no order, some twice."""
+    c = Case(F16, 128, 2, 2, 32, [7], [300], [20, 90, 1], seed=20)
+    n, w = c.table.shape
+    wide = torch.full((n + 3, w + 5), 12345, dtype=torch.int32, device="cuda")
+    wide[2:2 + n, 3:3 + w] = c.table
+    c.table = wide[2:2 + n, 3:3 + w]
+    order = torch.tensor([4, 0, 6, 4, 2, 1, 5], device="cuda")
+    c.seq_ids, c.lengths = c.seq_ids[order].contiguous(), c.lengths[order].contiguous()
+    for longest in (400, 4000):
+        plan = c.plan(max_length=longest)
+        c.check(*c.run(plan))
+        assert plan.status() == 0
+
+
+def test_calls_of_two_threads():
+    """Host threads with a stream and a plan each, at the same time."""
+    import threading
+    cases = [Case(F16, 128, 2, 2, 32, [9], [700], [20, 90], seed=21), Case(BF16, 64, 4, 1, 16, [3, 30], [100, 900], [7], seed=22)]
+    plans = [c.plan() for c in cases]
+    want = [c.run(p) for c, p in zip(cases, plans)]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(c, p, ref):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                out, lse = c.run(p)
+                if not (torch.equal(out, ref[0]) and torch.equal(lse, ref[1])):
+                    bad.append(c)
+    threads = [threading.Thread(target=work, args=x) for x in zip(cases, plans, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad and all(p.status() == 0 for p in plans)
+
+
 def test_empty_and_short_rows():
     """Length 0 gives 0 and -inf; a row shorter than its group's prefix is right on its own pages."""
     c = Case(F16, 128, 2, 2, 64, [6], [640], [40, 3], seed=6)
