@@ -6,16 +6,19 @@
 // three times its time on the device.)
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
 #include <optional>
 #include <tuple>
+#include <vector>
 
 #include "qwen_b200.h"
 #include "qwen_b200_paged.h"
 
 namespace {
 
+namespace py = pybind11;
 using torch::Tensor;
 
 void check_rc(int rc, const char *what) {
@@ -54,43 +57,82 @@ QwenPageTable table_of(const Tensor &t) {
                        t.size(0) > 1 ? t.stride(0) : t.size(1)};
 }
 
-// A list of integers on the host, as contiguous int32.
-struct HostList {
-  Tensor t;
-  HostList(const Tensor &given, const char *name, int64_t n = -1) : t(given) {
+// A list of integers on the host, as contiguous int32: any Python iterable of
+// integers, or a tensor.  (Lists are read here: through torch.tensor a copy of
+// one page took 7.7 us on the host, 3.1 now, of 255 pages 50 and 17.)
+class HostList {
+ public:
+  HostList(const py::object &given, const char *name, int64_t n = -1) {
+    if (THPVariable_Check(given.ptr()))
+      read(THPVariable_Unpack(given.ptr()), name);
+    else
+      read(given, name);
+    TORCH_CHECK_VALUE(n < 0 || n_ == n, name, " has ", n_, " entries, the other lists ", n);
+    TORCH_CHECK_VALUE(n_ < (1ll << 31), name, " has over 2^31 entries");
+  }
+  const int *data() const { return data_; }
+  int size() const { return static_cast<int>(n_); }
+
+ private:
+  void read(const Tensor &t, const char *name) {
     TORCH_CHECK_VALUE(t.device().is_cpu() && t.dim() == 1 && at::isIntegralType(t.scalar_type(), false), name,
                       " must be a one-dimensional list of integers on the host");
-    TORCH_CHECK_VALUE(n < 0 || t.numel() == n, name, " has ", t.numel(), " entries, the other lists ", n);
-    TORCH_CHECK_VALUE(t.numel() < (1ll << 31), name, " has over 2^31 entries");
+    t_ = t;
     if (t.scalar_type() != torch::kInt) {
       const Tensor wide = t.to(torch::kLong);
       TORCH_CHECK_VALUE(wide.numel() == 0 || (wide.min().item<int64_t>() >= -(1ll << 31) &&
                                               wide.max().item<int64_t>() < (1ll << 31)),
                         name, " holds a value outside 32 bits");
-      t = wide.to(torch::kInt);
+      t_ = wide.to(torch::kInt);
     }
-    t = t.contiguous();
+    t_ = t_.contiguous();
+    data_ = t_.data_ptr<int>();
+    n_ = t_.numel();
   }
-  const int *data() const { return t.data_ptr<int>(); }
-  int size() const { return static_cast<int>(t.numel()); }
+  void read(const py::object &given, const char *name) {
+    const auto seq = py::reinterpret_steal<py::object>(PySequence_Fast(given.ptr(), ""));
+    if (!seq) PyErr_Clear();
+    TORCH_CHECK_VALUE(seq, name, " must be a one-dimensional list of integers on the host");
+    n_ = PySequence_Fast_GET_SIZE(seq.ptr());
+    v_.resize(n_);
+    for (int64_t i = 0; i < n_; ++i) {
+      // (A new reference: an item's __index__ may change the list.)
+      const auto item = py::reinterpret_borrow<py::object>(i < PySequence_Fast_GET_SIZE(seq.ptr())
+                                                               ? PySequence_Fast_GET_ITEM(seq.ptr(), i)
+                                                               : Py_None);
+      const auto x = py::reinterpret_steal<py::object>(PyNumber_Index(item.ptr()));
+      if (!x) PyErr_Clear();
+      TORCH_CHECK_VALUE(x, name, " must be a one-dimensional list of integers on the host");
+      int over = 0;
+      const long long value = PyLong_AsLongLongAndOverflow(x.ptr(), &over);
+      TORCH_CHECK_VALUE(over == 0 && value >= -(1ll << 31) && value < (1ll << 31), name,
+                        " holds a value outside 32 bits");
+      v_[i] = static_cast<int>(value);
+    }
+    data_ = v_.data();
+  }
+  Tensor t_;
+  std::vector<int> v_;
+  const int *data_ = nullptr;
+  int64_t n_ = 0;
 };
 
 void same_device(const Tensor &t, const Tensor &k) {
   TORCH_CHECK_VALUE(t.device() == k.device(), "page_table is on ", t.device(), ", the pools on ", k.device());
 }
 
-void copy_pages(const Tensor &k, const Tensor &v, const Tensor &src, const Tensor &dst,
-                const std::optional<Tensor> &tokens) {
+void copy_pages(const Tensor &k, const Tensor &v, const py::object &src, const py::object &dst,
+                const py::object &tokens) {
   const QwenPagePools p = pools_of(k, v);
   const HostList s(src, "src"), d(dst, "dst", s.size());
   std::optional<HostList> t;
-  if (tokens) t.emplace(*tokens, "tokens", s.size());
+  if (!tokens.is_none()) t.emplace(tokens, "tokens", s.size());
   const c10::cuda::CUDAGuard guard(k.device());
   check_rc(qwen_b200_pages_copy(&p, s.data(), d.data(), t ? t->data() : nullptr, s.size(), stream_of(k)), "copy_pages");
 }
 
-void fork_pages(const Tensor &table, const Tensor &k, const Tensor &v, const Tensor &parents, const Tensor &children,
-                const Tensor &lengths, const Tensor &new_pages) {
+void fork_pages(const Tensor &table, const Tensor &k, const Tensor &v, const py::object &parents,
+                const py::object &children, const py::object &lengths, const py::object &new_pages) {
   const QwenPagePools p = pools_of(k, v);
   const QwenPageTable t = table_of(table);
   same_device(table, k);
@@ -101,7 +143,8 @@ void fork_pages(const Tensor &table, const Tensor &k, const Tensor &v, const Ten
            "fork_pages");
 }
 
-void compact_pages(const Tensor &table, const Tensor &k, const Tensor &v, const Tensor &src, const Tensor &dst) {
+void compact_pages(const Tensor &table, const Tensor &k, const Tensor &v, const py::object &src,
+                   const py::object &dst) {
   const QwenPagePools p = pools_of(k, v);
   const QwenPageTable t = table_of(table);
   same_device(table, k);
@@ -110,7 +153,7 @@ void compact_pages(const Tensor &table, const Tensor &k, const Tensor &v, const 
   check_rc(qwen_b200_pages_compact(&p, &t, s.data(), d.data(), s.size(), stream_of(k)), "compact_pages");
 }
 
-void free_pages(const Tensor &table, const Tensor &seqs) {
+void free_pages(const Tensor &table, const py::object &seqs) {
   const QwenPageTable t = table_of(table);
   const HostList s(seqs, "seqs");
   const c10::cuda::CUDAGuard guard(table.device());

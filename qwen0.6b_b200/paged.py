@@ -65,19 +65,6 @@ def _ext():
 
 
 # ------------------------------------------------------------------- pages
-def _host_list(values, name: str) -> torch.Tensor:
-    """A sequence of integers as an int32 tensor on the host; a tensor as it is (the extension checks it)."""
-    if type(values) is torch.Tensor:
-        return values
-    try:
-        values = [operator.index(v) for v in values]
-    except TypeError as e:
-        raise ValueError(f"{name} must be a one-dimensional list of integers") from e
-    if values and not (min(values) >= -2**31 and max(values) < 2**31):
-        raise ValueError(f"{name} holds a value outside 32 bits")
-    return torch.tensor(values, dtype=torch.int32)
-
-
 def copy_pages(k_pool: torch.Tensor, v_pool: torch.Tensor, src, dst, tokens=None) -> None:
     """Copies the first tokens[i] tokens (default: all) of page src[i] into
     page dst[i], K and V, every layer and head.
@@ -85,8 +72,7 @@ def copy_pages(k_pool: torch.Tensor, v_pool: torch.Tensor, src, dst, tokens=None
     Pools: contiguous [num_pages, ..., page_tokens, dim].  src, dst, tokens:
     host lists.  Destinations are distinct and none is a source (ValueError);
     a source may repeat."""
-    _ext().copy_pages(k_pool, v_pool, _host_list(src, "src"), _host_list(dst, "dst"),
-                      None if tokens is None else _host_list(tokens, "tokens"))
+    _ext().copy_pages(k_pool, v_pool, src, dst, tokens)
 
 
 def fork_pages(page_table: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, parents, children, lengths,
@@ -99,20 +85,19 @@ def fork_pages(page_table: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Ten
     Host lists; children are distinct and none is a parent, the used new pages
     are distinct (ValueError) and free.  A parent's page outside the pool is
     skipped and recorded (``pages_status``)."""
-    _ext().fork_pages(page_table, k_pool, v_pool, _host_list(parents, "parents"), _host_list(children, "children"),
-                      _host_list(lengths, "lengths"), _host_list(new_pages, "new_pages"))
+    _ext().fork_pages(page_table, k_pool, v_pool, parents, children, lengths, new_pages)
 
 
 def compact_pages(page_table: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, src, dst) -> None:
     """Moves page src[i] to page dst[i] (K and V) and renames it in every table
     row.  Host lists; sources are distinct, destinations are distinct and none
     is a source (ValueError); no table row may hold a destination."""
-    _ext().compact_pages(page_table, k_pool, v_pool, _host_list(src, "src"), _host_list(dst, "dst"))
+    _ext().compact_pages(page_table, k_pool, v_pool, src, dst)
 
 
 def free_pages(page_table: torch.Tensor, seqs) -> None:
     """Unmaps every page of the sequences `seqs` (a host list): their table rows become -1."""
-    _ext().free_pages(page_table, _host_list(seqs, "seqs"))
+    _ext().free_pages(page_table, seqs)
 
 
 def pages_status(device=None) -> int:
@@ -123,6 +108,17 @@ def pages_status(device=None) -> int:
 
 
 # ------------------------------------------------- shared-prefix attention
+def _host_list(values, name: str) -> torch.Tensor:
+    """A sequence of integers, or a tensor of them, as an int32 tensor on the host."""
+    try:
+        values = [operator.index(v) for v in (values.tolist() if isinstance(values, torch.Tensor) else values)]
+    except TypeError as e:
+        raise ValueError(f"{name} must be a one-dimensional list of integers") from e
+    if values and not (min(values) >= -2**31 and max(values) < 2**31):
+        raise ValueError(f"{name} holds a value outside 32 bits")
+    return torch.tensor(values, dtype=torch.int32)
+
+
 class PrefixPlan:
     """The groups of a batch of rows and the split of their work over the SMs.
 
@@ -136,8 +132,7 @@ class PrefixPlan:
 
     def __init__(self, group_rows, prefix_lens, num_q_heads: int, num_kv_heads: int, head_dim: int, max_length: int,
                  device=None):
-        rows, lens = (_host_list(v.tolist() if isinstance(v, torch.Tensor) else v, name)
-                      for v, name in ((group_rows, "group_rows"), (prefix_lens, "prefix_lens")))
+        rows, lens = _host_list(group_rows, "group_rows"), _host_list(prefix_lens, "prefix_lens")
         if lens.numel() != rows.numel():
             raise ValueError(f"prefix_lens has {lens.numel()} entries, group_rows {rows.numel()}")
         if head_dim not in (64, 128):

@@ -192,6 +192,22 @@ def test_offsets_past_32_bits():
     assert not bool(k[68, :, :, 100:].any()) and not bool(k[:68].any())
 
 
+def test_lists_of_every_kind():
+    """Lists, tuples, ranges, generators, arrays and tensors of integers."""
+    import numpy as np
+    from paged import copy_pages
+    geo = (12, 1, 2, 16, 64, torch.float16)
+    raw, (k, v) = _pools(geo, 8)
+    kinds = [list, tuple, iter, np.array, torch.tensor, lambda x: torch.tensor(x, dtype=torch.int32)[::1],
+             lambda x: torch.tensor([y for z in x for y in (z, 99)])[::2]]
+    for i, kind in enumerate(kinds):
+        copy_pages(k, v, kind([0, 1]), kind([4 + i % 4, 8 + i % 4]), kind([16, 9]))
+        for pool, r in zip((k, v), raw):
+            r[4 + i % 4], r[8 + i % 4, :, :, :9] = r[0], r[1, :, :, :9]
+        _same(raw, (k, v))
+    copy_pages(k, v, range(0), [], ())
+
+
 def test_refusals_leave_the_pools_alone():
     from paged import compact_pages, copy_pages, fork_pages, free_pages
     geo = (10, 1, 2, 16, 64, torch.float16)
@@ -206,6 +222,12 @@ def test_refusals_leave_the_pools_alone():
             (lambda: copy_pages(k, v, torch.tensor([0.0]), [1]), "list of integers"),
             (lambda: copy_pages(k, v, torch.tensor([0], device="cuda"), [1]), "list of integers"),
             (lambda: copy_pages(k, v, torch.tensor([[0]]), [1]), "list of integers"),
+            (lambda: copy_pages(k, v, [0.0], [1]), "list of integers"),
+            (lambda: copy_pages(k, v, [[0]], [1]), "list of integers"),
+            (lambda: copy_pages(k, v, ["0"], [1]), "list of integers"),
+            (lambda: copy_pages(k, v, 0, [1]), "list of integers"),
+            (lambda: copy_pages(k, v, [0], [1], 5), "list of integers"),
+            (lambda: copy_pages(k, v, [-(1 << 70)], [1]), "32 bits"),
             (lambda: copy_pages(k[:, :, :, :8], v[:, :, :, :8], [0], [1]), "contiguous"),
             (lambda: copy_pages(k, v[:5], [0], [1]), "same shape"),
             (lambda: copy_pages(k, k, [0], [1]), "same pool"),
