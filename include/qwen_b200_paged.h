@@ -73,9 +73,12 @@ int qwen_b200_paged_status(uint64_t *detail);
 /* ------------------------------------------- shared-prefix attention
  * One token per row: row r is a query of sequence seq_ids[r] that sees the
  * positions 0 .. lengths[r] - 1 (+ length_bias) of that sequence's pages:
- *   out[r, h] = sum_t softmax_t(scale q[r, h] . k_t) v_t, in fp32,
+ *   out[r, h] = sum_t softmax_t(scale q[r, h] . k_t) v_t,
  * k and v of kv head h / (heads / kv_heads); lse[r, h] = log sum_t exp(scale
- * q . k_t).  A row that sees nothing gives 0 and -inf.  The rows come in
+ * q . k_t).  Scores, softmax statistics and sums are fp32.  The weights are
+ * rounded to the input type for their product with v (bf16: half a step each;
+ * fp16: half a step, or 2^-32 of the row's largest weight where that is more),
+ * the result once more at the end; lse counts the weights unrounded.  A row that sees nothing gives 0 and -inf.  The rows come in
  * groups: consecutive rows whose sequences hold the same tokens in their
  * first prefix_lens[g] positions.  Those are read and multiplied once for the
  * whole group, through the pages of its first row that is as long as the

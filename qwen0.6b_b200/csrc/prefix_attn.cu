@@ -141,23 +141,43 @@ __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatil
   return __all_sync(0xffffffffu, ok);
 }
 
+// The weights 2^(s - m) enter the second product rounded to the input type.
+// fp16 holds 11 bits of a value only down to 2^-14 and nothing below 2^-25, so
+// that the long tail behind a dominant token would be lost from the product and
+// still be counted in the sum.  Its weights are therefore kept 2^kShift times
+// larger, by a reference m that lies kShift below the maximum at which it was
+// taken: they hold 11 bits down to 2^-(14 + kShift) of that maximum, and what
+// is smaller is off by 2^-(25 + kShift) of it at most.  The reference moves when
+// a score has outgrown it by 2^kLazy more, so weights stay at or below
+// 2^(kShift + kLazy) = 2^15 < 65504 (saturated there: the rounding of a score of
+// over 2^22 is worth more than the rest).  bf16 has the exponents of fp32 and
+// needs no shift.  Measured: 64 x 8 rows over 30000 tokens 160 us with and
+// without the shift; a shift of 11 and 2^4 to outgrow, 164.
 template <typename T>
 struct Type;
 template <>
 struct Type<__half> {
   static constexpr int kBf16 = 0;
+  static constexpr float kLazy = 8.f, kShift = 7.f;
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
+  }
+  static __device__ __forceinline__ uint32_t weights(float a, float b) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
   }
 };
 template <>
 struct Type<__nv_bfloat16> {
   static constexpr int kBf16 = 1;
+  static constexpr float kLazy = 8.f, kShift = 0.f;
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
   }
+  static __device__ __forceinline__ uint32_t weights(float a, float b) { return pack(a, b); }
 };
 
 // Length of row r (bias added), or -1 when its sequence or length lies
@@ -333,7 +353,7 @@ __device__ __forceinline__ int v_place(bool dual, int t, int n) {
 //   S_s = Q_s K^T       tcgen05, both operands in shared memory
 //   P_s = 2^(S_s - m)   rounded to the input type over S_s in tensor memory
 //   O_s += P_s V        tcgen05, P from tensor memory, V as it lies (MN-major)
-// The maximum m moves only when a row has outgrown it by 2^8, so the output is
+// The reference m moves only when a row has outgrown it by 2^8, so the output is
 // hardly ever rescaled.  Warps: 0 copies K and V tiles (a ring of five of 32
 // KB; the pages of the next 32 boxes are looked up ahead), 1 issues every
 // product, 2 waits for tiles on its behalf, 4 to 7 and 8 to 11 are the
@@ -691,15 +711,15 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int k = 0; k < 8; ++k) mx[k] = max3(mx[k], v[c >> 6][(c & 63) + k], v[(c + 8) >> 6][((c + 8) & 63) + k]);
 #pragma unroll
           for (int k = 0; k < 8; ++k) mx[k] = max3(mx[k], v[1][56 + k], v[1][56 + k]);
-          const float rowmax =
-              max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), max3(mx[6], mx[7], mx[7])) * a.scale_log2;
+          // The reference that this tile's maximum would give.
+          const float ref = fmaf(max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), max3(mx[6], mx[7], mx[7])),
+                                 a.scale_log2, -Type<T>::kShift);
           if (i == 0) {
-            m = rowmax;
-          } else if (__any_sync(0xffffffffu, !(rowmax <= m + 8.f))) {
-            // The maximum moves only when a row has outgrown it by 2^8: the
-            // weights stay below 2^8, exact in relative terms, and the output
+            m = ref;
+          } else if (__any_sync(0xffffffffu, !(ref <= m + Type<T>::kLazy))) {
+            // It moves only when a row has outgrown it by 2^kLazy: the output
             // is rescaled a few times at most.
-            const float mn = max3(m, rowmax, rowmax);
+            const float mn = max3(m, ref, ref);
             const float f = mn == -INFINITY ? 1.f : ex2_approx(m - mn);
             m = mn;
             l *= f;
@@ -729,9 +749,9 @@ __global__ void __launch_bounds__(THREADS, 1)
               x = ex2_approx(x);
               y = ex2_approx(y);
               sum[k & 1] = add2(sum[k & 1], pair2(x, y));
-              // The weights enter the second product rounded to the input type
-              // (half a step each, as the values they weigh); their sum is not.
-              w[k] = Type<T>::pack(x, y);
+              // The weights enter the second product rounded to the input type;
+              // their sum is not.
+              w[k] = Type<T>::weights(x, y);
             }
             tmem_st16(ts + c0 / 2, w);
             if (c0 == 32) {
@@ -999,7 +1019,7 @@ __device__ __forceinline__ void put_result(const Args &a, int row, int head, int
 // registers, a block's K is replaced as soon as it has been multiplied, its V
 // likewise; fragments are loaded as 8 x 8 matrices, V transposed on the way
 // (its 16-byte chunks are exchanged by the token's number, so that no read has
-// bank conflicts); the maximum moves only when a column has outgrown it by 2^8,
+// bank conflicts); the reference moves only when a column has outgrown it by 2^8,
 // as in the prefix kernel.  Measured: 256 rows of up to 256 own tokens, 142 MB,
 // 36 us beside the prefix kernel (4 TB/s); 112 rows of 1000 with no prefix 74
 // us (6.2 TB/s, 0.95 of a copy's rate).
@@ -1204,9 +1224,9 @@ __global__ void __launch_bounds__(32 * W, kOwnPerSm<W>) own_kernel(const Args a)
       for (int k = 1; k < NB; ++k) mx[h] = fmaxf(mx[h], fmaxf(s[k][h], s[k][2 + h]));
       mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 4));
       mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 8));
-      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 16)) * a.scale_log2;
+      mx[h] = fmaf(fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 16)), a.scale_log2, -Type<T>::kShift);
     }
-    if (__any_sync(0xffffffffu, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f)) {
+    if (__any_sync(0xffffffffu, mx[0] > m[0] + Type<T>::kLazy || mx[1] > m[1] + Type<T>::kLazy)) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float mn = fmaxf(m[h], mx[h]);
@@ -1222,8 +1242,8 @@ __global__ void __launch_bounds__(32 * W, kOwnPerSm<W>) own_kernel(const Args a)
     }
     const float mu0 = m[0] == -INFINITY ? 0.f : m[0], mu1 = m[1] == -INFINITY ? 0.f : m[1];
     // P^T as the B operand (n = column g, k = tokens 2c, 2c+1 / 2c+8, 2c+9).
-    // The weights are rounded to the input type for the product (half a step
-    // each, as the values they weigh); their sum is not.
+    // The weights are rounded to the input type for the product; their sum is
+    // not.
     uint32_t pb[NB][2];
 #pragma unroll
     for (int k = 0; k < NB; ++k) {
@@ -1233,8 +1253,8 @@ __global__ void __launch_bounds__(32 * W, kOwnPerSm<W>) own_kernel(const Args a)
       s[k][3] = ex2_approx(fmaf(s[k][3], a.scale_log2, -mu1));
       l[0] += s[k][0] + s[k][2];
       l[1] += s[k][1] + s[k][3];
-      pb[k][0] = transpose8x8(Type<T>::pack(s[k][0], s[k][1]));
-      pb[k][1] = transpose8x8(Type<T>::pack(s[k][2], s[k][3]));
+      pb[k][0] = transpose8x8(Type<T>::weights(s[k][0], s[k][1]));
+      pb[k][1] = transpose8x8(Type<T>::weights(s[k][2], s[k][3]));
     }
     copy_wait<1>();
     __syncwarp();

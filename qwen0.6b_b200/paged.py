@@ -180,7 +180,10 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
                             out: torch.Tensor | None = None, return_lse: bool = False):
     """softmax(scale q . K^T) V of every row over its sequence's pages, the
     prefix of each of the plan's groups read and multiplied once for all its
-    rows (fp32 sums, one rounding at the end).
+    rows.  Scores, softmax statistics and sums are fp32; the weights are rounded
+    to q's type for their product with V (bf16: half a step each; fp16: half a
+    step, or 2^-32 of the row's largest weight where that is more), and the
+    result once at the end.
 
     q [rows, q heads, dim] (fp16 or bf16, dim 64 or 128): row r is a token of
     sequence seq_ids[r] that sees its positions 0 .. lengths[r] - 1.  Several

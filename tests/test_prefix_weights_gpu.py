@@ -1,0 +1,139 @@
+"""The softmax weights of shared_prefix_attention: a long tail behind one
+dominant token, and tokens that alone decide a row's result, one at each place
+where the work is cut (tiles of 128 tokens, parts of the plan, splits of the own
+part, the border of the prefix, blocks of 16 tokens, pages)."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+F16, BF16 = torch.float16, torch.bfloat16
+
+# fp16 weights are held to 11 bits, or to 2^-32 of their row's largest weight
+# where that is more (half of fp16's smallest step, 2^-25, of weights kept 2^7
+# times larger).
+FLOOR = {F16: 2.0 ** -32, BF16: 0.0}
+
+
+def _pools(k, v, page, seed):
+    """k, v [kv heads, n, dim] as pages in no order: pools, and the page of each `page` tokens."""
+    kv, n, d = k.shape
+    pages = -(-n // page)
+    order = torch.randperm(pages, generator=torch.Generator().manual_seed(seed))
+    pools = []
+    for x in (k, v):
+        pool = torch.full((pages, kv, page, d), math.nan, dtype=x.dtype)
+        for i in range(pages):
+            part = x[:, i * page:(i + 1) * page]
+            pool[order[i], :, :part.shape[1]] = part
+        pools.append(pool.cuda())
+    return pools, order.int()
+
+
+def _run(q, pools, order, n, plan):
+    """Rows of n tokens with a table row each, all of them over the same pages."""
+    from paged import shared_prefix_attention
+    rows = q.shape[0]
+    ids = torch.arange(rows, dtype=torch.int32, device="cuda")
+    out, lse = shared_prefix_attention(q.cuda(), *pools, order.repeat(rows, 1).cuda(), ids, torch.full_like(ids, n),
+                                       plan, return_lse=True)
+    assert plan.status() == 0
+    return out.double().cpu(), lse.double().cpu()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("n,prefix,longest", [
+    (30000, 29952, 30000),      # the prefix kernel
+    (30000, 0, 30000),          # the own kernel, split over many CTAs
+    (900, 896, 1000), (900, 0, 900)])
+@pytest.mark.parametrize("gap", [14.0, 17.0, 18.0])
+@pytest.mark.parametrize("at", [0, -1])
+def test_a_tail_behind_a_dominant_token(dtype, n, prefix, longest, gap, at):
+    """The dominant token's value is 0: what the row gives is its tail, of
+    weight e^-gap each and n e^-gap together.
+
+    Bounds: a score is off by e (products exact in fp32, each of 128 additions
+    by 2^-23 of what was added at most), so a normalised weight by w (2 e +
+    2^-19) and its rounding: u w, or FLOOR of the largest one."""
+    from paged import PrefixPlan
+    g = torch.Generator().manual_seed(3)
+    d, rows = 128, 2
+    k = 0.02 * torch.randn(1, n, d, generator=g)
+    k[..., 0] = 0.0
+    k[0, at, 0] = gap / 1.4142135
+    v = 1.0 + 0.25 * torch.randn(1, n, d, generator=g)
+    v[0, at] = 0.0
+    q = 0.1 * torch.randn(rows, 1, d, generator=g)
+    q[..., 0] = 16.0                                    # x dim^-0.5 = 1.414
+    q, k, v = (x.to(dtype) for x in (q, k, v))
+    pools, order = _pools(k, v, 128, 1)
+    out, lse = _run(q, pools, order, n, PrefixPlan([rows], [prefix], 1, 1, d, max_length=longest))
+    qd, kd, vd = q.double()[:, 0], k.double()[0], v.double()[0]
+    s = qd @ kd.T * d ** -0.5
+    w = torch.softmax(s, -1)
+    ref = w @ vd
+    e = d * 2.0 ** -23 * d ** -0.5 * (qd.abs() @ kd.abs().T)
+    u = torch.finfo(dtype).eps / 2
+    # The largest error of a score bounds that of the sum, each weight has its own.
+    off = w * (u + e + e.amax(-1, keepdim=True) + 2.0 ** -19) + FLOOR[dtype] * w.amax(-1, keepdim=True)
+    tiny = 2.0 ** -25 if dtype == F16 else 0.0          # the smallest step of the output
+    bound = off @ vd.abs() + u * ref.abs() + tiny
+    err = (out[:, 0] - ref).abs()
+    assert bool((err <= bound).all()), f"{float((err / bound).max())} times the bound, {float((err / ref.abs()).max())} of the result"
+    want = torch.logsumexp(s, -1)
+    assert bool(((lse[:, 0] - want).abs() <= 2 * e.amax(-1) + 2.0 ** -19 + 2.0 ** -22 * want.abs()).all())
+
+
+def _needles(n, prefix, own_from):
+    """Every border of 16 tokens and its two neighbours, thinned to about 1,500 of them, and the ends."""
+    at = {0, 1, n - 2, n - 1, prefix - 1, prefix, own_from - 1, own_from}
+    for b in range(16, n, 16 if n < 8000 else 128):
+        at |= {b - 1, b}
+    return sorted(x for x in at if 0 <= x < n)
+
+
+@pytest.mark.parametrize("dtype,dim,ratio,page,n,prefix,rows,longest", [
+    (F16, 128, 2, 128, 2200, 1920, 4, 2300),            # a prefix in parts of two tiles, an own part of 280
+    (F16, 128, 2, 128, 2200, 1900, 4, 6000),            # cut inside a block of 16; own part split
+    (BF16, 64, 4, 16, 1100, 1000, 3, 1100),             # small pages
+    (F16, 128, 8, 64, 700, 640, 40, 700),               # 320 queries: a pair of tiles and a single one
+    (BF16, 128, 2, 128, 1300, 0, 2, 1300),              # nothing shared: own splits
+    (F16, 64, 2, 32, 9000, 8000, 2, 9000),
+    (BF16, 128, 1, 48, 30000, 29000, 3, 30000),
+    (F16, 128, 2, 128, 250, 128, 2, 250),               # one CTA alone
+])
+def test_a_token_that_decides_is_counted_once(dtype, dim, ratio, page, n, prefix, rows, longest):
+    """Query j points along dimension j and one token's key does too, far
+    enough that its weight is all but 1: the result is that token's value and
+    the logarithm is its score.  A token left out would give the mean of the
+    others, one counted twice ln 2 more.  One call asks for dim tokens."""
+    from paged import PrefixPlan
+    plan = PrefixPlan([rows], [prefix], ratio, 1, dim, max_length=longest)
+    g = torch.Generator().manual_seed(4)
+    at = _needles(n, prefix, prefix // 16 * 16)
+    v = torch.randn(1, n, dim, generator=g).to(dtype)
+    base = (0.02 * torch.randn(1, n, dim, generator=g)).to(dtype)
+    heads = ratio
+    scale = dim ** -0.5
+    u = torch.finfo(dtype).eps / 2
+    for i in range(0, len(at), dim):
+        some = at[i:i + dim]
+        k = base.clone()
+        k[0, some, :] = 0.0
+        k[0, some, range(len(some))] = 20.0
+        pools, order = _pools(k, v, page, 1)
+        for first in range(0, len(some), rows * heads):
+            mine = some[first:first + rows * heads]
+            q = torch.zeros(rows * heads, dim)
+            q[range(len(mine)), range(first, first + len(mine))] = 32.0
+            q = q.reshape(rows, heads, dim).to(dtype)
+            out, lse = _run(q, pools, order, n, plan)
+            out, lse = out.reshape(-1, dim)[:len(mine)], lse.reshape(-1)[:len(mine)]
+            s = q.double().reshape(-1, dim)[:len(mine)] @ k.double()[0].T * scale
+            ref = torch.softmax(s, -1) @ v.double()[0]
+            e = dim * 2.0 ** -23 * scale * 640.0
+            rest = n * math.exp(-40.0)                  # what the other tokens weigh: 640 scale - 3 > 40
+            bound = (2 * u + 4 * e + 2.0 ** -18) * ref.abs() + 8.0 * rest + 2.0 ** -24
+            assert bool(((out - ref).abs() <= bound).all())
+            assert bool(((lse - torch.logsumexp(s, -1)).abs() <= 2 * e + 2.0 ** -19 + 2.0 ** -22 * 80).all())
