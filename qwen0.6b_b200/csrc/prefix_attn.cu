@@ -149,9 +149,9 @@ __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatil
 // taken: they hold 11 bits down to 2^-(14 + kShift) of that maximum, and what
 // is smaller is off by 2^-(25 + kShift) of it at most.  The reference moves when
 // a score has outgrown it by 2^kLazy more, so weights stay at or below
-// 2^(kShift + kLazy) = 2^15 < 65504 (saturated there: the rounding of a score of
-// over 2^22 is worth more than the rest).  bf16 has the exponents of fp32 and
-// needs no shift.  Measured: 64 x 8 rows over 30000 tokens 160 us with and
+// 2^(kShift + kLazy) = 2^15 < 65504 (scores of over 2^22, which are themselves
+// rounded by more than the factor of 2 that is left, saturate).  bf16 has the
+// exponents of fp32 and needs no shift.  Measured: 64 x 8 rows over 30000 tokens 160 us with and
 // without the shift; a shift of 11 and 2^4 to outgrow, 164.
 template <typename T>
 struct Type;
@@ -680,6 +680,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // Queries of this warp past the group: nothing to compute.
       const bool live = s.q0 + (dual ? st * QT : 0) + 32 * quad < s.nq;
       float m = -INFINITY, l = 0.f;
+      bool seen = mapped && my_steps > 0;  // whether a token is visible at all
       for (int i = 0; i < my_steps && ok; ++i) {
         const int t = s.t0 + (dual ? i : 2 * i + st);
         const int ntok = min(TN, s.prefix - t * TN);
@@ -697,6 +698,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               bool bad = true;
               if (lane < boxes) page_of(row, s, t * boxes + lane, &bad);
               valid = __ballot_sync(0xffffffffu, !bad);
+              seen = seen || (valid & ((1u << ((ntok + a.box - 1) >> a.box_shift)) - 1u)) != 0;
             }
 #pragma unroll
             for (int c = 0; c < TN; ++c)
@@ -780,7 +782,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       // A visible part whose scores are all -inf: the sum tells it from an
       // empty one (the softmax of nothing but -inf is NaN).  A NaN among them
       // is in the sum already.
-      if (my_steps > 0 && m == -INFINITY && l == 0.f) l = 1.f;
+      if (seen && m == -INFINITY && l == 0.f) l = 1.f;
       float f0 = 1.f, f1 = 0.f;
       const bool both = !dual && nt > 1;
       if (both) {
