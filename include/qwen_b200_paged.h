@@ -38,8 +38,9 @@ typedef struct QwenPageTable {
 /* The lists below are HOST arrays of n entries, read before the call returns
  * (they travel as kernel parameters: a captured graph holds their values).
  * They are checked in full; what only the device knows (the pages that a
- * table row names) is range-checked there: such an entry is skipped and
- * recorded for qwen_b200_paged_status().
+ * table row names) is range-checked there: such an entry is skipped (fork: -1 in
+ * the child's row, or a tail that is not copied) and recorded for
+ * qwen_b200_paged_status().
  *
  * copy: the first tokens[i] tokens (NULL: all) of page src[i] into page
  * dst[i], K and V.  Destinations are distinct and no destination is a source;

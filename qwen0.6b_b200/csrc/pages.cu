@@ -166,8 +166,17 @@ __global__ void __launch_bounds__(FORK_THREADS) pages_fork_kernel(const MoveArgs
       const int *from = a.table + f.parent[x] * a.pitch;
       int *to = a.table + f.child[x] * a.pitch;
       const int full = f.length[x] / a.page_tokens, tail = f.length[x] % a.page_tokens;
-      for (int i = threadIdx.x; i < a.max_pages; i += FORK_THREADS)
-        to[i] = i < full ? from[i] : (i == full && tail ? f.l.dst[x] : -1);
+      for (int i = threadIdx.x; i < a.max_pages; i += FORK_THREADS) {
+        int page = i == full && tail ? f.l.dst[x] : -1;
+        if (i < full) {
+          page = from[i];
+          if (page < 0 || page >= a.num_pages) {
+            record_err(3, static_cast<uint32_t>(f.parent[x]));
+            page = -1;
+          }
+        }
+        to[i] = page;
+      }
     }
   } else {
     const int cta = blockIdx.x - a.table_ctas;

@@ -84,7 +84,8 @@ def fork_pages(page_table: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Ten
 
     Host lists; children are distinct and none is a parent, the used new pages
     are distinct (ValueError) and free.  A parent's page outside the pool is
-    skipped and recorded (``pages_status``)."""
+    skipped (a full one is -1 in the child, a partly filled one is not copied)
+    and recorded (``pages_status``)."""
     _ext().fork_pages(page_table, k_pool, v_pool, parents, children, lengths, new_pages)
 
 
