@@ -167,7 +167,9 @@ int qwen_b200_batched_step_logits(void *handle, int rows, const int *seq_ids, co
  * qwen_b200_prefix_workspace(plan_header, 128, max_length) bytes; max_length
  * as there.  Consecutive rows of a group must hold the same tokens in their
  * sequences' first prefix_lens[g] positions (e.g. after a fork).  Writes the
- * greedy tokens (tokens_out, logits NULL) or the logits (tokens_out NULL). */
+ * greedy tokens (tokens_out, logits NULL) or the logits (tokens_out NULL).
+ * What the attention records goes to the plan's status word and to
+ * qwen_b200_batched_status. */
 int qwen_b200_batched_step_prefix(void *handle, int rows, const int *seq_ids, const int *positions,
                                   const int *tokens_in, int *tokens_out, float *logits, long long ld,
                                   float *norm_out, const int *plan_header, void *plan, void *workspace,
@@ -176,8 +178,8 @@ int qwen_b200_batched_step_prefix(void *handle, int rows, const int *seq_ids, co
 
 /* Synchronises the device; returns 0 if no batched kernel has recorded an
  * error since the last call, else its code (1: a bounded wait gave up, 2: a
- * token id outside the vocabulary, 3: a sequence id or position outside the
- * caches; the offending row's access was skipped), and clears the record. */
+ * token id outside the vocabulary, 3: a sequence id, position or page outside
+ * the caches; the offending row's access was skipped), and clears the record. */
 int qwen_b200_batched_status(void *handle, uint64_t *detail);
 void qwen_b200_batched_destroy(void *handle);
 

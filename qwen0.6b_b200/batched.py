@@ -427,6 +427,9 @@ class BatchedDecoder:
         return out
 
     def status(self) -> int:
+        """Synchronises the device; 0, or the code that a step has recorded
+        since the last call (1: a bounded wait gave up, 2: a token outside the
+        vocabulary, 3: a sequence, position or page outside the tables)."""
         d = ctypes.c_uint64(0)
         return lib().qwen_b200_batched_status(self._h, ctypes.byref(d))
 

@@ -994,7 +994,7 @@ int step_layers(Plan *p, int rows, const int *seq_ids, const int *positions, con
       const size_t layer = static_cast<size_t>(l) * NKV * PAGE * HD;
       shared->k_pool = p->k_pool + layer;
       shared->v_pool = p->v_pool + layer;
-      if (int rc = qwen_b200_prefix_attention(shared, st)) return rc;
+      if (int rc = qb200_prefix_run(shared, w.err, st)) return rc;
     } else {
       LAUNCH(attn_split_kernel, dim3(nsplit, NKV, rows), dim3(ATT_THREADS), smem, p->tm_k,
              static_cast<const __half *>(w.qrot), static_cast<const __half *>(p->k_pool),

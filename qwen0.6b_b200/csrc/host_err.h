@@ -17,3 +17,6 @@ int qb200_encode_f16_2d(CUtensorMap *m, const void *ptr, long long inner, long l
 // The argument checks of qwen_b200_prefix_attention (prefix_attn.cu).
 struct QwenPrefixAttention;
 int qb200_prefix_check(const QwenPrefixAttention *a);
+// qwen_b200_prefix_attention that also records into the device word `also`
+// (null: the plan's alone), in the same form.
+int qb200_prefix_run(const QwenPrefixAttention *a, unsigned long long *also, void *stream);

@@ -100,7 +100,8 @@ struct Args {
   long long table_pitch;
   long long page_stride, head_stride, token_stride;
   const void *k_pool, *v_pool;
-  unsigned long long *err;
+  unsigned long long *err;   // the plan's status word
+  unsigned long long *also;  // the caller's, or null
   int rows, heads, kv_heads, ratio;
   int num_pages, page_tokens, box, box_shift, num_seqs, max_pages;
   int length_bias, own_splits, run_rows;
@@ -110,8 +111,10 @@ struct Args {
 };
 
 // Status of a launch: the first code recorded stays.
-__device__ __forceinline__ void record(unsigned long long *err, uint32_t code) {
-  atomicCAS(err, 0ull, (static_cast<unsigned long long>(code) << 32) | (blockIdx.x & 0xffffffu));
+__device__ __forceinline__ void record(const Args &a, uint32_t code) {
+  const unsigned long long v = (static_cast<unsigned long long>(code) << 32) | (blockIdx.x & 0xffffffu);
+  atomicCAS(a.err, 0ull, v);
+  if (a.also != nullptr) atomicCAS(a.also, 0ull, v);
 }
 
 // Bounded wait of a whole warp; false for all its lanes when it gave up (or
@@ -125,7 +128,7 @@ __device__ __forceinline__ void record(unsigned long long *err, uint32_t code) {
 // parities say no more), so whoever waits on a barrier waits for each of its
 // phases, in order, or for something that followed from them.
 __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile uint32_t *abort,
-                                         unsigned long long *err) {
+                                         const Args &a) {
   bool ok = mbar_try_wait(bar, parity);
   if (!ok) {
     const uint64_t t0 = qb200::globaltimer_ns();
@@ -133,7 +136,7 @@ __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatil
       if (*abort) break;
       if (static_cast<long long>(qb200::globaltimer_ns() - t0) > qb200tc::WAIT_NS) {
         *abort = 1;
-        record(err, 1);
+        record(a, 1);
         break;
       }
     }
@@ -462,7 +465,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       auto look = [&](int t, bool report) {
         bool bad = false;
         const int p = lane < wt * boxes ? page_of(row, s, (s.t0 + t) * boxes + lane, &bad) : a.num_pages;
-        if (bad && report && row != nullptr && s.t0 + t + lane / boxes < s.t1) record(a.err, 3);
+        if (bad && report && row != nullptr && s.t0 + t + lane / boxes < s.t1) record(a, 3);
         return p;
       };
       cur[0] = cur[1] = look(0, true);
@@ -501,7 +504,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           page = __shfl_sync(0xffffffffu, cur[0], (t - win[0]) * boxes + (lane < boxes ? lane : 0));
         }
         const int stage = place % ST;
-        if (place >= ST) ok = wait_bar(&kv_empty[stage], ((place / ST) - 1) & 1, abort, a.err);
+        if (place >= ST) ok = wait_bar(&kv_empty[stage], ((place / ST) - 1) & 1, abort, a);
         if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&kv_full[stage], TILE);
         __syncwarp();
@@ -518,7 +521,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     // Every issued copy lands before the CTA may exit (matters after an abort).
     for (int p = place > ST ? place - ST : 0; p < place; ++p)
-      wait_bar(&kv_full[p % ST], (p / ST) & 1, abort + 1, a.err);
+      wait_bar(&kv_full[p % ST], (p / ST) & 1, abort + 1, a);
   } else if (warp == 1) {
     // ---- MMAs
     constexpr uint32_t id_s = idesc16<T>(TN, false), id_o = idesc16<T>(D, true);
@@ -529,7 +532,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const Seg s = segment(si);
       const bool dual = s.dual != 0;
       const int nt = s.t1 - s.t0, n = dual ? 2 * nt : nt;
-      ok = wait_bar(q_full, (si - seg0) & 1, abort, a.err);
+      ok = wait_bar(q_full, (si - seg0) & 1, abort, a);
       if (!ok) break;
       tc_fence_after();
       auto score = [&](int i) {  // S of step i
@@ -554,7 +557,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int ks = min(TN, s.prefix - (s.t0 + t) * TN) / 16;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          ok = ok && wait_bar(&p_full[2 * st + half], (phase >> st) & 1, abort, a.err);
+          ok = ok && wait_bar(&p_full[2 * st + half], (phase >> st) & 1, abort, a);
           if (!ok) break;
           tc_fence_after();
           if (ks >= 4 * half + 4)
@@ -575,7 +578,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     // Tensor memory is freed, and the CTA ends, only after every product and
     // every arrival that was asked for (also after an abort).
     commit_elect(drained);
-    wait_bar(drained, 0, abort + 1, a.err);
+    wait_bar(drained, 0, abort + 1, a);
     __syncwarp();
   } else if (warp == 2) {
     // ---- tiles: waits for a step's V and the next K ahead of the MMA warp,
@@ -593,18 +596,18 @@ __global__ void __launch_bounds__(THREADS, 1)
       const bool dual = s.dual != 0;
       const int nt = s.t1 - s.t0, n = dual ? 2 * nt : nt;
       const auto landed = [&](int place) {
-        return wait_bar(&kv_full[(ring0 + place) % ST], ((ring0 + place) / ST) & 1, abort, a.err);
+        return wait_bar(&kv_full[(ring0 + place) % ST], ((ring0 + place) / ST) & 1, abort, a);
       };
       ok = landed(0) && (dual || n < 2 || landed(1));
       // (One arrival per phase, here and below: the one before has to be complete.)
-      if (ok && si > seg0) ok = wait_bar(q_full, (si - seg0 - 1) & 1, abort, a.err);
+      if (ok && si > seg0) ok = wait_bar(q_full, (si - seg0 - 1) & 1, abort, a);
       if (ok && lane == 0) mbar_arrive(q_full);
       __syncwarp();
       for (int i = 0; i < n && ok; ++i) {
         ok = landed(v_place(dual, dual ? i >> 1 : i, nt)) &&
              (i + 2 >= n || landed(k_place(dual, dual ? (i + 2) >> 1 : i + 2)));
         const int st = i & 1;
-        if (ok && ((begun >> st) & 1)) ok = wait_bar(&p_full[2 * st], ((phase >> st) & 1) ^ 1, abort, a.err);
+        if (ok && ((begun >> st) & 1)) ok = wait_bar(&p_full[2 * st], ((phase >> st) & 1) ^ 1, abort, a);
         phase ^= 1u << st;
         begun |= 1u << st;
         if (ok && lane == 0) mbar_arrive(&p_full[2 * st]);
@@ -684,7 +687,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int i = 0; i < my_steps && ok; ++i) {
         const int t = s.t0 + (dual ? i : 2 * i + st);
         const int ntok = min(TN, s.prefix - t * TN);
-        ok = wait_bar(&s_full[st], steps & 1, abort, a.err);
+        ok = wait_bar(&s_full[st], steps & 1, abort, a);
         if (!ok) break;
         ++steps;
         tc_fence_after();
@@ -775,7 +778,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[2 * st + 1]);
       }
-      ok = ok && wait_bar(o_full, (si - seg0) & 1, abort, a.err);
+      ok = ok && wait_bar(o_full, (si - seg0) & 1, abort, a);
       ok = !qb200::named_bar_or(1, 256, !ok || *abort);  // all eight warps go on, or none
       if (!ok) break;
       tc_fence_after();
@@ -1076,7 +1079,7 @@ __global__ void __launch_bounds__(32 * W, kOwnPerSm<W>) own_kernel(const Args a)
   len = __shfl_sync(0xffffffffu, len, min(me + lane, 31));  // lane i: row i of the run
   const int max_len = __reduce_max_sync(0xffffffffu, lane < nrun ? len : -1);
   const int min_len = __reduce_min_sync(0xffffffffu, lane < nrun ? len : 0x7fffffff);
-  if (max_len < 0 && threadIdx.x == 0) record(a.err, 3);
+  if (max_len < 0 && threadIdx.x == 0) record(a, 3);
   const int per = max(128, ((max_len - my_start + a.own_splits - 1) / a.own_splits + 15) / 16 * 16);
   const int lo = my_start + split * per, hi = min(max_len, lo + per);
   const bool fused = a.fused;
@@ -1111,7 +1114,7 @@ __global__ void __launch_bounds__(32 * W, kOwnPerSm<W>) own_kernel(const Args a)
       if (page >= 0 && page < a.num_pages)
         where = page * a.page_stride + static_cast<long long>(b - pi * a.page_tokens) * a.token_stride;
       else
-        record(a.err, 3);
+        record(a, 3);
     }
   };
   lookup(0);
@@ -1789,6 +1792,23 @@ long long qwen_b200_prefix_workspace(const int *h, int dim, int max_length) {
 
 int qwen_b200_prefix_attention(const QwenPrefixAttention *u, void *stream) {
   qb200_clear_error();
+  return qb200_prefix_run(u, nullptr, stream);
+}
+
+int qwen_b200_prefix_status(const int *h, void *plan, uint64_t *detail) {
+  if (!plan_ok(h) || plan == nullptr) return -1;
+  unsigned long long v = 0;
+  void *err = static_cast<int *>(plan) + h[PW_ERR];
+  if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpy(&v, err, sizeof(v), cudaMemcpyDeviceToHost) != cudaSuccess)
+    return -2;
+  if (detail) *detail = v;
+  if (v != 0) cudaMemset(err, 0, sizeof(v));
+  return static_cast<int>(v >> 32);
+}
+
+}  // extern "C"
+
+int qb200_prefix_run(const QwenPrefixAttention *u, unsigned long long *also, void *stream) {
   if (int rc = qb200_prefix_check(u)) return rc;
   const int *h = u->plan_header;
   Args a{};
@@ -1816,6 +1836,7 @@ int qwen_b200_prefix_attention(const QwenPrefixAttention *u, void *stream) {
   a.k_pool = u->k_pool;
   a.v_pool = u->v_pool;
   a.err = reinterpret_cast<unsigned long long *>(static_cast<int *>(u->plan) + h[PW_ERR]);
+  a.also = also;
   a.rows = u->rows;
   a.heads = u->heads;
   a.kv_heads = u->kv_heads;
@@ -1847,16 +1868,3 @@ int qwen_b200_prefix_attention(const QwenPrefixAttention *u, void *stream) {
     return u->dim == 128 ? launch<__half, 128>(*u, a, mk, mv, st) : launch<__half, 64>(*u, a, mk, mv, st);
   return u->dim == 128 ? launch<__nv_bfloat16, 128>(*u, a, mk, mv, st) : launch<__nv_bfloat16, 64>(*u, a, mk, mv, st);
 }
-
-int qwen_b200_prefix_status(const int *h, void *plan, uint64_t *detail) {
-  if (!plan_ok(h) || plan == nullptr) return -1;
-  unsigned long long v = 0;
-  void *err = static_cast<int *>(plan) + h[PW_ERR];
-  if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpy(&v, err, sizeof(v), cudaMemcpyDeviceToHost) != cudaSuccess)
-    return -2;
-  if (detail) *detail = v;
-  if (v != 0) cudaMemset(err, 0, sizeof(v));
-  return static_cast<int>(v >> 32);
-}
-
-}  // extern "C"
