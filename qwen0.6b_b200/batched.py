@@ -504,7 +504,8 @@ class BatchedDecoder:
         drawn with ``sampling``.  Paged pools.  Sequence i holds prompt i; the
         prefix is prefilled once, its full pages are shared by all sequences
         and every step attends to it once for the whole batch.  The sequences
-        must hold no pages; they keep theirs afterwards (``release``)."""
+        must hold no pages; they keep theirs afterwards (``release``).  Raises
+        RuntimeError when ``status`` reports an error after the last step."""
         if not self.paged:
             raise ValueError("generate_shared needs paged pools")
         n = len(suffixes)
@@ -539,6 +540,6 @@ class BatchedDecoder:
             tok = self.step(ids, pos, tok, longest - 1, out=torch.empty(n, **dev), sampling=sampling, prefix=steps)
             outs.append(tok)
             pos = pos + 1
-        if code := steps.status():
-            raise RuntimeError(f"shared-prefix attention has recorded error {code}")
+        if code := self.status() or steps.status():
+            raise RuntimeError(f"a step of generate_shared has recorded error {code}")
         return torch.stack(outs, 1).cpu().tolist()

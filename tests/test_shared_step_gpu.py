@@ -40,3 +40,35 @@ def test_status_reports_what_the_attention_recorded(weights_2l):
     assert bd.status() == 3 and plan.status() == 3
     bd.page_table[0].copy_(row)
     assert torch.equal(bd.step(*step, 300, prefix=plan), want) and bd.status() == 0 and plan.status() == 0
+
+
+@pytest.mark.parametrize("when", ["prompt", "suffixes", "answers"])
+def test_generate_shared_raises_what_any_of_its_steps_recorded(weights_2l, monkeypatch, when):
+    """A page that is missing during one step only, while the prefix, the
+    suffixes or the answers are computed."""
+    from batched import BatchedDecoder
+    bd = BatchedDecoder(weights_2l, num_seqs=4, max_rows=64, num_layers=2, paged=True, num_pages=24)
+    prefix, suffixes = _tokens(200, 2), [_tokens(4, 3), _tokens(70, 4), _tokens(9, 5)]
+    want = bd.generate_shared(prefix, suffixes, 4)
+    bd.release([0, 1, 2])
+    plain, steps = BatchedDecoder.step, []
+
+    def step(self, *args, **kw):
+        kind = "prompt" if kw.get("prefix") is None else "suffixes" if kw["prefix"].rows != 3 else "answers"
+        steps.append(kind)
+        if steps.count(kind) != 1 + (kind == "prompt") or kind != when:
+            return plain(self, *args, **kw)
+        row = self.page_table[0].clone()
+        self.page_table[0, 0] = -1
+        try:
+            return plain(self, *args, **kw)
+        finally:
+            self.page_table[0].copy_(row)
+
+    monkeypatch.setattr(BatchedDecoder, "step", step)
+    with pytest.raises(RuntimeError, match="recorded error 3"):
+        bd.generate_shared(prefix, suffixes, 4)
+    assert set(steps) == {"prompt", "suffixes", "answers"}
+    monkeypatch.undo()
+    bd.release([0, 1, 2])
+    assert bd.generate_shared(prefix, suffixes, 4) == want and bd.status() == 0
