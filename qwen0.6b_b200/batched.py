@@ -401,6 +401,9 @@ class BatchedDecoder:
                                  f"{prefix.num_kv_heads} heads of {prefix.head_dim}, the step has {rows} rows")
             if prefix.device != self.dev:
                 raise ValueError(f"the plan is on {prefix.device}, the decoder on {self.dev}")
+            if not 0 <= max_position < self.max_seq:  # refused as by the steps without a plan
+                raise RuntimeError(f"batched_step_prefix failed (code 11): max_position={max_position} outside the KV "
+                                   f"cache (max_seq={self.max_seq})")
             # From the caching allocator with every step, so that captured steps have one each.
             ws = torch.empty(prefix.workspace_bytes, dtype=torch.uint8, device=self.dev)
             with torch.cuda.device(self.dev):

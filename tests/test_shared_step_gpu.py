@@ -42,6 +42,15 @@ def test_status_reports_what_the_attention_recorded(weights_2l):
     assert torch.equal(bd.step(*step, 300, prefix=plan), want) and bd.status() == 0 and plan.status() == 0
 
 
+@pytest.mark.parametrize("position", [-1, 2048, 1 << 30])
+def test_positions_outside_the_cache_are_refused(weights_2l, position):
+    """With a plan as without one."""
+    bd, plan, step = _forked(weights_2l)
+    for prefix in (None, plan):
+        with pytest.raises(RuntimeError, match="outside the KV cache"):
+            bd.step(*step, position, prefix=prefix)
+
+
 @pytest.mark.parametrize("when", ["prompt", "suffixes", "answers"])
 def test_generate_shared_raises_what_any_of_its_steps_recorded(weights_2l, monkeypatch, when):
     """A page that is missing during one step only, while the prefix, the
