@@ -126,36 +126,48 @@ class PagePool:
 
     def reserve(self, seq: int, upto_position: int) -> bool:
         """Maps pages for positions 0..upto_position; True if the row changed."""
-        missing, row = self._missing(seq, upto_position), self.table[seq]
+        missing = self._missing(seq, upto_position)
         self._enough(len(missing))
+        self._map(seq, missing)
+        return bool(missing)
+
+    def _map(self, seq: int, missing: list[int]) -> None:
+        row = self.table[seq]
         for i in missing:
             row[i] = self._take()
-        return bool(missing)
 
     def _missing(self, seq: int, upto_position: int) -> list[int]:
         need = upto_position // PAGE + 1
         if not 0 <= seq < self.num_seqs or not 0 <= upto_position or need > self.max_pages:
             raise ValueError(f"sequence {seq} / position {upto_position} outside the page table")
-        row = self.table[seq]
-        return [i for i in range(need) if row[i] < 0]
+        row = self.table[seq][:need]
+        return [i for i, page in enumerate(row) if page < 0] if -1 in row else []
 
     def _shared(self, seq: int, write_from: int, upto_position: int) -> list[int]:
-        row = self.table[seq]
-        return [i for i in range(write_from // PAGE, upto_position // PAGE + 1) if row[i] >= 0 and self.refs[row[i]] > 1]
+        first = write_from // PAGE
+        row = self.table[seq][first:upto_position // PAGE + 1]
+        return [first + i for i, page in enumerate(row) if page >= 0 and self.refs[page] > 1]
 
     def claim(self, seq: int, write_from: int, upto_position: int) -> tuple[bool, list[tuple[int, int, int]]]:
         """reserve and unshare, both or (when the pool is exhausted) neither."""
-        self._enough(len(self._missing(seq, upto_position)) + len(self._shared(seq, write_from, upto_position)))
-        return self.reserve(seq, upto_position), self.unshare(seq, write_from, upto_position)
+        missing, shared = self._missing(seq, upto_position), self._shared(seq, write_from, upto_position)
+        if not missing and not shared:  # the usual call of a step loop
+            return False, []
+        self._enough(len(missing) + len(shared))
+        self._map(seq, missing)
+        return bool(missing), self._split(seq, shared, write_from)
 
     def unshare(self, seq: int, write_from: int, upto_position: int) -> list[tuple[int, int, int]]:
         """Gives sequence `seq` pages of its own for the positions
         write_from..upto_position, which are about to be written, where it
         shares them with another one: (source, destination, tokens to copy) of
         each; the tokens before write_from stay, those behind it are dropped."""
-        row, shared = self.table[seq], self._shared(seq, write_from, upto_position)
+        shared = self._shared(seq, write_from, upto_position)
         self._enough(len(shared))
-        moves = []
+        return self._split(seq, shared, write_from)
+
+    def _split(self, seq: int, shared: list[int], write_from: int) -> list[tuple[int, int, int]]:
+        row, moves = self.table[seq], []
         for i in shared:
             src, row[i] = row[i], self._take()
             self._drop(src)
@@ -317,10 +329,11 @@ class BatchedDecoder:
         if not 0 <= write_from <= upto_position:
             raise ValueError(f"write_from {write_from} outside [0, {upto_position}]")
         changed, moves = self.pages.claim(seq, write_from, upto_position)
+        if not changed and not moves:
+            return
         if any(t for _, _, t in moves):
             copy_pages(self.k_pool, self.v_pool, *zip(*moves))
-        if changed or moves:
-            self.page_table[seq].copy_(torch.tensor(self.pages.table[seq], dtype=torch.int32))
+        self.page_table[seq].copy_(torch.tensor(self.pages.table[seq], dtype=torch.int32))
 
     def release(self, seq: int | list[int]) -> None:
         """Returns every page of sequence `seq` (or of each in a list) to the
