@@ -123,7 +123,8 @@ long long qwen_b200_prefix_workspace(const int *plan_header, int dim, int max_le
 int qwen_b200_prefix_attention(const QwenPrefixAttention *a, void *stream);
 /* Synchronises the current device; 0, or the code that a launch with this
  * device plan has recorded since the last call (1: a bounded wait gave up,
- * 3: a sequence, length or page outside the tables, skipped). */
+ * 3: a sequence, length or page outside the tables, skipped), and clears the
+ * record.  Until a 1 has been read here, the rows that share a prefix give NaN. */
 int qwen_b200_prefix_status(const int *plan_header, void *plan, uint64_t *detail);
 
 #ifdef __cplusplus

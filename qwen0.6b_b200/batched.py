@@ -557,5 +557,5 @@ class BatchedDecoder:
             outs.append(tok)
             pos = pos + 1
         if code := self.status() or steps.status():
-            raise RuntimeError(f"a step of generate_shared has recorded error {code}")
+            raise RuntimeError(f"the decoder has recorded error {code}")
         return torch.stack(outs, 1).cpu().tolist()

@@ -110,11 +110,22 @@ struct Args {
   float scale_log2;
 };
 
-// Status of a launch: the first code recorded stays.
+// Status of a launch: the first code recorded stays, but a wait that gave up
+// (1) replaces another one, as the joins look for it.
 __device__ __forceinline__ void record(const Args &a, uint32_t code) {
   const unsigned long long v = (static_cast<unsigned long long>(code) << 32) | (blockIdx.x & 0xffffffu);
-  atomicCAS(a.err, 0ull, v);
+  if (code == 1) atomicExch(a.err, v);
+  else atomicCAS(a.err, 0ull, v);
   if (a.also != nullptr) atomicCAS(a.also, 0ull, v);
+}
+
+// The code in the plan's status word, behind the wait for the prefix kernel.  1:
+// a prefix kernel of this plan has given up a wait since the status was last
+// read; its partial results may be whatever the workspace held, so the rows
+// that would join them get NaN.  (Looked at where a result is written, so that
+// nothing waits for this load.)
+__device__ __forceinline__ uint32_t status_code(const Args &a) {
+  return __ldcg(reinterpret_cast<const uint32_t *>(a.err) + 1);
 }
 
 // Bounded wait of a whole warp; false for all its lanes when it gave up (or
@@ -1328,6 +1339,7 @@ __global__ void __launch_bounds__(32 * W, kOwnPerSm<W>) own_kernel(const Args a)
   }
   __syncthreads();
   if (a.after_prefix) qb200::griddep_wait();
+  const uint32_t code = shared ? status_code(a) : 0;
   for (int x0 = 0; x0 < nc * Q4; x0 += NT) {
     // Neighbouring threads take the columns: their prefix partials are adjacent.
     const int x = x0 + threadIdx.x, col = x % nc, d4 = x / nc;
@@ -1344,6 +1356,7 @@ __global__ void __launch_bounds__(32 * W, kOwnPerSm<W>) own_kernel(const Args a)
       j.add(s_m[w][col], s_l[w][col],
             *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(s_kv[w]) + col * OP + 4 * d4));
     if (fused) {
+      if (code == 1) j.none = __int_as_float(0x7fffffff);
       put_result<T>(a, r, head, d4, j);
     } else {
       float *part = a.own + ((static_cast<size_t>(r) * a.heads + head) * a.own_splits + split) * (D + 4);
@@ -1375,6 +1388,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args a) {
   const int grp = threadIdx.x / used;
   qb200::griddep_wait();
   qb200::griddep_launch_dependents();
+  const uint32_t code = status_code(a);
   int seq;
   const int len = row_length(a, row, &seq);
   const bool shared = rp.prefix > 0 && len >= rp.prefix;
@@ -1411,6 +1425,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_kernel(const Args a) {
         }
       }
     }
+    if (shared && code == 1) j.none = __int_as_float(0x7fffffff);
     if (grp == 0 && x < nout) put_result<T>(a, row, head, d4, j);
     if (x0 + used < nout) __syncthreads();
   }

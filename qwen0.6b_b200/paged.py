@@ -157,7 +157,8 @@ class PrefixPlan:
     def status(self) -> int:
         """Synchronises the device; 0, or what a call with this plan has
         recorded since the last one (1: a bounded wait gave up, 3: a sequence,
-        length or page outside the tables, which was skipped)."""
+        length or page outside the tables, which was skipped).  Until a 1 has
+        been read, the rows that share a prefix give NaN."""
         with torch.cuda.device(self.device):
             return lib().qwen_b200_prefix_status(self.header.data_ptr(), self.words.data_ptr(), None)
 
