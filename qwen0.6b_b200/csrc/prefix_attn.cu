@@ -129,17 +129,18 @@ __device__ __forceinline__ uint32_t status_code(const Args &a) {
 }
 
 // Bounded wait of a whole warp; false for all its lanes when it gave up (or
-// another role already did).  The lanes may leave the loop apart and meet
-// again in the vote: what follows a wait is warp-collective (tensor memory
-// accesses, elections, named barriers).  (Going round by votes costs 2 us in
-// 44.)  Inline like everything in the prefix kernel: a call would keep the
-// compiler from giving its warps different register counts.
+// another role already did), which *abort tells the kernel's end to record
+// (recorded here, at each of the waits, it took 1.2 us in 46: 13 rows over 60000
+// tokens).  The lanes may leave the loop apart and meet again in the vote: what
+// follows a wait is warp-collective (tensor memory accesses, elections, named
+// barriers).  (Going round by votes costs 2 us in 44.)  Inline like everything
+// in the prefix kernel: a call would keep the compiler from giving its warps
+// different register counts.
 //
 // A wait for a phase also passes while the phase before it is open (the
 // parities say no more), so whoever waits on a barrier waits for each of its
 // phases, in order, or for something that followed from them.
-__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile uint32_t *abort,
-                                         const Args &a) {
+__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile uint32_t *abort) {
   bool ok = mbar_try_wait(bar, parity);
   if (!ok) {
     const uint64_t t0 = qb200::globaltimer_ns();
@@ -147,7 +148,6 @@ __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatil
       if (*abort) break;
       if (static_cast<long long>(qb200::globaltimer_ns() - t0) > qb200tc::WAIT_NS) {
         *abort = 1;
-        record(a, 1);
         break;
       }
     }
@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     mbar_init(o_full, 1);
     mbar_init(drained, 1);
     *abort = 0;
-    abort[1] = 0;  // never set: the wait for what is in flight is not cut short
+    abort[1] = 0;  // of the waits for what is in flight, which *abort does not cut short
     qb200::fence_mbar_init();
   }
   __syncwarp();
@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           page = __shfl_sync(0xffffffffu, cur[0], (t - win[0]) * boxes + (lane < boxes ? lane : 0));
         }
         const int stage = place % ST;
-        if (place >= ST) ok = wait_bar(&kv_empty[stage], ((place / ST) - 1) & 1, abort, a);
+        if (place >= ST) ok = wait_bar(&kv_empty[stage], ((place / ST) - 1) & 1, abort);
         if (!ok) break;
         if (lane == 0) mbar_arrive_expect_tx(&kv_full[stage], TILE);
         __syncwarp();
@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     // Every issued copy lands before the CTA may exit (matters after an abort).
     for (int p = place > ST ? place - ST : 0; p < place; ++p)
-      wait_bar(&kv_full[p % ST], (p / ST) & 1, abort + 1, a);
+      wait_bar(&kv_full[p % ST], (p / ST) & 1, abort + 1);
   } else if (warp == 1) {
     // ---- MMAs
     constexpr uint32_t id_s = idesc16<T>(TN, false), id_o = idesc16<T>(D, true);
@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const Seg s = segment(si);
       const bool dual = s.dual != 0;
       const int nt = s.t1 - s.t0, n = dual ? 2 * nt : nt;
-      ok = wait_bar(q_full, (si - seg0) & 1, abort, a);
+      ok = wait_bar(q_full, (si - seg0) & 1, abort);
       if (!ok) break;
       tc_fence_after();
       auto score = [&](int i) {  // S of step i
@@ -568,7 +568,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int ks = min(TN, s.prefix - (s.t0 + t) * TN) / 16;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          ok = ok && wait_bar(&p_full[2 * st + half], (phase >> st) & 1, abort, a);
+          ok = ok && wait_bar(&p_full[2 * st + half], (phase >> st) & 1, abort);
           if (!ok) break;
           tc_fence_after();
           if (ks >= 4 * half + 4)
@@ -589,7 +589,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     // Tensor memory is freed, and the CTA ends, only after every product and
     // every arrival that was asked for (also after an abort).
     commit_elect(drained);
-    wait_bar(drained, 0, abort + 1, a);
+    wait_bar(drained, 0, abort + 1);
     __syncwarp();
   } else if (warp == 2) {
     // ---- tiles: waits for a step's V and the next K ahead of the MMA warp,
@@ -607,18 +607,18 @@ __global__ void __launch_bounds__(THREADS, 1)
       const bool dual = s.dual != 0;
       const int nt = s.t1 - s.t0, n = dual ? 2 * nt : nt;
       const auto landed = [&](int place) {
-        return wait_bar(&kv_full[(ring0 + place) % ST], ((ring0 + place) / ST) & 1, abort, a);
+        return wait_bar(&kv_full[(ring0 + place) % ST], ((ring0 + place) / ST) & 1, abort);
       };
       ok = landed(0) && (dual || n < 2 || landed(1));
       // (One arrival per phase, here and below: the one before has to be complete.)
-      if (ok && si > seg0) ok = wait_bar(q_full, (si - seg0 - 1) & 1, abort, a);
+      if (ok && si > seg0) ok = wait_bar(q_full, (si - seg0 - 1) & 1, abort);
       if (ok && lane == 0) mbar_arrive(q_full);
       __syncwarp();
       for (int i = 0; i < n && ok; ++i) {
         ok = landed(v_place(dual, dual ? i >> 1 : i, nt)) &&
              (i + 2 >= n || landed(k_place(dual, dual ? (i + 2) >> 1 : i + 2)));
         const int st = i & 1;
-        if (ok && ((begun >> st) & 1)) ok = wait_bar(&p_full[2 * st], ((phase >> st) & 1) ^ 1, abort, a);
+        if (ok && ((begun >> st) & 1)) ok = wait_bar(&p_full[2 * st], ((phase >> st) & 1) ^ 1, abort);
         phase ^= 1u << st;
         begun |= 1u << st;
         if (ok && lane == 0) mbar_arrive(&p_full[2 * st]);
@@ -631,6 +631,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_before();
   qb200::named_bar_sync(0, THREADS);
   if (warp == 1) tmem_dealloc(tmem, 512);
+  if (threadIdx.x == 0 && (abort[0] | abort[1])) record(a, 1);
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFT));
     // ---- softmax: thread = query
@@ -698,7 +699,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int i = 0; i < my_steps && ok; ++i) {
         const int t = s.t0 + (dual ? i : 2 * i + st);
         const int ntok = min(TN, s.prefix - t * TN);
-        ok = wait_bar(&s_full[st], steps & 1, abort, a);
+        ok = wait_bar(&s_full[st], steps & 1, abort);
         if (!ok) break;
         ++steps;
         tc_fence_after();
@@ -789,7 +790,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[2 * st + 1]);
       }
-      ok = ok && wait_bar(o_full, (si - seg0) & 1, abort, a);
+      ok = ok && wait_bar(o_full, (si - seg0) & 1, abort);
       ok = !qb200::named_bar_or(1, 256, !ok || *abort);  // all eight warps go on, or none
       if (!ok) break;
       tc_fence_after();
@@ -1090,7 +1091,7 @@ __global__ void __launch_bounds__(32 * W, kOwnPerSm<W>) own_kernel(const Args a)
   len = __shfl_sync(0xffffffffu, len, min(me + lane, 31));  // lane i: row i of the run
   const int max_len = __reduce_max_sync(0xffffffffu, lane < nrun ? len : -1);
   const int min_len = __reduce_min_sync(0xffffffffu, lane < nrun ? len : 0x7fffffff);
-  if (max_len < 0 && threadIdx.x == 0) record(a, 3);
+  bool bad = max_len < 0 && threadIdx.x == 0;  // something outside the tables, recorded at the end
   const int per = max(128, ((max_len - my_start + a.own_splits - 1) / a.own_splits + 15) / 16 * 16);
   const int lo = my_start + split * per, hi = min(max_len, lo + per);
   const bool fused = a.fused;
@@ -1125,7 +1126,7 @@ __global__ void __launch_bounds__(32 * W, kOwnPerSm<W>) own_kernel(const Args a)
       if (page >= 0 && page < a.num_pages)
         where = page * a.page_stride + static_cast<long long>(b - pi * a.page_tokens) * a.token_stride;
       else
-        record(a, 3);
+        bad = true;
     }
   };
   lookup(0);
@@ -1367,6 +1368,7 @@ __global__ void __launch_bounds__(32 * W, kOwnPerSm<W>) own_kernel(const Args a)
       }
     }
   }
+  if (bad) record(a, 3);
 }
 
 // -------------------------------------------------------------- join kernel
