@@ -417,6 +417,8 @@ class BatchedDecoder:
             if not 0 <= max_position < self.max_seq:  # refused as by the steps without a plan
                 raise RuntimeError(f"batched_step_prefix failed (code 11): max_position={max_position} outside the KV "
                                    f"cache (max_seq={self.max_seq})")
+            if stream != prefix.stream:  # the plan may be dropped while this step still reads it
+                prefix.words.record_stream(torch.cuda.current_stream(self.dev))
             # From the caching allocator with every step, so that captured steps have one each.
             ws = torch.empty(prefix.workspace_bytes, dtype=torch.uint8, device=self.dev)
             with torch.cuda.device(self.dev):

@@ -4,6 +4,7 @@
 // outputs.  Bad arguments raise ValueError, failed launches RuntimeError.
 // (Through ctypes the same checks in Python took 41 us per attention call,
 // three times its time on the device.)
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -196,6 +197,9 @@ std::tuple<Tensor, std::optional<Tensor>> prefix_attention(
                       x == &lengths ? "lengths" : "seq_ids", " must be a contiguous int32 tensor [", rows, "] on ",
                       q.device());
   const c10::cuda::CUDAGuard guard(q.device());
+  // A plan may be dropped while calls on other streams than its own still read it.
+  c10::cuda::CUDACachingAllocator::recordStream(words.storage().data_ptr(),
+                                                c10::cuda::getCurrentCUDAStream(q.device().index()));
   Tensor out;
   if (out_) {
     out = *out_;

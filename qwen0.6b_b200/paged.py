@@ -129,7 +129,8 @@ class PrefixPlan:
     is split; longer rows are still right).  Made once when sequences are
     forked and kept for their steps; the lengths may change from call to call.
     The device part is read only (but for the status word), so calls on several
-    streams may share a plan."""
+    streams may share a plan.  It may be dropped when the last call has been
+    made; a captured graph needs it for as long as it is replayed."""
 
     def __init__(self, group_rows, prefix_lens, num_q_heads: int, num_kv_heads: int, head_dim: int, max_length: int,
                  device=None):
@@ -151,7 +152,9 @@ class PrefixPlan:
         self.num_q_heads, self.num_kv_heads, self.head_dim = num_q_heads, num_kv_heads, head_dim
         self.max_length = int(max_length)
         self.header = words[:_HEADER].clone()
-        self.words = words.to(self.device)
+        self.stream = torch.cuda.current_stream(self.device).cuda_stream
+        with torch.cuda.device(self.device):
+            self.words = words.to(self.device)
         self.workspace_bytes = lib().qwen_b200_prefix_workspace(self.header.data_ptr(), head_dim, self.max_length)
 
     def status(self) -> int:
