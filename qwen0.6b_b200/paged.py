@@ -120,6 +120,17 @@ def _host_list(values, name: str) -> torch.Tensor:
     return torch.tensor(values, dtype=torch.int32)
 
 
+def _int(value, name: str) -> int:
+    """An integer of 32 bits (ctypes would cut a larger one down to them)."""
+    try:
+        value = operator.index(value)
+    except TypeError as e:
+        raise ValueError(f"{name} must be an integer, not {value!r}") from e
+    if not -2**31 <= value < 2**31:
+        raise ValueError(f"{name}={value} is outside 32 bits")
+    return value
+
+
 class PrefixPlan:
     """The groups of a batch of rows and the split of their work over the SMs.
 
@@ -137,6 +148,8 @@ class PrefixPlan:
         rows, lens = _host_list(group_rows, "group_rows"), _host_list(prefix_lens, "prefix_lens")
         if lens.numel() != rows.numel():
             raise ValueError(f"prefix_lens has {lens.numel()} entries, group_rows {rows.numel()}")
+        num_q_heads, num_kv_heads = _int(num_q_heads, "num_q_heads"), _int(num_kv_heads, "num_kv_heads")
+        head_dim, max_length = _int(head_dim, "head_dim"), _int(max_length, "max_length")
         if head_dim not in (64, 128):
             raise ValueError(f"head_dim={head_dim}: 64 or 128")
         if max_length < 0:
@@ -150,7 +163,7 @@ class PrefixPlan:
                            torch.cuda.get_device_properties(self.device).multi_processor_count)
         self.rows = int(words[1])
         self.num_q_heads, self.num_kv_heads, self.head_dim = num_q_heads, num_kv_heads, head_dim
-        self.max_length = int(max_length)
+        self.max_length = max_length
         self.header = words[:_HEADER].clone()
         self.stream = torch.cuda.current_stream(self.device).cuda_stream
         with torch.cuda.device(self.device):
