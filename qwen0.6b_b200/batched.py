@@ -522,7 +522,8 @@ class BatchedDecoder:
         drawn with ``sampling``.  Paged pools.  Sequence i holds prompt i; the
         prefix is prefilled once, its full pages are shared by all sequences
         and every step attends to it once for the whole batch.  The sequences
-        must hold no pages; they keep theirs afterwards (``release``).  Raises
+        must hold no pages; they keep theirs afterwards (``release``); none is
+        taken when the pool has too few (RuntimeError).  Raises
         RuntimeError when ``status`` reports an error after the last step."""
         if not self.paged:
             raise ValueError("generate_shared needs paged pools")
@@ -537,6 +538,9 @@ class BatchedDecoder:
             raise ValueError("generation would run past max_seq")
         # Shared positions: the prefix, but for a last token that some prompt still has to feed.
         shared = min(len(prefix), min(len(p) for p in prompts) - 1)
+        # All pages or none: the shared ones once, each sequence's own.
+        full = shared // PAGE
+        self.pages._enough(full + sum((len(p) + max_tokens - 2) // PAGE + 1 - full for p in prompts))
         self.prefill_parallel([prompts[0][:shared + 1]], seqs=[0])
         self.fork(0, list(range(1, n)), shared)
         dev = dict(dtype=torch.int32, device=self.dev)

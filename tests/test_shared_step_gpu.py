@@ -81,3 +81,27 @@ def test_generate_shared_raises_what_any_of_its_steps_recorded(weights_2l, monke
     monkeypatch.undo()
     bd.release([0, 1, 2])
     assert bd.generate_shared(prefix, suffixes, 4) == want and bd.status() == 0
+
+
+@pytest.mark.parametrize("prefix,suffixes,new", [
+    (300, [3, 70, 130], 20),     # a partly filled page of each; one more for the last
+    (256, [0, 0, 0], 1),         # shared up to position 254: nothing shared of page 1
+    (256, [1, 1, 1], 129),       # whole pages shared
+    (5, [0, 300, 0], 4),
+])
+def test_generate_shared_takes_all_its_pages_or_none(weights_2l, prefix, suffixes, new):
+    from batched import BatchedDecoder
+    prompt, tails = _tokens(prefix, 6), [_tokens(n, 7 + i) for i, n in enumerate(suffixes)]
+    bd = BatchedDecoder(weights_2l, num_seqs=4, max_rows=64, num_layers=2, paged=True, num_pages=24)
+    want = bd.generate_shared(prompt, tails, new)
+    used = bd.pages_in_use
+    exact = BatchedDecoder(weights_2l, num_seqs=4, max_rows=64, num_layers=2, paged=True, num_pages=used + 1)
+    exact.reserve(3, 0)
+    assert exact.generate_shared(prompt, tails, new) == want and exact.pages_in_use == used + 1
+    exact.release([0, 1, 2])
+    exact.reserve(3, 128)                               # one page fewer
+    for _ in range(2):                                  # and again: it holds none
+        with pytest.raises(RuntimeError, match="exhausted"):
+            exact.generate_shared(prompt, tails, new)
+        assert exact.pages_in_use == 2 and exact.page_table[:3].cpu().tolist() == exact.pages.table[:3]
+        assert all(page < 0 for row in exact.pages.table[:3] for page in row)
