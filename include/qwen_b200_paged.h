@@ -19,8 +19,9 @@ extern "C" {
 
 /* ------------------------------------------------------------------ pages
  * K and V pools of one geometry: [num_pages][inner][page_tokens][token_bytes]
- * each (inner = layers x kv heads of a page), contiguous, 16-byte aligned,
- * token_bytes a multiple of 16 (the element type does not matter). */
+ * each (inner = layers x kv heads of a page), contiguous, 16-byte aligned, in
+ * memory of their own, token_bytes a multiple of 16 (the element type does not
+ * matter). */
 typedef struct QwenPagePools {
   void *k_pool, *v_pool;
   int num_pages, inner, page_tokens, token_bytes;

@@ -265,6 +265,9 @@ int check_pools(const QwenPagePools *p) {
                 p->num_pages, p->inner, p->page_tokens, p->token_bytes);
   if (static_cast<long long>(p->inner) * p->page_tokens * (p->token_bytes / 16) > 0x3fffffffll)
     return fail(10, "pools: a page of over 16 GB");
+  const uintptr_t k = reinterpret_cast<uintptr_t>(p->k_pool), v = reinterpret_cast<uintptr_t>(p->v_pool);
+  const uintptr_t page = static_cast<uintptr_t>(p->inner) * p->page_tokens * p->token_bytes;
+  if ((k < v ? v - k : k - v) < page * p->num_pages) return fail(14, "K and V pools overlap");
   return 0;
 }
 
