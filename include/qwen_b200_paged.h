@@ -100,7 +100,7 @@ int qwen_b200_prefix_plan(int groups, const int *group_rows, const int *prefix_l
 
 typedef struct QwenPrefixAttention {
   const void *q;            /* [rows, heads, dim], last dimension contiguous */
-  void *out;                /* the same shape and type */
+  void *out;                /* the same shape and type; q itself, or memory of its own */
   float *lse;               /* [rows, heads] contiguous, or NULL */
   const void *k_pool, *v_pool; /* [num_pages, kv_heads, page_tokens, dim], strides below */
   const int *page_table, *seq_ids, *lengths; /* device */

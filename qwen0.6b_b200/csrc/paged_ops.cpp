@@ -4,6 +4,7 @@
 // outputs.  Bad arguments raise ValueError, failed launches RuntimeError.
 // (Through ctypes the same checks in Python took 41 us per attention call,
 // three times its time on the device.)
+#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -205,6 +206,10 @@ std::tuple<Tensor, std::optional<Tensor>> prefix_attention(
     out = *out_;
     TORCH_CHECK_VALUE(out.sizes() == q.sizes() && out.scalar_type() == type && out.device() == q.device(),
                       "out must have q's shape, type and device");
+    for (const Tensor *t : {&q, &k, &v})
+      TORCH_CHECK_VALUE(at::get_overlap_status(out, *t) != at::MemOverlapStatus::Partial &&
+                            (t == &q || at::get_overlap_status(out, *t) != at::MemOverlapStatus::Full),
+                        "out overlaps ", t == &q ? "q (it may be q itself)" : "the pools");
     // One of rows and heads lies within a step of the other.
     const int64_t sr = out.size(0) > 1 ? out.stride(0) : 1ll << 60, sh = out.size(1) > 1 ? out.stride(1) : 1ll << 60;
     const int64_t inner = sr < sh ? sr : sh, n = sr < sh ? out.size(0) : out.size(1);

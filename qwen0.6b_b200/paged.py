@@ -213,7 +213,8 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     as long as the prefix; a row shorter than that runs on its own pages.  A
     row of length 0 gives 0 (lse -inf; with seq_id 0 a padding row).  scale defaults to dim ** -0.5.
 
-    Returns out [rows, q heads, dim], with return_lse also the natural
+    Returns out [rows, q heads, dim] (the given one, which may be q itself but
+    no other memory of q or the pools), with return_lse also the natural
     logarithm of each softmax sum, fp32 [rows, q heads].  A sequence, length or
     page outside the tables is skipped and recorded (``plan.status()``)."""
     if not isinstance(plan, PrefixPlan):
