@@ -137,3 +137,23 @@ def test_a_token_that_decides_is_counted_once(dtype, dim, ratio, page, n, prefix
             bound = (2 * u + 4 * e + 2.0 ** -18) * ref.abs() + 8.0 * rest + 2.0 ** -24
             assert bool(((out - ref).abs() <= bound).all())
             assert bool(((lse - torch.logsumexp(s, -1)).abs() <= 2 * e + 2.0 ** -19 + 2.0 ** -22 * 80).all())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("prefix", [0, 1920])
+@pytest.mark.parametrize("size", [100.0, 700.0, 3000.0])
+def test_large_finite_scores_stay_finite(dtype, prefix, size):
+    """Scores up to 1e7: one step of a score in fp32 is then more than the
+    distance between the largest fp16 number and the largest weight."""
+    from paged import PrefixPlan
+    g = torch.Generator().manual_seed(5)
+    n, d = 2000, 128
+    q, k = (size * torch.randn(*s, d, generator=g) for s in ((20, 2), (1, n)))
+    v = torch.randn(1, n, d, generator=g)
+    q, k, v = (x.to(dtype) for x in (q, k, v))
+    pools, order = _pools(k, v, 64, 2)
+    out, lse = _run(q, pools, order, n, PrefixPlan([20], [prefix], 2, 1, d, max_length=n))
+    top = (q.double().reshape(40, d) @ k.double()[0].T * d ** -0.5).amax(-1)
+    assert bool(torch.isfinite(out).all()) and float(out.abs().max()) <= 1.01 * float(v.abs().max())
+    e = d * 2.0 ** -23 * d ** -0.5 * (q.double().reshape(40, d).abs() @ k.double()[0].abs().T).amax(-1)
+    assert bool(((lse.reshape(-1) - top).abs() <= 2 * e + math.log(n) + 2.0 ** -22 * top.abs()).all())
