@@ -4,9 +4,11 @@
  * compacting and freeing pages.  No upstream counterpart: upstream keeps one
  * contiguous cache of one sequence (Model/Qwen06B_architecture.py:233-237).
  * All calls are asynchronous on `stream` (a cudaStream_t), neither allocate
- * nor synchronise, can be captured into a CUDA graph, and return 0 or a
- * nonzero code with a message from qwen_b200_last_error()
- * (include/qwen_b200.h); on an error nothing has been launched.
+ * device memory nor synchronise, can be captured into a CUDA graph, and return
+ * 0 or a nonzero code with a message from qwen_b200_last_error()
+ * (include/qwen_b200.h); arguments are checked before the first launch, so
+ * after a refusal nothing has been launched (code 20, a launch that failed,
+ * may come after others).
  */
 #ifndef QWEN_B200_PAGED_H
 #define QWEN_B200_PAGED_H

@@ -377,10 +377,11 @@ __device__ __forceinline__ int v_place(bool dual, int t, int n) {
 // tokens, 123 MB: 28 us, 4.4 TB/s with the queries' start and the results'
 // end; the ring holds 160 KB in flight per SM).  With many rows (64 x 8 rows
 // over 30000 tokens, 126 GFLOP) the softmax: a pair of tiles takes 3650 clocks,
-// of which the tensor cores work 47 %, its 256 x 128 exponentials half of the
-// rest; 113 us, 1.1 PFLOP/s where the products alone would allow 1.66.
-// Measured against it: exponentials half by a polynomial on the FMA pipe 143
-// us in all (140), weights announced at 64 or 96 columns of 128 142, two
+// of which the tensor cores work 53 % and its 256 x 128 exponentials take 2050;
+// 113 us, 1.1 PFLOP/s where the products alone would allow 1.66.
+// Measured against it, in replayed graphs (141 us in all; 160 where the host
+// issues call after call): exponentials half by a polynomial on the FMA pipe 143
+// us (140), weights announced at 64 or 96 columns of 128 142, two
 // threads per query 288 (they do not fit the registers).
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, 1)
