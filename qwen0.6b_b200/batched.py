@@ -23,7 +23,7 @@ import os
 
 import torch
 
-from paged import PrefixPlan, compact_pages, copy_pages, fork_pages, free_pages
+from paged import PrefixPlan, _host_list, _int, compact_pages, copy_pages, fork_pages, free_pages
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 _lib = None
@@ -179,6 +179,8 @@ class PagePool:
         first `length` positions: its full pages are shared, the last, partly
         filled one is a new page of each child.  Returns those pages (-1:
         none)."""
+        parent, length = _int(parent, "parent"), _int(length, "length")
+        children = _host_list(children, "children").tolist()
         full, tail = divmod(length, PAGE)
         if not 0 <= parent < self.num_seqs or not 0 <= length <= self.max_pages * PAGE:
             raise ValueError(f"sequence {parent} / length {length} outside the page table")

@@ -55,3 +55,31 @@ def test_claim_is_reserve_and_unshare(seed):
     for bad in ((5, 0, 0), (0, 0, -1), (0, 0, 6 * PAGE)):
         with pytest.raises(ValueError, match="outside the page table"):
             pp.claim(*bad)
+
+
+@pytest.mark.parametrize("kind", ["list", "numpy", "tensor"])
+def test_fork_takes_integers_of_any_type(kind):
+    """The same child twice is the same child, also as two numbers that are not the same object."""
+    import numpy as np
+    import torch
+    make = {"list": list, "numpy": np.array, "tensor": torch.tensor}[kind]
+    pp = PagePool(num_pages=8, num_seqs=4, max_pages=3)
+    pp.reserve(0, PAGE + 5)
+    before = copy.deepcopy(pp.__dict__)
+    for children in ([1, 1], [1, 0], [2, 4]):
+        with pytest.raises(ValueError):
+            pp.fork(make([0])[0], make(children), make([PAGE + 6])[0])
+        assert pp.__dict__ == before
+    assert pp.fork(make([0])[0], make([3, 1]), make([PAGE + 6])[0]) == [2, 3]
+    assert pp.table == [[0, 1, -1], [0, 3, -1], [-1] * 3, [0, 2, -1]] and pp.refs[:4] == [3, 1, 1, 1]
+    assert all(type(x) is int for row in pp.table for x in row)
+
+
+@pytest.mark.parametrize("args", [(0.0, [1], 5), (0, [1.0], 5), (0, [1], 5.0), (0, [None], 5), (0, 1, 5)])
+def test_fork_refuses_what_is_no_integer(args):
+    pp = PagePool(num_pages=8, num_seqs=4, max_pages=3)
+    pp.reserve(0, PAGE + 5)
+    before = copy.deepcopy(pp.__dict__)
+    with pytest.raises(ValueError):
+        pp.fork(*args)
+    assert pp.__dict__ == before
