@@ -161,12 +161,23 @@ __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatil
 // still be counted in the sum.  Its weights are therefore kept 2^kShift times
 // larger, by a reference m that lies kShift below the maximum at which it was
 // taken: they hold 11 bits down to 2^-(14 + kShift) of that maximum, and what
-// is smaller is off by 2^-(25 + kShift) of it at most.  The reference moves when
-// a score has outgrown it by 2^kLazy more, so weights stay at or below
-// 2^(kShift + kLazy) = 2^15 < 65504 (scores of over 2^22, which are themselves
-// rounded by more than the factor of 2 that is left, saturate).  bf16 has the
-// exponents of fp32 and needs no shift.  Measured: 64 x 8 rows over 30000 tokens 160 us with and
-// without the shift; a shift of 11 and 2^4 to outgrow, 164.
+// is smaller is off by 2^-(25 + kShift) of it at most.  The reference moves at
+// the latest when a score has outgrown it by 2^kLazy more, so weights stay at or
+// below 2^(kShift + kLazy) = 2^15 < 65504 (scores of over 2^22, which are
+// themselves rounded by more than the factor of 2 that is left, saturate).  bf16
+// has the exponents of fp32 and needs no shift.  Measured: 64 x 8 rows over 30000
+// tokens 160 us with and without the shift; a shift of 11 and 2^4 to outgrow, 164.
+//
+// The token at which the reference was taken has the weight 2^kShift, which
+// rounds to itself.  In a row that one token dominates its rounding would be the
+// whole error, so the own kernel's reference is always the maximum, and the
+// prefix kernel's moves to a new maximum that outweighs kShare of what its stream
+// has summed up (error against 64 bits over 250 drawn batches, times that of
+// weights in fp32: 1.58 at most and 1.21 in the median where references moved by
+// 2^8 alone, now 1.26 and 1.09; always moving there, 1.24 and 1.08, but 64 x 8
+// rows 176 us, now 165; weights as a sum of two 16-bit parts 1.00, but 195 us
+// there and 46.7 us for 256 rows behind 2048, now 43.1).
+constexpr float kShare = 0.25f;
 template <typename T>
 struct Type;
 template <>
@@ -367,7 +378,7 @@ __device__ __forceinline__ int v_place(bool dual, int t, int n) {
 //   S_s = Q_s K^T       tcgen05, both operands in shared memory
 //   P_s = 2^(S_s - m)   rounded to the input type over S_s in tensor memory
 //   O_s += P_s V        tcgen05, P from tensor memory, V as it lies (MN-major)
-// The reference m moves only when a row has outgrown it by 2^8, so the output is
+// The reference m hardly moves once the first tiles are through, so the output is
 // hardly ever rescaled.  Warps: 0 copies K and V tiles (a ring of five of 32
 // KB; the pages of the next 32 boxes are looked up ahead), 1 issues every
 // product, 2 waits for tiles on its behalf, 4 to 7 and 8 to 11 are the
@@ -379,9 +390,9 @@ __device__ __forceinline__ int v_place(bool dual, int t, int n) {
 // over 30000 tokens, 126 GFLOP) the softmax: a pair of tiles takes 3650 clocks,
 // of which the tensor cores work 53 % and its 256 x 128 exponentials take 2050;
 // 113 us, 1.1 PFLOP/s where the products alone would allow 1.66.
-// Measured against it, in replayed graphs (141 us in all; 160 where the host
-// issues call after call): exponentials half by a polynomial on the FMA pipe 143
-// us (140), weights announced at 64 or 96 columns of 128 142, two
+// Measured against it, in replayed graphs (then 140 us in all; now 147, and 165
+// where the host issues call after call): exponentials half by a polynomial on
+// the FMA pipe 143 us, weights announced at 64 or 96 columns of 128 142, two
 // threads per query 288 (they do not fit the registers).
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -734,9 +745,10 @@ __global__ void __launch_bounds__(THREADS, 1)
                                  a.scale_log2, -Type<T>::kShift);
           if (i == 0) {
             m = ref;
-          } else if (__any_sync(0xffffffffu, !(ref <= m + Type<T>::kLazy))) {
-            // It moves only when a row has outgrown it by 2^kLazy: the output
-            // is rescaled a few times at most.
+          } else if (__any_sync(0xffffffffu, !(ref <= m + Type<T>::kLazy) ||
+                                                 (ref > m && ex2_approx(ref - m + Type<T>::kShift) > kShare * l))) {
+            // It moves only when a row has outgrown it by 2^kLazy or to a token
+            // that weighs: the output is rescaled a few times at most.
             const float mn = max3(m, ref, ref);
             const float f = mn == -INFINITY ? 1.f : ex2_approx(m - mn);
             m = mn;
@@ -1037,8 +1049,7 @@ __device__ __forceinline__ void put_result(const Args &a, int row, int head, int
 // registers, a block's K is replaced as soon as it has been multiplied, its V
 // likewise; fragments are loaded as 8 x 8 matrices, V transposed on the way
 // (its 16-byte chunks are exchanged by the token's number, so that no read has
-// bank conflicts); the reference moves only when a column has outgrown it by 2^8,
-// as in the prefix kernel.  Measured: 256 rows of up to 256 own tokens, 142 MB,
+// bank conflicts).  Measured: 256 rows of up to 256 own tokens, 142 MB,
 // 36 us beside the prefix kernel (4 TB/s); 112 rows of 1000 with no prefix 74
 // us (6.2 TB/s, 0.95 of a copy's rate).
 // With one split the CTA also joins the prefix's partial results and writes the
@@ -1244,7 +1255,7 @@ __global__ void __launch_bounds__(32 * W, kOwnPerSm<W>) own_kernel(const Args a)
       mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 8));
       mx[h] = fmaf(fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 16)), a.scale_log2, -Type<T>::kShift);
     }
-    if (__any_sync(0xffffffffu, mx[0] > m[0] + Type<T>::kLazy || mx[1] > m[1] + Type<T>::kLazy)) {
+    if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float mn = fmaxf(m[h], mx[h]);

@@ -157,3 +157,50 @@ def test_large_finite_scores_stay_finite(dtype, prefix, size):
     assert bool(torch.isfinite(out).all()) and float(out.abs().max()) <= 1.01 * float(v.abs().max())
     e = d * 2.0 ** -23 * d ** -0.5 * (q.double().reshape(40, d).abs() @ k.double()[0].abs().T).amax(-1)
     assert bool(((lse.reshape(-1) - top).abs() <= 2 * e + math.log(n) + 2.0 ** -22 * top.abs()).all())
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim,kv,n,prefix,longest", [
+    (128, 8, 8000, 7936, 8000),    # the prefix kernel, several tiles to a part
+    (64, 8, 12000, 11904, 12000),
+    (128, 1, 450, 0, 450),         # the own kernel alone
+    (64, 2, 3000, 0, 3000),        # its splits
+    (64, 2, 1900, 640, 4000),      # all three kernels
+])
+@pytest.mark.parametrize("at", [300, 449, 1500, 4000, 6677, -1])
+@pytest.mark.parametrize("rows", [3, 90])
+def test_a_dominant_token_is_not_rounded(dtype, dim, kv, n, prefix, longest, at, rows):
+    """One token has most of the weight, between two steps of the input type as
+    seen from the largest scores before it, which lie 2.2 to 5.2 lower.  The
+    result may be off by the roundings of the other weights, u w each, and its
+    own (and by 2^-23 of what has been added at each of n / 16 steps of the
+    products)."""
+    from paged import PrefixPlan
+    g = torch.Generator().manual_seed(6)
+    at = at % n
+    before = [at - x for x in (16, 32, 64, 128, 256, 384) if x <= at]
+    k = 0.01 * torch.randn(kv, n, dim, generator=g)
+    k[..., :2] = 0.0
+    k[:, before + [at]] = 0.0
+    k[:, at, 0], k[:, before, 1] = 8.0, 8.0
+    v = torch.randn(kv, n, dim, generator=g)
+    q = 0.05 * torch.randn(rows, 2 * kv, dim, generator=g)
+    q[..., 0] = 14.0 / 8.0 * dim ** 0.5
+    q[..., 1] = ((14.0 - torch.linspace(2.2, 5.2, 2 * kv * rows)) / 8.0 * dim ** 0.5).view(rows, 2 * kv)
+    q, k, v = (x.to(dtype) for x in (q, k, v))
+    pools, order = _pools(k, v, 128, 3)
+    out, _ = _run(q, pools, order, n, PrefixPlan([rows], [prefix], 2 * kv, kv, dim, max_length=longest))
+    qd, kd, vd = (x.double().cuda() for x in (q.view(rows, kv, 2, dim).transpose(0, 1).reshape(kv, -1, dim), k, v))
+    w = torch.softmax(qd @ kd.mT * dim ** -0.5, -1)
+    ref = w @ vd
+    e = dim * 2.0 ** -23 * dim ** -0.5 * (qd.abs() @ kd.abs().mT)
+    u = torch.finfo(dtype).eps / 2
+    others = w.clone()
+    others[..., at] = 0.0
+    off = u * others + w * (e + e.amax(-1, keepdim=True) + 2.0 ** -19 + n / 16 * 2.0 ** -23)
+    off += FLOOR[dtype] * w.amax(-1, keepdim=True)
+    bound = off @ vd.abs() + u * ref.abs() + 2.0 ** -25
+    err = (out.view(rows, kv, 2, dim).transpose(0, 1).reshape(kv, -1, dim).cuda() - ref).abs()
+    heavy = w[..., at] > 0.5
+    assert bool(heavy.any())
+    assert bool((err <= bound)[heavy].all()), f"{float((err / bound)[heavy].max())} times the bound"
