@@ -172,12 +172,14 @@ __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatil
 // rounds to itself.  In a row that one token dominates its rounding would be the
 // whole error, so the own kernel's reference is always the maximum, and the
 // prefix kernel's moves to a new maximum that outweighs kShare of what its stream
-// has summed up (error against 64 bits over 250 drawn batches, times that of
-// weights in fp32: 1.58 at most and 1.21 in the median where references moved by
-// 2^8 alone, now 1.26 and 1.09; always moving there, 1.24 and 1.08, but 64 x 8
-// rows 176 us, now 165; weights as a sum of two 16-bit parts 1.00, but 195 us
-// there and 46.7 us for 256 rows behind 2048, now 43.1).
-constexpr float kShare = 0.25f;
+// has summed up.  Error against 64 bits over 250 drawn batches, times that of
+// weights in fp32, and the time of 64 x 8 rows:
+//   moved by 2^8 alone           1.58 at most, 1.21 in the median   160 us
+//   kShare = 1, 1/2, 1/4         1.35, 1.31, 1.26; 1.09             161, 162, 165
+//   always the maximum           1.24; 1.08                         176
+//   weights in two 16-bit parts  1.00; 1.00                         195
+// (256 rows behind 2048 tokens: 41.6, 42.9, 43.2, 43.3, 43.0, 46.7).
+constexpr float kShare = 0.5f;
 template <typename T>
 struct Type;
 template <>
@@ -387,10 +389,10 @@ __device__ __forceinline__ int v_place(bool dual, int t, int n) {
 // What bounds it: with few rows the bytes of K and V (13 rows over 60000
 // tokens, 123 MB: 28 us, 4.4 TB/s with the queries' start and the results'
 // end; the ring holds 160 KB in flight per SM).  With many rows (64 x 8 rows
-// over 30000 tokens, 126 GFLOP) the softmax: a pair of tiles takes 3650 clocks,
-// of which the tensor cores work 53 % and its 256 x 128 exponentials take 2050;
-// 113 us, 1.1 PFLOP/s where the products alone would allow 1.66.
-// Measured against it, in replayed graphs (then 140 us in all; now 147, and 165
+// over 30000 tokens, 126 GFLOP) the softmax: a pair of tiles takes 3750 clocks,
+// of which the tensor cores work 51 % and its 256 x 128 exponentials take 2050;
+// 116 us, 1.1 PFLOP/s where the products alone would allow 1.66.
+// Measured against it, in replayed graphs (then 140 us in all; now 144, and 162
 // where the host issues call after call): exponentials half by a polynomial on
 // the FMA pipe 143 us, weights announced at 64 or 96 columns of 128 142, two
 // threads per query 288 (they do not fit the registers).
